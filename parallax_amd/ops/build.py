@@ -31,7 +31,10 @@ def build(verbose=True):
         sources=sources,
         extra_include_paths=[CSRC],
         extra_cflags=['-O3'],
-        extra_cuda_cflags=['-O3'],
+        # packed fp32 arithmetic (two floats an instruction) is left out of
+        # the generated code: some of its forms have given wrong results
+        extra_cuda_cflags=['-O3', '-Xclang', '-target-feature', '-Xclang',
+                           '-packed-fp32-ops'],
         build_directory=LIB_DIR,
         verbose=verbose,
         with_cuda=True,
