@@ -532,7 +532,15 @@ void multi_tensor_momentum(std::vector<at::Tensor> params,
                            std::vector<at::Tensor> masters) {
   check_contig(params, "mt_momentum");
   check_same_layout(params, grads, "mt_momentum");
-  check_same_layout(params, bufs, "mt_momentum");
+  // the momentum buffers are fp32 whatever the params' type
+  TORCH_CHECK(params.size() == bufs.size(),
+              "mt_momentum: list size mismatch");
+  for (size_t i = 0; i < bufs.size(); ++i) {
+    TORCH_CHECK(bufs[i].scalar_type() == at::kFloat &&
+                    same_dense_layout(params[i], bufs[i]),
+                "mt_momentum: buffer ", i, " must be fp32 with the param's "
+                "layout");
+  }
   check_masters(params, masters, "mt_momentum");
   mt_launch(params, grads, bufs, {}, {},
             MomentumOp{(float)lr, (float)mom, (float)wd, nesterov},
