@@ -1509,9 +1509,11 @@ void px_wgrad3x3_kernel(const ushort* __restrict__ DY,  // [M, Cout]
       const int mm = idx & 63;
       const int cg = (idx >> 6) * 8;
       const long m = m0 + mm;
-      uint2 dv, xv;
+      uint4 dv = {0u, 0u, 0u, 0u}, xv = {0u, 0u, 0u, 0u};
       if (m < M) {
-        dv = *reinterpret_cast<const uint2*>(&DY[m * Cout + co0 + cg]);
+        if (co0 + cg < Cout) {
+          dv = *reinterpret_cast<const uint4*>(&DY[m * Cout + co0 + cg]);
+        }
         const long n_img = m / ((long)OH * OW);
         const long rem = m - n_img * ((long)OH * OW);
         const int oy = (int)(rem / OW);
@@ -1519,15 +1521,12 @@ void px_wgrad3x3_kernel(const ushort* __restrict__ DY,  // [M, Cout]
         const ushort* src = XP +
             (((n_img * HP) + (long)oy * stride + tdy) * WP +
              (long)ox * stride + tdx) * Cin + ci0 + cg;
-        xv = *reinterpret_cast<const uint2*>(src);
-      } else {
-        dv.x = dv.y = 0u;
-        xv.x = xv.y = 0u;
+        xv = *reinterpret_cast<const uint4*>(src);
       }
       const ushort* de = reinterpret_cast<const ushort*>(&dv);
       const ushort* xe = reinterpret_cast<const ushort*>(&xv);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         dyT[(cg + j) * WG_LDP + mm] = de[j];
         xT[(cg + j) * WG_LDP + mm] = xe[j];
       }
