@@ -79,6 +79,7 @@ from parallax_amd.ops.embedding import (ParallaxEmbedding,
                                         embedding_lookup)
 from parallax_amd.ops.layernorm import layer_norm, ParallaxLayerNorm
 from parallax_amd.ops.softmax_ce import softmax_cross_entropy
+from parallax_amd.ops.linear_ce import linear_cross_entropy
 from parallax_amd.ops.lstm import lstm_cell, ParallaxLSTM
 from parallax_amd.ops.sampled_softmax import sampled_softmax_loss
 from parallax_amd.ops.misc import (clip_by_global_norm, global_norm,

@@ -150,6 +150,20 @@ std::vector<at::Tensor> sampled_ce_bwd(const at::Tensor& true_logits,
                                        const at::Tensor& lse,
                                        const at::Tensor& dloss);
 
+// linear_ce.hip
+std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
+                                      const at::Tensor& w,
+                                      const c10::optional<at::Tensor>& bias,
+                                      const at::Tensor& labels,
+                                      int64_t ignore, double smoothing,
+                                      int64_t reduction);
+std::vector<at::Tensor> linear_ce_bwd(
+    const at::Tensor& dloss, const at::Tensor& x, const at::Tensor& w,
+    const c10::optional<at::Tensor>& bias, const at::Tensor& labels,
+    const at::Tensor& lse, const at::Tensor& count, const at::Tensor& tops,
+    int64_t ignore, double smoothing, int64_t reduction, bool want_dx,
+    bool want_dw, bool want_db);
+
 // lstm_cell.hip
 std::vector<at::Tensor> lstm_gates_fwd(const at::Tensor& gates,
                                        const at::Tensor& c_prev,
@@ -243,6 +257,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("softmax_ce_bwd", &softmax_ce_bwd);
   m.def("sampled_ce_fwd", &sampled_ce_fwd);
   m.def("sampled_ce_bwd", &sampled_ce_bwd);
+  m.def("linear_ce_fwd", &linear_ce_fwd,
+        "softmax CE of a projection onto a vocabulary, logits not kept");
+  m.def("linear_ce_bwd", &linear_ce_bwd);
   m.def("lstm_gates_fwd", &lstm_gates_fwd);
   m.def("lstm_gates_bwd", &lstm_gates_bwd);
   m.def("lstm_gates_fwd_out", &lstm_gates_fwd_out);

@@ -1,0 +1,119 @@
+"""Softmax cross entropy of a projection onto a large vocabulary.
+
+``linear_cross_entropy(inputs, weight, bias, labels)`` is
+``softmax_cross_entropy(inputs @ weight.t() + bias, labels)`` without the
+[N, V] logits: for LM1B's 793,470 words and 2,560 tokens they would take
+8.1 GB in fp32.  Beside the sampled softmax it gives the exact loss, for
+held-out perplexity and for training on the whole vocabulary.
+
+GPU: hand-written MFMA kernels (ops/hip/csrc/linear_ce.hip); the backward
+computes the logits again, piece by piece of the vocabulary.  CPU: torch
+reference, which does keep them.
+"""
+
+import torch
+
+from parallax_amd import ops as _ops
+
+_REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
+
+
+class _LinearCEFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, labels, ignore_index, smoothing,
+                reduction):
+        loss, lse, total, tops = _ops.ext().linear_ce_fwd(
+            x, weight, bias, labels, ignore_index, smoothing, reduction)
+        ctx.save_for_backward(x, weight, bias, labels, lse, total, tops)
+        ctx.args = (ignore_index, smoothing, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, weight, bias, labels, lse, total, tops = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        dx, dw, db = _ops.ext().linear_ce_bwd(
+            dloss.float().contiguous(), x, weight, bias, labels, lse, total,
+            tops, *ctx.args, want[0], want[1],
+            bias is not None and want[2])
+        return dx, dw, db, None, None, None, None
+
+
+def _check(inputs, weight, bias, labels, label_smoothing, reduction):
+    if reduction not in _REDUCTIONS:
+        raise ValueError("linear_cross_entropy: reduction is 'mean', 'sum' "
+                         "or 'none', got %r" % (reduction,))
+    if not 0.0 <= label_smoothing < 1.0:
+        raise ValueError('linear_cross_entropy: label_smoothing in [0, 1) '
+                         'expected, got %r' % (label_smoothing,))
+    if weight.dim() != 2 or inputs.dim() < 2 \
+            or inputs.shape[-1] != weight.shape[1]:
+        raise ValueError('linear_cross_entropy: inputs [..., D] and weight '
+                         '[V, D] expected, got %s and %s'
+                         % (tuple(inputs.shape), tuple(weight.shape)))
+    if labels.shape != inputs.shape[:-1]:
+        raise ValueError('linear_cross_entropy: labels %s expected, got %s'
+                         % (tuple(inputs.shape[:-1]), tuple(labels.shape)))
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError('linear_cross_entropy: bias %s expected, got %s'
+                         % (tuple(weight.shape[:1]), tuple(bias.shape)))
+    for t, name in ((inputs, 'inputs'), (weight, 'weight'), (bias, 'bias')):
+        if t is not None and not t.is_floating_point():
+            raise TypeError('linear_cross_entropy: %s of type %s'
+                            % (name, t.dtype))
+    if labels.is_floating_point() or labels.dtype == torch.bool:
+        raise TypeError('linear_cross_entropy: labels of type %s'
+                        % labels.dtype)
+
+
+def _plain(x, weight, bias, labels, ignore_index, smoothing, reduction):
+    logits = x.float() @ weight.float().t()
+    if bias is not None:
+        logits = logits + bias.float()
+    # labels outside the vocabulary go to its nearest end, as on the GPU
+    live = labels != ignore_index
+    y = torch.where(live, labels.clamp(0, weight.shape[0] - 1), 0)
+    lse = torch.logsumexp(logits, 1)
+    losses = lse - (1 - smoothing) * logits.gather(1, y[:, None])[:, 0]
+    if smoothing:
+        losses = losses - smoothing * logits.mean(1)
+    losses = torch.where(live, losses, torch.zeros_like(losses))
+    if reduction == 'none':
+        return losses
+    total = losses.sum()
+    return total / live.sum() if reduction == 'mean' else total
+
+
+def linear_cross_entropy(inputs, weight, bias, labels, reduction='mean',
+                         ignore_index=-100, label_smoothing=0.0):
+    """loss[i] = lse_i - (1 - e) z_i[labels_i] - e mean_v z_i[v] with
+    z = inputs @ weight.t() + bias and e = label_smoothing.
+
+    inputs [..., D], weight [V, D], bias [V] or None, labels [...] integer.
+    Rows whose label is ``ignore_index`` have no loss and no gradient, and
+    their inputs are not read; other labels are clamped to the vocabulary.
+    'mean' is over the rows that count (NaN where none does).  The loss is
+    fp32: a scalar, or the shape of ``labels`` for 'none'.  ``weight`` is
+    cast to the type of ``inputs`` where the two differ.
+    """
+    _check(inputs, weight, bias, labels, label_smoothing, reduction)
+    x = inputs.reshape(-1, inputs.shape[-1])
+    y = labels.reshape(-1).long()
+    if weight.dtype != x.dtype:
+        weight = weight.to(x.dtype)
+    if x.shape[0] == 0:  # no rows: what a sum over nothing is
+        z = (x.float().sum() + weight.float().sum() * 0) * 0
+        if bias is not None:
+            z = z + bias.float().sum() * 0
+        if reduction == 'none':
+            return x.float().sum(-1).reshape(labels.shape)
+        return z / 0 if reduction == 'mean' else z
+    if _ops.use_native(x):
+        losses = _LinearCEFn.apply(x, weight, bias, y.contiguous(),
+                                   ignore_index, float(label_smoothing),
+                                   _REDUCTIONS[reduction])
+    else:
+        losses = _plain(x, weight, bias, y, ignore_index, label_smoothing,
+                        reduction)
+    return losses.view(labels.shape) if reduction == 'none' else losses
