@@ -57,6 +57,15 @@ void multi_tensor_pack(std::vector<at::Tensor> tensors, at::Tensor flat);
 void multi_tensor_unpack(std::vector<at::Tensor> tensors, at::Tensor flat,
                          double scale);
 
+void multi_tensor_muon_update(std::vector<at::Tensor> grads,
+                              std::vector<at::Tensor> bufs,
+                              std::vector<at::Tensor> updates, double mom,
+                              bool nesterov);
+void multi_tensor_muon_apply(std::vector<at::Tensor> params,
+                             std::vector<at::Tensor> updates,
+                             std::vector<double> scales, double decay,
+                             std::vector<at::Tensor> masters);
+
 // gru_cell.hip
 std::vector<at::Tensor> gru_gates_fwd(const at::Tensor& xg,
                                       const at::Tensor& hg,
@@ -164,6 +173,10 @@ std::vector<at::Tensor> linear_ce_bwd(
     int64_t ignore, double smoothing, int64_t reduction, bool want_dx,
     bool want_dw, bool want_db);
 
+// newton_schulz.hip
+void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
+                   double a, double b, double c, double eps, bool exact);
+
 // lstm_cell.hip
 std::vector<at::Tensor> lstm_gates_fwd(const at::Tensor& gates,
                                        const at::Tensor& c_prev,
@@ -260,6 +273,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_ce_fwd", &linear_ce_fwd,
         "softmax CE of a projection onto a vocabulary, logits not kept");
   m.def("linear_ce_bwd", &linear_ce_bwd);
+  m.def("newton_schulz", &newton_schulz,
+        "Newton-Schulz orthogonalisation of a batch of matrices");
+  m.def("multi_tensor_muon_update", &multi_tensor_muon_update);
+  m.def("multi_tensor_muon_apply", &multi_tensor_muon_apply);
   m.def("lstm_gates_fwd", &lstm_gates_fwd);
   m.def("lstm_gates_bwd", &lstm_gates_bwd);
   m.def("lstm_gates_fwd_out", &lstm_gates_fwd_out);

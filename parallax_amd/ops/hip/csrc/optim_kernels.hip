@@ -212,6 +212,58 @@ struct MomentumOp {
   }
 };
 
+// a: gradients, c: momentum buffers, d: updates (both fp32)
+struct MuonUpdateOp {
+  static constexpr bool vec = true;
+  float mom;
+  bool nesterov;
+  template <typename T>
+  __device__ void apply(const MTMeta& m, int ti, long j) const {
+    const float g = to_f32<T>(reinterpret_cast<const T*>(m.a[ti])[j]);
+    float* buf = reinterpret_cast<float*>(m.c[ti]);
+    const float b = mom * buf[j] + g;
+    buf[j] = b;
+    reinterpret_cast<float*>(m.d[ti])[j] = nesterov ? g + mom * b : b;
+  }
+  template <typename T>
+  __device__ void apply4(const MTMeta& m, int ti, long j) const {
+    float* buf = reinterpret_cast<float*>(m.c[ti]);
+    const V4<T> g = ld4(reinterpret_cast<const T*>(m.a[ti]), j);
+    V4<float> b = ld4(buf, j), u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float gv = to_f32<T>(g.v[k]);
+      b.v[k] = mom * b.v[k] + gv;
+      u.v[k] = nesterov ? gv + mom * b.v[k] : b.v[k];
+    }
+    st4(buf, j, b);
+    st4(reinterpret_cast<float*>(m.d[ti]), j, u);
+  }
+};
+
+// a: parameters (f: their fp32 masters), c: orthogonal updates (fp32),
+// e: learning rate of each
+struct MuonApplyOp {
+  static constexpr bool vec = true;
+  float decay;
+  template <typename T>
+  __device__ void apply(const MTMeta& m, int ti, long j) const {
+    T* p = reinterpret_cast<T*>(m.a[ti]);
+    const float o = reinterpret_cast<const float*>(m.c[ti])[j];
+    stp(m, ti, j, p, ldp(m, ti, j, p) * decay - m.e[ti] * o);
+  }
+  template <typename T>
+  __device__ void apply4(const MTMeta& m, int ti, long j) const {
+    T* p = reinterpret_cast<T*>(m.a[ti]);
+    const V4<float> o = ld4(reinterpret_cast<const float*>(m.c[ti]), j);
+    float pw[4];
+    ldp4(m, ti, j, p, pw);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) pw[k] = pw[k] * decay - m.e[ti] * o.v[k];
+    stp4(m, ti, j, p, pw);
+  }
+};
+
 struct AdagradOp {
   static constexpr bool vec = true;
   float lr, eps;
@@ -615,6 +667,46 @@ void multi_tensor_ema(std::vector<at::Tensor> shadows,
                       std::vector<at::Tensor> values, double decay) {
   check_contig(shadows, "mt_ema");
   mt_launch(shadows, values, {}, {}, {}, EMAOp{(float)decay});
+}
+
+static void check_fp32_state(const std::vector<at::Tensor>& a,
+                             const std::vector<at::Tensor>& state,
+                             const char* name) {
+  TORCH_CHECK(a.size() == state.size(), name, ": list size mismatch");
+  for (size_t i = 0; i < a.size(); ++i) {
+    TORCH_CHECK(state[i].scalar_type() == at::kFloat &&
+                    state[i].numel() == a[i].numel() &&
+                    state[i].is_non_overlapping_and_dense() &&
+                    state[i].device() == a[i].device(),
+                name, ": fp32 state ", i, " with the tensor's numel expected");
+  }
+}
+
+// Muon, before the products: buf = mom buf + g and the update that is to be
+// made orthogonal, written behind one another for the batched products.
+void multi_tensor_muon_update(std::vector<at::Tensor> grads,
+                              std::vector<at::Tensor> bufs,
+                              std::vector<at::Tensor> updates, double mom,
+                              bool nesterov) {
+  check_contig(grads, "mt_muon_update");
+  check_fp32_state(grads, bufs, "mt_muon_update");
+  check_fp32_state(grads, updates, "mt_muon_update");
+  mt_launch(grads, {}, bufs, updates, {},
+            MuonUpdateOp{(float)mom, nesterov});
+}
+
+// Muon, after them: w = decay w - scale O
+void multi_tensor_muon_apply(std::vector<at::Tensor> params,
+                             std::vector<at::Tensor> updates,
+                             std::vector<double> scales, double decay,
+                             std::vector<at::Tensor> masters) {
+  check_contig(params, "mt_muon_apply");
+  check_fp32_state(params, updates, "mt_muon_apply");
+  check_masters(params, masters, "mt_muon_apply");
+  TORCH_CHECK(scales.size() == params.size(),
+              "mt_muon_apply: list size mismatch");
+  std::vector<float> e(scales.begin(), scales.end());
+  mt_launch(params, {}, updates, {}, e, MuonApplyOp{(float)decay}, masters);
 }
 
 // Fused zero of a tensor list (one launch per 32 tensors) — replaces the

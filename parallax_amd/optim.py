@@ -330,8 +330,11 @@ class Adam(ParallaxOptimizer):
         self._dev_step_params = set()
 
     def _dense_step(self, params, grads, group):
-        lr, (b1, b2), eps = group['lr'], group['betas'], group['eps']
-        wd = group['weight_decay']
+        self._adam_step(params, grads, group, group['lr'],
+                        group['weight_decay'])
+
+    def _adam_step(self, params, grads, group, lr, wd):
+        (b1, b2), eps = group['betas'], group['eps']
         ms, vs, steps = [], [], []
         for p in params:
             st = self._state(p)
@@ -451,3 +454,144 @@ class RMSProp(ParallaxOptimizer):
         sq.index_copy_(0, ids, sq_rows)
         upd = (g32 / (sq_rows.sqrt() + eps)).to(param.dtype)
         param.index_add_(0, ids, upd, alpha=-lr)
+
+
+def _same_layout(p, g):
+    return g.shape == p.shape and all(
+        n <= 1 or s == t for n, s, t in zip(p.shape, p.stride(), g.stride()))
+
+
+def _is_dense(p):
+    """The strides of a permuted contiguous tensor."""
+    step = 1
+    for s, n in sorted((s, n) for s, n in zip(p.stride(), p.shape) if n > 1):
+        if s != step:
+            return False
+        step *= n
+    return True
+
+
+def _storage_matrix(p):
+    """(rows, cols) of a parameter's storage read as one matrix: a matrix or
+    its transpose, a convolution's [out, everything else].  Newton-Schulz
+    products commute with a transposition and with an order of the columns,
+    so the storage is swept as it lies."""
+    rows, n = p.shape[0], p.numel()
+    if p.is_contiguous() or (_is_dense(p) and p.stride(0) * rows == n):
+        return rows, n // max(rows, 1)
+    if p.dim() == 2 and p.t().is_contiguous():
+        return p.shape[1], p.shape[0]
+    raise ValueError('Muon: parameter of shape %s and strides %s does not '
+                     'lie as a matrix' % (tuple(p.shape), p.stride()))
+
+
+class Muon(Adam):
+    """Momentum whose update is made orthogonal (ops.newton_schulz):
+
+        buf = momentum buf + g,  u = g + momentum buf  (nesterov)
+        w  <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) NS(u)
+
+    for the matrices: parameters of two or more dimensions (a convolution
+    is [out, in kh kw]) in groups with ``muon=True``.  Vectors, sparse rows
+    and groups with ``muon=False`` (embeddings, heads) take Adam with
+    ``adam_lr`` and no weight decay.  Matrices of one size go through the
+    products as one batch.  fp32 parameters get products in 22 bits, bf16
+    ones with fp32 masters what bf16's rounding can show."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True,
+                 weight_decay=0.0, ns_steps=5, muon=True, adam_lr=3e-4,
+                 betas=(0.9, 0.95), eps=1e-8):
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError('Muon: momentum in [0, 1) expected, got %r'
+                             % (momentum,))
+        if int(ns_steps) != ns_steps or not 1 <= ns_steps <= 64:
+            raise ValueError('Muon: 1 to 64 ns_steps expected, got %r'
+                             % (ns_steps,))
+        super().__init__(params, lr=lr, betas=betas, eps=eps,
+                         weight_decay=weight_decay)
+        extra = dict(momentum=momentum, nesterov=nesterov,
+                     ns_steps=int(ns_steps), muon=muon, adam_lr=adam_lr)
+        for k, v in extra.items():
+            self.defaults[k] = v
+            for group in self.param_groups:
+                group.setdefault(k, v)
+
+    def _dense_step(self, params, grads, group):
+        mats, rest = [], []
+        for p, g in zip(params, grads):
+            if group['muon'] and p.dim() >= 2:
+                mats.append((p, g))
+            else:
+                rest.append((p, g))
+        if rest:
+            self._adam_step([p for p, _ in rest], [g for _, g in rest],
+                            group, group['adam_lr'], 0.0)
+        # one batch for each size, type and device
+        batches = {}
+        for p, g in mats:
+            if p.numel():
+                key = (tuple(sorted(_storage_matrix(p))), p.dtype, p.device)
+                batches.setdefault(key, []).append((p, g))
+        for batch in batches.values():
+            self._muon_step([p for p, _ in batch], [g for _, g in batch],
+                            group)
+
+    def _muon_step(self, params, grads, group):
+        from parallax_amd.ops.newton_schulz import COEFFICIENTS, _into
+        lr, mom = group['lr'], group['momentum']
+        decay = 1.0 - lr * group['weight_decay']
+        bufs = []
+        for p in params:
+            st = self.state[p]
+            if 'momentum_buffer' not in st:
+                st['momentum_buffer'] = torch.zeros_like(
+                    p, dtype=torch.float32)
+            elif not _same_layout(p, st['momentum_buffer']):
+                raise ValueError('Muon: momentum buffer of shape %s for a '
+                                 'parameter of shape %s, or of other strides'
+                                 % (tuple(st['momentum_buffer'].shape),
+                                    tuple(p.shape)))
+            bufs.append(st['momentum_buffer'])
+        masters, has_m = self._ensure_masters(params)
+        scales = [lr * max(1.0, p.shape[0] / (p.numel() // p.shape[0])) ** 0.5
+                  for p in params]
+        shapes = [_storage_matrix(p) for p in params]
+        exact = params[0].dtype != torch.bfloat16
+        # tall and wide ones of one size: a stack for each
+        for shape in dict.fromkeys(shapes):
+            ii = [i for i, s in enumerate(shapes) if s == shape]
+            ps, gs, bs = ([t[i] for i in ii] for t in (params, grads, bufs))
+            ms = [masters[i] for i in ii] if has_m else []
+            sc = [scales[i] for i in ii]
+            if not _use_native(ps):
+                for k, (p, g, b) in enumerate(zip(ps, gs, bs)):
+                    g = g.to(b.dtype)
+                    b.mul_(mom).add_(g)
+                    v = g.add(b, alpha=mom) if group['nesterov'] else b
+                    o = v.reshape(1, p.shape[0], -1).clone()
+                    _into(o, o, group['ns_steps'], COEFFICIENTS, 1e-7, exact)
+                    w = ms[k] if ms else p
+                    w.mul_(decay).add_(o.view(p.shape).to(w.dtype),
+                                       alpha=-sc[k])
+                    if w is not p:
+                        p.copy_(w)
+                continue
+            e = _ops.ext()
+            gs = [g if _same_layout(p, g)
+                  else torch.empty_like(p, dtype=g.dtype).copy_(g)
+                  for p, g in zip(ps, gs)]
+            u = torch.empty((len(ii),) + shape, dtype=torch.float32,
+                            device=ps[0].device)
+            us = list(u.unbind(0))
+            for gg, bb, uu in _dtype_groups(gs, bs, us):
+                e.multi_tensor_muon_update(gg, bb, uu, mom,
+                                           group['nesterov'])
+            _into(u, u, group['ns_steps'], COEFFICIENTS, 1e-7, exact)
+            e.multi_tensor_muon_apply(ps, us, sc, decay, ms)
+
+    @torch.no_grad()
+    def sparse_row_step(self, param, ids, grad_rows, group=None,
+                        nvalid=None):
+        group = group or self.group_of(param)
+        super().sparse_row_step(param, ids, grad_rows,
+                                dict(group, lr=group['adam_lr']), nvalid)
