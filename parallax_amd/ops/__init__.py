@@ -83,6 +83,8 @@ from parallax_amd.ops.linear_ce import linear_cross_entropy
 from parallax_amd.ops.lstm import lstm_cell, ParallaxLSTM
 from parallax_amd.ops.sampled_softmax import sampled_softmax_loss
 from parallax_amd.ops.newton_schulz import newton_schulz
+from parallax_amd.ops.rotary import (apply_rotary, rotary_tables,
+                                     ParallaxRotary)
 from parallax_amd.ops.misc import (clip_by_global_norm, global_norm,
                                    ema_update)
 from parallax_amd.ops.linear import PxLinear

@@ -177,6 +177,13 @@ std::vector<at::Tensor> linear_ce_bwd(
 void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
                    double a, double b, double c, double eps, bool exact);
 
+// rotary.hip
+std::vector<at::Tensor> rotary(const at::Tensor& q,
+                               const c10::optional<at::Tensor>& k,
+                               const at::Tensor& cos, const at::Tensor& sin,
+                               const c10::optional<at::Tensor>& positions,
+                               int64_t offset, bool interleaved, bool back);
+
 // lstm_cell.hip
 std::vector<at::Tensor> lstm_gates_fwd(const at::Tensor& gates,
                                        const at::Tensor& c_prev,
@@ -277,6 +284,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Newton-Schulz orthogonalisation of a batch of matrices");
   m.def("multi_tensor_muon_update", &multi_tensor_muon_update);
   m.def("multi_tensor_muon_apply", &multi_tensor_muon_apply);
+  m.def("rotary", &rotary, "rotary positions of queries and keys");
   m.def("lstm_gates_fwd", &lstm_gates_fwd);
   m.def("lstm_gates_bwd", &lstm_gates_bwd);
   m.def("lstm_gates_fwd_out", &lstm_gates_fwd_out);
