@@ -26,6 +26,7 @@ import torch
 
 import data_utils
 from parallax_amd.models.lm1b import LM1BModel
+from parallax_amd.ops import linear_cross_entropy
 
 
 @torch.no_grad()
@@ -48,10 +49,8 @@ def evaluate_perplexity(model, dataset, batch_size=16, num_steps=20,
         if emb.dtype != body:
             emb = emb.to(body)
         hs, state = model.lstm(emb, state)
-        logits = (hs.reshape(-1, hs.shape[-1]).float()
-                  @ w_full.t().float() + b_full.float())
-        nll = torch.nn.functional.cross_entropy(
-            logits, y.reshape(-1), reduction='sum')
+        nll = linear_cross_entropy(hs.float(), w_full, b_full, y,
+                                   reduction='sum')
         tot_nll += float(nll)
         tot_tok += y.numel()
         # detach the carried state between windows

@@ -38,6 +38,14 @@ def main():
     ap.add_argument('--heads', type=int, default=8)
     ap.add_argument('--ffn', type=int, default=2048)
     ap.add_argument('--layers', type=int, default=6)
+    ap.add_argument('--optimizer', default='adam',
+                    choices=['adam', 'muon'])
+    ap.add_argument('--positions', default='learned',
+                    choices=['learned', 'rotary'])
+    ap.add_argument('--softmax', default='sampled',
+                    choices=['sampled', 'full'])
+    ap.add_argument('--label_smoothing', type=float, default=0.0,
+                    help='with --softmax full')
     ap.add_argument('--run_option', default='HYBRID')
     ap.add_argument('--ckpt_dir', default=None)
     ap.add_argument('--save_ckpt_steps', type=int, default=None)
@@ -47,7 +55,10 @@ def main():
 
     examples = sv = tv = None
     graph_kw = dict(d_model=args.d_model, heads=args.heads, ffn=args.ffn,
-                    enc_layers=args.layers, dec_layers=args.layers)
+                    enc_layers=args.layers, dec_layers=args.layers,
+                    optimizer=args.optimizer, positions=args.positions,
+                    softmax=args.softmax,
+                    label_smoothing=args.label_smoothing)
     if args.src:
         from utils import iterator_utils, vocab_utils
         with open(args.src) as f:

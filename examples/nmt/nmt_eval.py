@@ -38,6 +38,11 @@ def main():
     ap.add_argument('--d-model', type=int, default=64)
     ap.add_argument('--heads', type=int, default=4)
     ap.add_argument('--ffn', type=int, default=128)
+    ap.add_argument('--positions', default='learned',
+                    choices=['learned', 'rotary'])
+    ap.add_argument('--softmax', default='sampled',
+                    choices=['sampled', 'full'],
+                    help='as the checkpoint was trained')
     ap.add_argument('--beam-width', type=int, default=0,
                     help='0 = greedy (reference nmt.py beam_width flag)')
     ap.add_argument('--length-penalty', type=float, default=0.0)
@@ -69,7 +74,8 @@ def main():
         model = NMTTransformer(
             src_vocab=len(sv), tgt_vocab=len(tv), d_model=args.d_model,
             heads=args.heads, ffn=args.ffn, enc_layers=args.layers,
-            dec_layers=args.layers, min_partitions=2)
+            dec_layers=args.layers, min_partitions=2,
+            positions=args.positions, softmax=args.softmax)
     if args.ckpt:
         from parallax_amd.checkpoint import latest_checkpoint
         state = torch.load(latest_checkpoint(args.ckpt),

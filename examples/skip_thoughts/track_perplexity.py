@@ -12,10 +12,11 @@ import os
 import sys
 
 import torch
-import torch.nn.functional as F
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)),
                                 '..', '..'))
+
+from parallax_amd.ops import linear_cross_entropy  # noqa: E402
 
 
 def _decoder_nll(model, dec, thought, tgt):
@@ -24,10 +25,10 @@ def _decoder_nll(model, dec, thought, tgt):
     B, T, _ = emb.shape
     th = thought.unsqueeze(1).expand(B, T, thought.shape[-1])
     outs, _ = dec(torch.cat([emb, th], dim=-1))
-    h = model.out_proj(outs).reshape(B * T, -1)
-    logits = h @ model.emb.full_weight().t()
-    y = tgt[:, 1:].reshape(-1)
-    return F.cross_entropy(logits, y, reduction='sum'), y.numel()
+    h = model.out_proj(outs)
+    y = tgt[:, 1:]
+    return linear_cross_entropy(h, model.emb.full_weight(), None, y,
+                                reduction='sum'), y.numel()
 
 
 @torch.no_grad()

@@ -26,7 +26,9 @@ from parallax_amd import optim
 from parallax_amd.ops.embedding import PartitionedEmbedding
 from parallax_amd.ops.layernorm import ParallaxLayerNorm
 from parallax_amd.ops.linear import PxLinear
+from parallax_amd.ops.linear_ce import linear_cross_entropy
 from parallax_amd.ops.lstm import ParallaxLSTM
+from parallax_amd.ops.rotary import ParallaxRotary
 from parallax_amd.ops.sampled_softmax import sampled_softmax_loss
 from parallax_amd.ops.softmax_ce import softmax_cross_entropy
 from parallax_amd.partitions import get_partitioner
@@ -42,10 +44,12 @@ class _MHA(nn.Module):
     parameter would produce no gradient and trip the dense engine's
     incomplete-bucket guard at world_size > 1."""
 
-    def __init__(self, d, heads, cross=False):
+    def __init__(self, d, heads, cross=False, rotary=None):
         super().__init__()
         self.d = d
         self.h = heads
+        # shared by all layers: held outside the module tree
+        self._rotary = (rotary,)
         if cross:
             self.kv = PxLinear(d, 2 * d, bias=False)
             self.q = PxLinear(d, d, bias=False)
@@ -63,20 +67,24 @@ class _MHA(nn.Module):
         S = k.shape[1]
 
         def split(t, n):
-            return t.view(B, n, self.h, D // self.h).transpose(1, 2)
+            return t.view(B, n, self.h, D // self.h)
 
         q, k, v = split(q, T), split(k, S), split(v, S)
+        if self._rotary[0] is not None:
+            q, k = self._rotary[0](q, k)
+        q, k, v = (t.transpose(1, 2) for t in (q, k, v))
         from parallax_amd.ops.attention import px_attention
         o = px_attention(q, k, v, is_causal=causal)
         return self.out(o.transpose(1, 2).reshape(B, T, D))
 
 
 class _Block(nn.Module):
-    def __init__(self, d, heads, ffn, cross=False, dropout=0.1):
+    def __init__(self, d, heads, ffn, cross=False, dropout=0.1,
+                 rotary=None):
         super().__init__()
         self.p = dropout
         self.ln1 = ParallaxLayerNorm(d)
-        self.attn = _MHA(d, heads)
+        self.attn = _MHA(d, heads, rotary=rotary)
         self.cross = cross
         if cross:
             self.ln_x = ParallaxLayerNorm(d)
@@ -101,10 +109,28 @@ class _Block(nn.Module):
 
 
 class NMTTransformer(nn.Module):
+    """positions: 'learned' (one row of a table for each of ``max_len``
+    places) or 'rotary' (self-attention queries and keys turned by their
+    place; ``max_len`` rows of fixed tables).
+
+    softmax: 'sampled' (over the tied target table, whose gradient stays
+    indexed slices) or 'full' (ops.linear_cross_entropy over an output
+    table of its own, whose gradient is dense and goes over the all-reduce
+    plane, with ``label_smoothing``; targets of -100 are ignored)."""
+
     def __init__(self, src_vocab=SRC_VOCAB, tgt_vocab=TGT_VOCAB, d_model=512,
                  heads=8, ffn=2048, enc_layers=6, dec_layers=6,
-                 min_partitions=8, max_len=512):
+                 min_partitions=8, max_len=512, positions='learned',
+                 softmax='sampled', label_smoothing=0.0):
         super().__init__()
+        if positions not in ('learned', 'rotary'):
+            raise ValueError("positions is 'learned' or 'rotary', got %r"
+                             % (positions,))
+        if softmax not in ('sampled', 'full'):
+            raise ValueError("softmax is 'sampled' or 'full', got %r"
+                             % (softmax,))
+        if label_smoothing and softmax != 'full':
+            raise ValueError("label_smoothing needs softmax='full'")
         part = get_partitioner(min_partitions)
         self.d_model = d_model
         self.tgt_vocab = tgt_vocab
@@ -112,29 +138,51 @@ class NMTTransformer(nn.Module):
                                             init_scale=0.05)
         self.tgt_emb = PartitionedEmbedding(tgt_vocab, d_model, part,
                                             init_scale=0.05)
-        self.pos = nn.Parameter(torch.zeros(max_len, d_model))
         from parallax_amd.tagging import mark_dense
-        mark_dense(self.pos)
+        self.pos = self.rotary = None
+        if positions == 'learned':
+            self.pos = nn.Parameter(torch.zeros(max_len, d_model))
+            mark_dense(self.pos)
+        else:
+            self.rotary = ParallaxRotary(d_model // heads, max_len)
         self.enc = nn.ModuleList(
-            [_Block(d_model, heads, ffn) for _ in range(enc_layers)])
+            [_Block(d_model, heads, ffn, rotary=self.rotary)
+             for _ in range(enc_layers)])
         self.dec = nn.ModuleList(
-            [_Block(d_model, heads, ffn, cross=True)
+            [_Block(d_model, heads, ffn, cross=True, rotary=self.rotary)
              for _ in range(dec_layers)])
         self.ln_f = ParallaxLayerNorm(d_model)
+        self.label_smoothing = label_smoothing
+        self.out_w = None
+        if softmax == 'full':
+            w = torch.empty(tgt_vocab, d_model)
+            nn.init.normal_(w, std=d_model ** -0.5)
+            self.out_w = nn.Parameter(w)
+            mark_dense(self.out_w)
+
+    def _embed(self, table, ids):
+        """Scaled rows (+ learned positions).  Lookups come from the
+        (always-fp32) sparse tables; cast to the body dtype (bf16 in
+        pure-bf16 mode, no-op otherwise)."""
+        e = table(ids).to(self.ln_f.weight.dtype) * math.sqrt(self.d_model)
+        return e if self.pos is None else e + self.pos[:ids.shape[1]]
+
+    def _output_table(self):
+        return self.tgt_emb.full_weight() if self.out_w is None \
+            else self.out_w.detach()
 
     def forward(self, src, tgt_in, tgt_out):
-        scale = math.sqrt(self.d_model)
-        # lookups come from the (always-fp32) sparse tables; cast to the
-        # body dtype (bf16 in pure-bf16 mode, no-op otherwise)
-        body = self.pos.dtype
-        e = self.src_emb(src).to(body) * scale + self.pos[:src.shape[1]]
+        e = self._embed(self.src_emb, src)
         for blk in self.enc:
             e = blk(e)
-        d = self.tgt_emb(tgt_in).to(body) * scale \
-            + self.pos[:tgt_in.shape[1]]
+        d = self._embed(self.tgt_emb, tgt_in)
         for blk in self.dec:
             d = blk(d, mem=e, causal=True)
         d = self.ln_f(d)
+        if self.out_w is not None:
+            return linear_cross_entropy(
+                d, self.out_w, None, tgt_out,
+                label_smoothing=self.label_smoothing)
         # Tied output softmax over the partitioned tgt table, via sampled
         # softmax so the table's gradient stays indexed-slices (a full
         # dense logits GEMM would produce a dense [V, D] grad and push the
@@ -149,9 +197,7 @@ class NMTTransformer(nn.Module):
 
     @torch.no_grad()
     def encode(self, src):
-        scale = math.sqrt(self.d_model)
-        body = self.pos.dtype
-        e = self.src_emb(src).to(body) * scale + self.pos[:src.shape[1]]
+        e = self._embed(self.src_emb, src)
         for blk in self.enc:
             e = blk(e)
         return e
@@ -164,14 +210,12 @@ class NMTTransformer(nn.Module):
         Returns a list of id-lists (without SOS, truncated at EOS)."""
         mem = self.encode(src)
         B = src.shape[0]
-        W = self.tgt_emb.full_weight().to(mem.dtype)   # [V, D]
+        W = self._output_table().to(mem.dtype)   # [V, D]
         ys = torch.full((B, 1), sos_id, dtype=torch.long,
                         device=src.device)
         done = torch.zeros(B, dtype=torch.bool, device=src.device)
-        scale = math.sqrt(self.d_model)
         for _ in range(max_len):
-            d = self.tgt_emb(ys).to(mem.dtype) * scale \
-                + self.pos[:ys.shape[1]]
+            d = self._embed(self.tgt_emb, ys)
             for blk in self.dec:
                 d = blk(d, mem=mem, causal=True)
             d = self.ln_f(d)[:, -1]                    # [B, D]
@@ -205,9 +249,8 @@ class NMTTransformer(nn.Module):
         B, S, D = mem.shape
         K = beam_width
         dev = src.device
-        W = self.tgt_emb.full_weight().to(mem.dtype)    # [V, D]
+        W = self._output_table().to(mem.dtype)    # [V, D]
         V = W.shape[0]
-        scale = math.sqrt(self.d_model)
         mem = mem.unsqueeze(1).expand(B, K, S, D).reshape(B * K, S, D)
         ys = torch.full((B * K, 1), sos_id, dtype=torch.long, device=dev)
         # only beam 0 is live at the start (all beams hold identical
@@ -225,8 +268,7 @@ class NMTTransformer(nn.Module):
             return ((5.0 + length) / 6.0) ** length_penalty_weight
 
         for _ in range(max_len):
-            d = self.tgt_emb(ys).to(mem.dtype) * scale \
-                + self.pos[:ys.shape[1]]
+            d = self._embed(self.tgt_emb, ys)
             for blk in self.dec:
                 d = blk(d, mem=mem, causal=True)
             d = self.ln_f(d)[:, -1]                     # [B*K, D]
@@ -427,23 +469,50 @@ class GNMTAttention(nn.Module):
 def build_nmt_graph(arch='transformer', src_vocab=SRC_VOCAB,
                     tgt_vocab=TGT_VOCAB, d_model=512, heads=8, ffn=2048,
                     enc_layers=6, dec_layers=6, min_partitions=8, lr=1e-3,
-                    use_bf16=True, pure_bf16=False, **kw):
-    """pure_bf16 (transformer only): the dense body lives in bf16 — no
+                    use_bf16=True, pure_bf16=False, optimizer='adam',
+                    muon_lr=0.02, positions='learned', softmax='sampled',
+                    label_smoothing=0.0, **kw):
+    """optimizer: 'adam', or 'muon' for the body's matrices with Adam (at
+    ``lr``) for the rest.  positions, softmax, label_smoothing: see
+    NMTTransformer.
+
+    pure_bf16 (transformer only): the dense body lives in bf16 — no
     per-step autocast weight-cast kernels — with fp32 update precision via
     the optimizers' fused master-weight path; the sparse embedding tables
     stay fp32 (row updates keep full precision)."""
+    if optimizer not in ('adam', 'muon'):
+        raise ValueError("optimizer is 'adam' or 'muon', got %r"
+                         % (optimizer,))
     if arch == 'transformer':
         model = NMTTransformer(src_vocab, tgt_vocab, d_model, heads, ffn,
-                               enc_layers, dec_layers, min_partitions)
+                               enc_layers, dec_layers, min_partitions,
+                               positions=positions, softmax=softmax,
+                               label_smoothing=label_smoothing)
         if pure_bf16:
             model.to(torch.bfloat16)
             model.src_emb.float()
             model.tgt_emb.float()
     else:
+        if (positions, softmax, label_smoothing) != ('learned', 'sampled',
+                                                     0.0):
+            raise ValueError('positions, softmax and label_smoothing are '
+                             'options of the transformer')
         pure_bf16 = False
         model = GNMTAttention(src_vocab, tgt_vocab, d_model,
                               kw.get('units', d_model), min_partitions)
-    optimizer = optim.Adam(model.parameters(), lr=lr)
+    if optimizer == 'muon':
+        # embeddings, output and position tables are no maps between
+        # features: they and the vectors take Adam
+        tables = [p for n, p in model.named_parameters()
+                  if n in ('pos', 'out_w') or n.split('.')[0] in (
+                      'src_emb', 'tgt_emb')]
+        body = [p for p in model.parameters()
+                if not any(p is t for t in tables)]
+        optimizer = optim.Muon([dict(params=body),
+                                dict(params=tables, muon=False)],
+                               lr=muon_lr, adam_lr=lr, betas=(0.9, 0.999))
+    else:
+        optimizer = optim.Adam(model.parameters(), lr=lr)
 
     def step_fn(m, batch):
         src, tgt_in, tgt_out = batch

@@ -95,10 +95,13 @@ def linear_cross_entropy(inputs, weight, bias, labels, reduction='mean',
     their inputs are not read; other labels are clamped to the vocabulary.
     'mean' is over the rows that count (NaN where none does).  The loss is
     fp32: a scalar, or the shape of ``labels`` for 'none'.  ``weight`` is
-    cast to the type of ``inputs`` where the two differ.
+    cast to the type of ``inputs`` where the two differ; under autocast
+    both are cast to its type, as a product's operands are.
     """
     _check(inputs, weight, bias, labels, label_smoothing, reduction)
     x = inputs.reshape(-1, inputs.shape[-1])
+    if torch.is_autocast_enabled(x.device.type):
+        x = x.to(torch.get_autocast_dtype(x.device.type))
     y = labels.reshape(-1).long()
     if weight.dtype != x.dtype:
         weight = weight.to(x.dtype)
@@ -114,6 +117,7 @@ def linear_cross_entropy(inputs, weight, bias, labels, reduction='mean',
                                    ignore_index, float(label_smoothing),
                                    _REDUCTIONS[reduction])
     else:
-        losses = _plain(x, weight, bias, y, ignore_index, label_smoothing,
-                        reduction)
+        with torch.autocast(x.device.type, enabled=False):
+            losses = _plain(x, weight, bias, y, ignore_index,
+                            label_smoothing, reduction)
     return losses.view(labels.shape) if reduction == 'none' else losses

@@ -36,7 +36,8 @@ def _into(g, out, steps, coefficients, eps, exact):
     if _ops.use_native(g):
         _ops.ext().newton_schulz(g, out, steps, *coefficients, eps, exact)
     else:
-        out.copy_(_plain(g, steps, coefficients, eps))
+        with torch.autocast(g.device.type, enabled=False):
+            out.copy_(_plain(g, steps, coefficients, eps))
     return out
 
 

@@ -195,6 +195,9 @@ def test_leading_dimensions_and_mixed_types(dev):
     assert torch.equal(mixed.detach(), same)
     mixed.backward()
     assert wl.grad.dtype == torch.float32
+    with torch.autocast(dev, dtype=torch.bfloat16):
+        auto = ops.linear_cross_entropy(x, w, b, y)
+    assert torch.equal(auto, same) and auto.dtype == torch.float32
 
 
 @GPU
