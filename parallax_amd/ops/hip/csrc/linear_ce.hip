@@ -37,10 +37,12 @@ namespace {
 
 using namespace mm;
 
+// exponentials are powers of 2, so logits are held times log2 e
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 // G of one piece of the vocabulary takes at most this much
-constexpr long kPieceBytes = 128L << 20;
+constexpr long kPieceBytes = 176L << 20;
 // and so do the split parts of an fp32 table's piece
 constexpr long kSplitBytes = 64L << 20;
 
@@ -59,6 +61,40 @@ __device__ __forceinline__ float load_as(const void* p, long i, int type) {
   const ushort u = static_cast<const ushort*>(p)[i];
   return type == 1 ? half_bits(u) : __uint_as_float((unsigned)u << 16);
 }
+
+// log2 e times the bias of the words v..v+3, 0 behind the last one
+struct Bias {
+  const void* p;  // of the piece's first word, or nullptr
+  long stride;
+  int type;
+  bool four;      // four at a time can be read
+  __device__ __forceinline__ void load(float (&out)[4], int v,
+                                       int words) const {
+    if (p == nullptr) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) out[r] = 0.f;
+    } else if (four && v + 4 <= words) {
+      if (type == 2) {
+        const f4 b = reinterpret_cast<const f4*>(p)[v >> 2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) out[r] = b[r] * kLog2e;
+      } else {
+        const ushort4 b = reinterpret_cast<const ushort4*>(p)[v >> 2];
+        const ushort e[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          out[r] = kLog2e * (type == 1 ? half_bits(e[r])
+                                       : __uint_as_float((unsigned)e[r]
+                                                         << 16));
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        out[r] = v + r < words
+                     ? kLog2e * load_as(p, (v + r) * stride, type) : 0.f;
+    }
+  }
+};
 
 __device__ __forceinline__ ushort bf16_bits(float v) {
   return __builtin_bit_cast(ushort, (__bf16)v);
@@ -87,8 +123,9 @@ __device__ __forceinline__ float scale_to_half(float top) {
 }
 
 // --- laying out an operand --------------------------------------------------
-// out[rows_out][dp] 16-bit, zeros behind d and behind the rows; fp32 input:
-// a high and a low fp16 plane, scaled by a power of two.  One wave a row.
+// out[rows_out][dp] 16-bit, zeros behind d and behind the rows, and the same
+// in blocks of 32 columns where `blocks` is given; fp32 input: a high and a
+// low fp16 plane, scaled by a power of two.  One wave a row.
 // labels (x only): rows whose label is `ignore` become zeros.
 // fixed: the scale of every row (fp32 only) is found from top[0..ntop);
 // otherwise each row has its own.  inv[r] = 1 / scale.  bmax: the largest
@@ -96,8 +133,8 @@ __device__ __forceinline__ float scale_to_half(float top) {
 template <int SEG>
 __global__ __launch_bounds__(256) void lce_pack_kernel(
     const void* __restrict__ src, int type, long rs, long cs, long rows,
-    int d, ushort* __restrict__ out, int dp, long rows_out,
-    const int64_t* __restrict__ labels, int64_t ignore, bool fixed,
+    int d, ushort* __restrict__ out, ushort* __restrict__ blocks, int dp,
+    long rows_out, const int64_t* __restrict__ labels, int64_t ignore, bool fixed,
     const float* __restrict__ top, int ntop, float* __restrict__ inv,
     float* __restrict__ bmax) {
   __shared__ float scratch[PX_BLOCK / WAVE];
@@ -117,7 +154,8 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(
         ushort u = 0;
         if (live && c < d)
           u = static_cast<const ushort*>(src)[r * rs + c * cs];
-        out[r * dp + c] = u;
+        if (out) out[r * dp + c] = u;
+        if (blocks) blocks[((c >> 5) * rows_out + r) * 32 + (c & 31)] = u;
       }
     } else {
       const float* s = static_cast<const float*>(src) + r * rs;
@@ -139,8 +177,15 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(
         const float v = live && c < d ? s[c * cs] * scale : 0.f;
         ushort h, l;
         split(v, h, l);
-        out[r * dp + c] = h;
-        out[rows_out * dp + r * dp + c] = l;
+        const long at = ((c >> 5) * rows_out + r) * 32 + (c & 31);
+        if (out) {
+          out[r * dp + c] = h;
+          out[rows_out * dp + r * dp + c] = l;
+        }
+        if (blocks) {
+          blocks[at] = h;
+          blocks[rows_out * dp + at] = l;
+        }
       }
     }
   }
@@ -156,17 +201,15 @@ struct Logits {
   Operand x, w;
   const float* xinv;  // SEG 3: scales to undo, by row and by word
   const float* winv;
-  const void* bias;
-  int bias_type;
-  long bias_stride;
+  Bias bias;
   int n;     // rows
   int vp;    // words in this piece
   int dp;
 };
 
-// max, sum of exp and (SMOOTH) total of each row over `tpb` tiles of words
-template <class C, int SEG, bool BF, bool SMOOTH>
-__global__ __launch_bounds__(C::THREADS, 2) void lce_fwd_kernel(
+// max, sum of exp and (SMOOTH) total of each row, in powers of 2, over `tpb` tiles of words
+template <class C, int XL, int SEG, bool BF, bool SMOOTH>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
     Logits p, float* __restrict__ part, int part_rows, int vb0,
     int nblocks, int nmt, int nvb, int tpb) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -196,17 +239,17 @@ __global__ __launch_bounds__(C::THREADS, 2) void lce_fwd_kernel(
     const int n0 = (vb * tpb + q) * C::BN;
     if (n0 >= p.vp) break;
     f4 acc[C::FM][C::FN] = {};
-    product<C, KROWS, KROWS, SEG, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
+    product<C, XL, KROWS, SEG, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
     float add[C::FN][4], ws[C::FN][4];
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+      p.bias.load(add[j], n0 + wn + j * 16 + (lane >> 4) * 4, p.vp);
 #pragma unroll
     for (int j = 0; j < C::FN; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int v = n0 + wn + j * 16 + (lane >> 4) * 4 + r;
-        add[j][r] = p.bias && v < p.vp
-                        ? load_as(p.bias, v * p.bias_stride, p.bias_type)
-                        : 0.f;
-        ws[j][r] = SEG == 3 && v < p.vp ? p.winv[v] : 1.f;
+        ws[j][r] = SEG == 3 && v < p.vp ? p.winv[v] * kLog2e : kLog2e;
       }
     if (n0 + C::BN > p.vp) {  // words behind the last one
 #pragma unroll
@@ -225,19 +268,19 @@ __global__ __launch_bounds__(C::THREADS, 2) void lce_fwd_kernel(
       for (int j = 0; j < C::FN; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float z = acc[i][j][r];
-          if (SEG == 3) z = z * xs[i] * ws[j][r];
-          z += add[j][r];
+          const float z = fmaf(SEG == 3 ? acc[i][j][r] * xs[i]
+                                        : acc[i][j][r],
+                               ws[j][r], add[j][r]);
           acc[i][j][r] = z;
           top = fmaxf(top, z);
         }
       const float off = top == -INFINITY ? 0.f : top;
-      float s = se[i] * exp2_fast((mx[i] - off) * kLog2e);
+      float s = se[i] * exp2_fast(mx[i] - off);
 #pragma unroll
       for (int j = 0; j < C::FN; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s += exp2_fast((acc[i][j][r] - off) * kLog2e);
+          s += exp2_fast(acc[i][j][r] - off);
           if (SMOOTH) {
             const int v = n0 + wn + j * 16 + (lane >> 4) * 4 + r;
             if (v < p.vp) tot[i] += acc[i][j][r];
@@ -258,8 +301,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void lce_fwd_kernel(
       if (SMOOTH) tot[i] += __shfl_xor(tot[i], o, 64);
       const float top = fmaxf(mx[i], m2);
       const float off = top == -INFINITY ? 0.f : top;
-      se[i] = se[i] * exp2_fast((mx[i] - off) * kLog2e) +
-              s2 * exp2_fast((m2 - off) * kLog2e);
+      se[i] = se[i] * exp2_fast(mx[i] - off) + s2 * exp2_fast(m2 - off);
       mx[i] = top;
     }
     if (lane < 16) {
@@ -277,7 +319,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void lce_fwd_kernel(
       const float* at = red + (w * C::BM + r) * 3;
       const float top = fmaxf(m, at[0]);
       const float off = top == -INFINITY ? 0.f : top;
-      s = s * exp2_fast((m - off) * kLog2e) + at[1] * exp2_fast((at[0] - off) * kLog2e);
+      s = s * exp2_fast(m - off) + at[1] * exp2_fast(at[0] - off);
       m = top;
       t += at[2];
     }
@@ -310,7 +352,7 @@ __global__ __launch_bounds__(256) void lce_join_kernel(
       const float m2 = part[at], s2 = part[at + plane];
       const float top = fmaxf(m, m2);
       const float off = top == -INFINITY ? 0.f : top;
-      s = s * exp2_fast((m - off) * kLog2e) + s2 * exp2_fast((m2 - off) * kLog2e);
+      s = s * exp2_fast(m - off) + s2 * exp2_fast(m2 - off);
       m = top;
       if (eps != 0.f) t += part[at + 2 * plane];
     }
@@ -339,15 +381,15 @@ __global__ __launch_bounds__(256) void lce_join_kernel(
       const float m2 = sm[0][row][b], s2 = sm[1][row][b];
       const float top = fmaxf(m, m2);
       const float off = top == -INFINITY ? 0.f : top;
-      s = s * exp2_fast((m - off) * kLog2e) + s2 * exp2_fast((m2 - off) * kLog2e);
+      s = s * exp2_fast(m - off) + s2 * exp2_fast(m2 - off);
       m = top;
       t += sm[2][row][b];
     }
-    const float l = m + logf(s);
+    const float l = m * kLn2 + logf(s);
     const int r = r0 + row;
     lse[r] = l;
     float out = l - (1.f - eps) * zy[row];
-    if (eps != 0.f) out -= eps * (t / (float)V);
+    if (eps != 0.f) out -= eps * (t * kLn2 / (float)V);
     loss[r] = labels[r] == ignore ? 0.f : out;
   }
 }
@@ -383,20 +425,37 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(
 
 // --- backward ---------------------------------------------------------------
 
-// g[n]: what each row's G is multiplied by, and sc = {S, 1/S} for 16-bit G
+// What the gradient needs of a row.  Rows that do not count: an infinite l
+// makes their exponentials 0, and g = 0.
+struct Row {
+  float l;   // log2 e lse
+  float g;   // what the row's G is multiplied by
+  int y;     // label
+  float xs;  // scale to undo
+};
+
+// the rows, and sc = {S, 1/S} for 16-bit G
 __global__ __launch_bounds__(1024) void lce_rows_kernel(
     const float* __restrict__ dloss, bool scalar,
     const float* __restrict__ count, const int64_t* __restrict__ labels,
-    int64_t ignore, int n, int n_out, bool half, float* __restrict__ g,
+    int64_t ignore, int n, int n_out, bool half,
+    const float* __restrict__ lse, long V, Row* __restrict__ rows,
     float* __restrict__ sc) {
   __shared__ float red[16];
   const float div = count ? count[0] : 1.f;
   float most = 0.f;
   for (int i = threadIdx.x; i < n_out; i += 1024) {
-    float v = 0.f;
-    if (i < n && labels[i] != ignore) v = dloss[scalar ? 0 : i] / div;
-    g[i] = v;
-    most = fmaxf(most, fabsf(v));
+    Row row = {INFINITY, 0.f, 0, 1.f};
+    if (i < n) {
+      const int64_t y = labels[i];
+      row.y = (int)(y < 0 ? 0 : (y >= V ? V - 1 : y));
+      if (y != ignore) {
+        row.g = dloss[scalar ? 0 : i] / div;
+        row.l = lse[i] * kLog2e;
+      }
+    }
+    rows[i] = row;
+    most = fmaxf(most, fabsf(row.g));
   }
   most = block_reduce_max(most, red);
   if (threadIdx.x == 0) {
@@ -409,11 +468,10 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(
 
 // G of one piece, [rows padded to BM][ldg]; zeros outside the matrix.
 // DB: column sums of each row tile into dbp[row tile][ldg].
-template <class C, int SEG, bool BF, bool DB>
-__global__ __launch_bounds__(C::THREADS, 2) void lce_grad_kernel(
-    Logits p, const float* __restrict__ lse, const float* __restrict__ g,
-    const float* __restrict__ sc, const int64_t* __restrict__ labels, long V,
-    long v0, float eps, ushort* __restrict__ G, int ldg, long glo,
+template <class C, int XL, int SEG, bool BF, bool DB>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
+    Logits p, const Row* __restrict__ rows, const float* __restrict__ sc,
+    long V, long v0, float eps, ushort* __restrict__ G, int ldg, long glo,
     float* __restrict__ dbp, int nmt, int nvt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int bid = die_contiguous(blockIdx.x, nmt * nvt);
@@ -424,70 +482,84 @@ __global__ __launch_bounds__(C::THREADS, 2) void lce_grad_kernel(
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
   f4 acc[C::FM][C::FN] = {};
-  product<C, KROWS, KROWS, SEG, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
+  product<C, XL, KROWS, SEG, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
   const int c0 = n0 + wn + (lane >> 4) * 4;
   const float S = sc[0], uni = eps / (float)V;
-  float add[C::FN][4], ws[C::FN][4], col[C::FN][4];
+  const float xs = SEG == 3 ? p.xinv[0] : 1.f;  // one for all rows
+  float add[C::FN][4], ws[C::FN][4];
+#pragma unroll
+  for (int j = 0; j < C::FN; ++j) p.bias.load(add[j], c0 + j * 16, p.vp);
 #pragma unroll
   for (int j = 0; j < C::FN; ++j)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int v = c0 + j * 16 + r;
-      col[j][r] = 0.f;
-      add[j][r] = p.bias && v < p.vp
-                      ? load_as(p.bias, v * p.bias_stride, p.bias_type)
-                      : 0.f;
-      ws[j][r] = SEG == 3 && v < p.vp ? p.winv[v] : 1.f;
+      ws[j][r] = SEG == 3 && v < p.vp ? p.winv[v] * kLog2e : kLog2e;
     }
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
-    const int m = m0 + wm + i * 16 + (lane & 15);
-    const bool in = m < p.n;
-    const float l = in ? lse[m] : 0.f, gm = in ? g[m] : 0.f;
-    const float xs = SEG == 3 && in ? p.xinv[m] : 1.f;
-    int64_t y = in ? labels[m] : 0;
-    y = y < 0 ? 0 : (y >= V ? V - 1 : y);
-    const int hit = in ? (int)(y - v0 < -1 ? -1
-                               : (y - v0 > p.vp ? p.vp : y - v0)) - c0
-                       : -1;
-#pragma unroll
-    for (int j = 0; j < C::FN; ++j) {
-      ushort hi[4], lo[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float z = acc[i][j][r];
-        if (SEG == 3) z = z * xs * ws[j][r];
-        z += add[j][r];
-        float v = exp2_fast((z - l) * kLog2e) - uni;
-        if (hit == j * 16 + r) v -= 1.f - eps;
-        // rows that do not count have to be zero whatever z is
-        v = gm == 0.f || c0 + j * 16 + r >= p.vp ? 0.f : v * gm;
-        if (DB) col[j][r] += v;
-        if (BF) {
-          hi[r] = bf16_bits(v);
-        } else if (SEG == 1) {
-          hi[r] = fp16_bits(v * S);
-        } else {
-          split(v * S, hi[r], lo[r]);
-        }
-      }
-      const long at = (long)m * ldg + c0 + j * 16;
-      *reinterpret_cast<ushort4*>(G + at) =
-          make_ushort4(hi[0], hi[1], hi[2], hi[3]);
-      if (SEG == 3)
-        *reinterpret_cast<ushort4*>(G + glo + at) =
-            make_ushort4(lo[0], lo[1], lo[2], lo[3]);
-    }
-  }
-  if (DB) {
-    float* red = reinterpret_cast<float*>(smem);  // [waves_m][BN]
+    // one load of 16 bytes: there are rows up to a whole tile
+    const f4 row = reinterpret_cast<const f4*>(
+        rows)[m0 + wm + i * 16 + (lane & 15)];
+    const float l = row[0], gm = row[1];
 #pragma unroll
     for (int j = 0; j < C::FN; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float c = col[j][r];
+        const float z = SEG == 3 ? acc[i][j][r] * xs : acc[i][j][r];
+        acc[i][j][r] =
+            (exp2_fast(fmaf(z, ws[j][r], add[j][r] - l)) - uni) * gm;
+      }
+    // the label's word: in few tiles, so not a comparison for each value
+    const long y = (long)__builtin_bit_cast(int, (float)row[2]) - v0 - n0 - wn;
+    const int hit = y >= 0 && y < C::WN ? (int)y - (lane >> 4) * 4 : -1;
+    if (__any(hit >= 0)) {
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) c += __shfl_xor(c, o, 64);
+      for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (hit == j * 16 + r) acc[i][j][r] -= (1.f - eps) * gm;
+    }
+  }
+  if (n0 + C::BN > p.vp) {  // words behind the last one
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (c0 + j * 16 + r >= p.vp) {
+#pragma unroll
+          for (int i = 0; i < C::FM; ++i) acc[i][j][r] = 0.f;
+        }
+  }
+  ushort* at = G + (long)m0 * ldg + n0;
+  store_tile<C>(smem, at, ldg, C::BM, C::BN, [&](int i, int j) {
+    const f4 v = acc[i][j];
+    if (BF)
+      return make_ushort4(bf16_bits(v[0]), bf16_bits(v[1]), bf16_bits(v[2]),
+                          bf16_bits(v[3]));
+    return make_ushort4(fp16_bits(v[0] * S), fp16_bits(v[1] * S),
+                        fp16_bits(v[2] * S), fp16_bits(v[3] * S));
+  });
+  if (SEG == 3) {
+    __syncthreads();
+    store_tile<C>(smem, at + glo, ldg, C::BM, C::BN, [&](int i, int j) {
+      ushort h, l[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) split(acc[i][j][r] * S, h, l[r]);
+      return make_ushort4(l[0], l[1], l[2], l[3]);
+    });
+  }
+  if (DB) {
+    float* red = reinterpret_cast<float*>(smem);  // [waves_m][BN]
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float c = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::FM; ++i) c += acc[i][j][r];
+        c = sum16(c);
         if ((lane & 15) == 0)
           red[(wave / C::WAVES_N) * C::BN + wn + j * 16 + (lane >> 4) * 4 +
               r] = c;
@@ -513,7 +585,7 @@ __global__ __launch_bounds__(256) void lce_db_kernel(
 
 // dw[v, :] = 1/S sum_n G[n, v] x[n, :]  (G and x both k-strided)
 template <class C, int SEG, bool BF>
-__global__ __launch_bounds__(C::THREADS, 2) void lce_dw_kernel(
+__global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
     Operand G, Operand x, int kn, const float* __restrict__ sc,
     const float* __restrict__ xinv, void* __restrict__ dw, int type, int vp,
     int d, int nmt, int nnt) {
@@ -527,6 +599,18 @@ __global__ __launch_bounds__(C::THREADS, 2) void lce_dw_kernel(
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
   const float back = sc[1] * (SEG == 3 ? xinv[0] : 1.f);
+  if (type != 2 && (d & 7) == 0) {
+    store_tile<C>(smem, static_cast<ushort*>(dw) + (long)m0 * d + n0, d,
+                  vp - m0, d - n0, [&](int i, int j) {
+      const f4 v = acc[i][j] * back;
+      if (BF)
+        return make_ushort4(bf16_bits(v[0]), bf16_bits(v[1]),
+                            bf16_bits(v[2]), bf16_bits(v[3]));
+      return make_ushort4(fp16_bits(v[0]), fp16_bits(v[1]), fp16_bits(v[2]),
+                          fp16_bits(v[3]));
+    });
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
     const int v = m0 + wm + i * 16 + (lane & 15);
@@ -535,18 +619,9 @@ __global__ __launch_bounds__(C::THREADS, 2) void lce_dw_kernel(
     for (int j = 0; j < C::FN; ++j) {
       const int c = n0 + wn + j * 16 + (lane >> 4) * 4;
       const long at = (long)v * d + c;
-      if (c + 4 <= d && (d & 3) == 0) {
-        f4 o = acc[i][j] * back;
-        if (type == 2) {
-          *reinterpret_cast<f4*>(static_cast<float*>(dw) + at) = o;
-        } else {
-          ushort4 u;
-          u.x = BF ? bf16_bits(o[0]) : fp16_bits(o[0]);
-          u.y = BF ? bf16_bits(o[1]) : fp16_bits(o[1]);
-          u.z = BF ? bf16_bits(o[2]) : fp16_bits(o[2]);
-          u.w = BF ? bf16_bits(o[3]) : fp16_bits(o[3]);
-          *reinterpret_cast<ushort4*>(static_cast<ushort*>(dw) + at) = u;
-        }
+      if (type == 2 && c + 4 <= d && (d & 3) == 0) {
+        *reinterpret_cast<f4*>(static_cast<float*>(dw) + at) =
+            acc[i][j] * back;
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -558,7 +633,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void lce_dw_kernel(
 
 // part[slice][n, :] (+)= sum over a slice of the piece's words G[n, v] w[v, :]
 template <class C, int SEG, bool BF>
-__global__ __launch_bounds__(C::THREADS, 2) void lce_dx_kernel(
+__global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dx_kernel(
     Operand G, Operand w, int kv, int kslice, float* __restrict__ part,
     int n_rows, int dp, bool first, int nmt, int nnt, int slices) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -605,14 +680,13 @@ __global__ __launch_bounds__(256) void lce_dx_sum_kernel(
 
 // --- host -------------------------------------------------------------------
 
-// 256 x 128, 4 waves of 128 x 64: the shape whose LDS reads (96 B a cycle of
-// 128) leave the matrix units fed, in 72 KB so that two workgroups share a
-// CU and one's exponentials run under the other's products.
-using Big = Tile<256, 128, 128, 64, 32, 3>;
-using Mid = Tile<128, 128, 64, 64, 32, 3>;
+// Sixteen waves of 64 x 64, one workgroup on a CU: the most products for a
+// byte that comes from memory, and four waves on a SIMD to wait for another.
+using Big = Tile<256, 256, 64, 64, 64, 2>;
+using Mid = Tile<128, 128, 64, 64, 64, 2>;
 // few rows: wide in the words
-using Flat = Tile<64, 256, 64, 64, 32, 3>;
-using Small = Tile<64, 64, 32, 32, 32, 3>;
+using Flat = Tile<64, 256, 64, 32, 64, 2>;
+using Small = Tile<64, 64, 32, 32, 64, 2>;
 
 int type_code(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -649,7 +723,7 @@ Plan make_plan(const at::Tensor& x, const at::Tensor& w) {
   p.d = x.size(1);
   p.v = w.size(0);
   p.dp = up(p.d, 64);
-  p.np = up(p.n, 64);
+  p.np = up(p.n, 256);
   p.type = type_code(x);
   p.seg = p.type == 2 ? 3 : 1;
   p.w_direct = p.seg == 1 && p.d == p.dp && w.stride(1) == 1 &&
@@ -666,15 +740,18 @@ int pack_blocks(long rows) {
 }
 
 void pack(const at::Tensor& src, long row0, long rows, long rows_out,
-          const Plan& p, at::Tensor& out, const int64_t* labels,
-          int64_t ignore, bool fixed, const at::Tensor& top,
+          const Plan& p, at::Tensor& out, at::Tensor& blocks,
+          const int64_t* labels, int64_t ignore, bool fixed, const at::Tensor& top,
           at::Tensor& inv, float* bmax, hipStream_t stream) {
   const char* s = static_cast<const char*>(src.data_ptr()) +
                   row0 * src.stride(0) * src.element_size();
   auto launch = [&](auto kernel) {
     kernel<<<pack_blocks(rows_out), 256, 0, stream>>>(
         s, p.type, src.stride(0), src.stride(1), rows, (int)p.d,
-        reinterpret_cast<ushort*>(out.data_ptr()), (int)p.dp, rows_out,
+        out.defined() ? reinterpret_cast<ushort*>(out.data_ptr()) : nullptr,
+        blocks.defined() ? reinterpret_cast<ushort*>(blocks.data_ptr())
+                         : nullptr,
+        (int)p.dp, rows_out,
         labels, ignore, fixed,
         top.defined() ? top.data_ptr<float>() : nullptr,
         top.defined() ? (int)top.numel() : 0,
@@ -699,6 +776,17 @@ Operand rows_operand(const ushort* p, long rows, long ld, long lo,
   return o;
 }
 
+Bias bias_of(const c10::optional<at::Tensor>& bias, long v0) {
+  Bias b = {nullptr, 0, 0, false};
+  if (!bias.has_value()) return b;
+  b.stride = bias->stride(0);
+  b.type = type_code(*bias);
+  b.p = static_cast<const char*>(bias->data_ptr()) +
+        v0 * b.stride * bias->element_size();
+  b.four = b.stride == 1 && reinterpret_cast<uintptr_t>(b.p) % 16 == 0;
+  return b;
+}
+
 void check(const at::Tensor& x, const at::Tensor& w,
            const c10::optional<at::Tensor>& bias, const at::Tensor& labels) {
   TORCH_CHECK(x.is_cuda() && w.is_cuda() && labels.is_cuda(),
@@ -715,6 +803,9 @@ void check(const at::Tensor& x, const at::Tensor& w,
   TORCH_CHECK(x.size(0) >= 1 && x.size(0) <= (1 << 20),
               "linear_ce: 1 to 2^20 rows expected");
   TORCH_CHECK(w.size(0) < (1L << 31) - 1024, "linear_ce: too many words");
+  TORCH_CHECK(up(x.size(0), 256) * up(x.size(1), 64) <= (1L << 29),
+              "linear_ce: x has more than 2^29 values: take fewer rows at a "
+              "time");
   TORCH_CHECK(labels.scalar_type() == at::kLong && labels.dim() == 1 &&
                   labels.size(0) == x.size(0) && labels.is_contiguous(),
               "linear_ce: labels [N] int64 expected");
@@ -737,14 +828,35 @@ void with_types(const Plan& p, F f) {
   }
 }
 
+// The tile of the logits, forward and backward.  Many 16-bit rows: 256 x 128
+// in two workgroups a CU, so that one's exponentials and stores run under the
+// other's products, with x in blocks.
+using Logit = Tile<256, 128, 64, 64, 32, 3>;
+
+template <class C>
+constexpr int x_layout() {
+  return std::is_same<C, Logit>::value ? KBLOCK : KROWS;
+}
+
+// two-part operands never meet that tile: its registers do not hold them
+template <class C, int SEG>
+constexpr bool reached() {
+  return !(std::is_same<C, Logit>::value && SEG == 3);
+}
+
+bool blocked(const Plan& p) {
+  // not where 256-row tiles would be empty by more than they gain
+  return p.seg == 1 && p.n > 64 && up(p.n, 256) * 100 <= up(p.n, 128) * 115;
+}
+
 template <typename F>
-void with_row_tile(long n, F f) {
-  if (n <= 64) {
+void with_row_tile(const Plan& p, F f) {
+  if (p.n <= 64) {
     f(Flat{});
-  } else if (n <= 128) {
-    f(Mid{});
+  } else if (blocked(p)) {
+    f(Logit{});
   } else {
-    f(Big{});
+    f(Mid{});
   }
 }
 
@@ -766,10 +878,11 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
   const auto* lab = labels.data_ptr<int64_t>();
   const float eps = (float)smoothing;
 
+  const bool blk = blocked(p);
   auto xpk = at::empty({p.seg == 3 ? 2 * p.np : p.np, p.dp}, u16);
   at::Tensor xinv, winv, none, tops, wpk;
   if (p.seg == 3) xinv = at::empty({p.np}, f32);
-  pack(x, 0, p.n, p.np, p, xpk, lab, ignore, false, none, xinv, nullptr,
+  pack(x, 0, p.n, p.np, p, blk ? none : xpk, blk ? xpk : none, lab, ignore, false, none, xinv, nullptr,
        stream);
 
   const long piece = p.w_direct ? p.v : p.w_rows;
@@ -785,7 +898,7 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
   auto loss = at::empty({p.n}, f32);
   auto lse = at::empty({p.n}, f32);
   auto total = at::empty({2}, f32);
-  with_row_tile(p.n, [&](auto tile) {
+  with_row_tile(p, [&](auto tile) {
     using C = decltype(tile);
     const int nmt = (int)((p.n + C::BM - 1) / C::BM);
     const long piece_tiles = (std::min(piece, p.v) + C::BN - 1) / C::BN;
@@ -808,25 +921,21 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
       if (p.w_direct) {
         q.w = rows_operand(bits(w), vp, w.stride(0), 0, p.dp);
       } else {
-        pack(w, v0, vp, p.w_rows, p, wpk, nullptr, 0, false, none, winv,
+        pack(w, v0, vp, p.w_rows, p, wpk, none, nullptr, 0, false, none, winv,
              p.seg == 3 ? tops.data_ptr<float>() + i * wblocks : nullptr,
              stream);
         q.w = rows_operand(bits(wpk), p.w_rows, p.dp, p.w_rows * p.dp, p.dp);
       }
       q.xinv = p.seg == 3 ? xinv.data_ptr<float>() : nullptr;
       q.winv = p.seg == 3 ? winv.data_ptr<float>() : nullptr;
-      q.bias_type = bias.has_value() ? type_code(*bias) : 0;
-      q.bias_stride = bias.has_value() ? bias->stride(0) : 0;
-      q.bias = bias.has_value()
-                   ? static_cast<const char*>(bias->data_ptr()) +
-                         v0 * q.bias_stride * bias->element_size()
-                   : nullptr;
+      q.bias = bias_of(bias, v0);
       q.n = (int)p.n;
       q.vp = (int)vp;
       q.dp = (int)p.dp;
       const int nvb =
           (int)((vp + (long)C::BN * tpb - 1) / ((long)C::BN * tpb));
       with_types(p, [&](auto seg, auto bf) {
+        if constexpr (reached<C, decltype(seg)::value>()) {
         auto launch = [&](auto kernel) {
           allow_lds(kernel, C::LDS_BYTES);
           kernel<<<nmt * nvb, C::THREADS, C::LDS_BYTES, stream>>>(
@@ -835,11 +944,12 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
           HIP_CHECK_KERNEL();
         };
         if (eps != 0.f) {
-          launch(lce_fwd_kernel<C, decltype(seg)::value, decltype(bf)::value,
-                                true>);
+          launch(lce_fwd_kernel<C, x_layout<C>(), decltype(seg)::value,
+                                decltype(bf)::value, true>);
         } else {
-          launch(lce_fwd_kernel<C, decltype(seg)::value, decltype(bf)::value,
-                                false>);
+          launch(lce_fwd_kernel<C, x_layout<C>(), decltype(seg)::value,
+                                decltype(bf)::value, false>);
+        }
         }
       });
     }
@@ -886,28 +996,34 @@ std::vector<at::Tensor> linear_ce_bwd(
   const bool s3 = p.seg == 3;
 
   const long nrows = up(p.n, 256);
-  auto g = at::empty({nrows}, f32);
+  auto rows = at::empty({nrows, 4}, f32);
   auto sc = at::empty({2}, f32);
   lce_rows_kernel<<<1, 1024, 0, stream>>>(
       dloss.data_ptr<float>(), reduction != 0,
       reduction == 1 ? count.data_ptr<float>() + 1 : nullptr, lab, ignore,
-      (int)p.n, (int)nrows, p.type != 0, g.data_ptr<float>(),
-      sc.data_ptr<float>());
+      (int)p.n, (int)nrows, p.type != 0, lse.data_ptr<float>(), p.v,
+      reinterpret_cast<Row*>(rows.data_ptr()), sc.data_ptr<float>());
   HIP_CHECK_KERNEL();
 
   at::Tensor xpk = at::empty({s3 ? 2 * p.np : p.np, p.dp}, u16);
-  at::Tensor xinv, winv, none, xtop, wpk;
+  at::Tensor xinv, winv, none, xtop, wpk, xblk;
+  if (blocked(p)) xblk = at::empty_like(xpk);
   if (s3) {
     // one scale for all rows, as the rows are summed over: the first call
     // only finds the largest value
     xinv = at::empty({p.np}, f32);
     xtop = at::empty({pack_blocks(p.np)}, f32);
-    pack(x, 0, p.n, p.np, p, xpk, lab, ignore, false, none, xinv,
+    pack(x, 0, p.n, p.np, p, xpk, none, lab, ignore, false, none, xinv,
          xtop.data_ptr<float>(), stream);
   }
-  pack(x, 0, p.n, p.np, p, xpk, lab, ignore, s3, xtop, xinv, nullptr, stream);
+  pack(x, 0, p.n, p.np, p, xpk, xblk, lab, ignore, s3, xtop, xinv, nullptr,
+       stream);
 
-  long piece = kPieceBytes / (nrows * (s3 ? 4 : 2)) / 256 * 256;
+  // words for which the tiles of dw fill the chip's 256 CUs once
+  const long wave_of_words = 256 * 256 / ((p.dp + 255) / 256);
+  long piece = kPieceBytes / (nrows * (s3 ? 4 : 2));
+  piece = piece >= wave_of_words ? piece / wave_of_words * wave_of_words
+                                 : piece / 256 * 256;
   piece = std::max(256L, std::min(piece, up(p.v, 256)));
   if (!p.w_direct) piece = std::min(piece, p.w_rows);
   // offsets inside a piece of w stay below 2^31
@@ -928,35 +1044,31 @@ std::vector<at::Tensor> linear_ce_bwd(
     dbp = at::empty({(p.n + 63) / 64, ldg}, f32);
   }
   // dx: few tiles and a long k, so k is cut until the chip is full
-  int slices = 1;
-  const bool dx_big = p.n > 128 && p.dp >= 128;
-  const long dx_tiles = dx_big ? ((p.n + 127) / 128) * ((p.dp + 127) / 128)
-                               : ((p.n + 63) / 64) * ((p.dp + 63) / 64);
-  slices = (int)std::min<long>(std::max(1L, 512 / dx_tiles),
-                               std::max(1L, piece / 512));
+  const int dx_tile = p.n > 128 && p.dp >= 128 ? (getenv("DXBIG") && p.dp>=256 ? 256:128) : 64;
+  const long dx_tiles = ((p.n + dx_tile - 1) / dx_tile) *
+                        ((p.dp + dx_tile - 1) / dx_tile);
+  const int slices = (int)std::min<long>(
+      std::max(1L, (dx_tile == 256 ? 256 : 512) / dx_tiles),
+      std::max(1L, piece / 512));
   if (want_dx) part = at::empty({slices, p.n, p.dp}, f32);
 
   for (long v0 = 0; v0 < p.v; v0 += piece) {
     const long vp = std::min(piece, p.v - v0);
     Logits q;
-    q.x = rows_operand(bits(xpk), p.np, p.dp, p.np * p.dp, p.dp);
+    q.x = rows_operand(bits(xblk.defined() ? xblk : xpk), p.np, p.dp,
+                       p.np * p.dp, p.dp);
     if (p.w_direct) {
       q.w = rows_operand(bits(w) + v0 * w.stride(0), vp, w.stride(0), 0,
                          p.dp);
     } else {
-      pack(w, v0, vp, up(vp, 64), p, wpk, nullptr, 0, s3, tops, winv,
+      pack(w, v0, vp, up(vp, 64), p, wpk, none, nullptr, 0, s3, tops, winv,
            nullptr, stream);
       q.w = rows_operand(bits(wpk), up(vp, 64), p.dp, up(vp, 64) * p.dp,
                          p.dp);
     }
     q.xinv = s3 ? xinv.data_ptr<float>() : nullptr;
     q.winv = s3 ? winv.data_ptr<float>() : nullptr;
-    q.bias_type = bias.has_value() ? type_code(*bias) : 0;
-    q.bias_stride = bias.has_value() ? bias->stride(0) : 0;
-    q.bias = bias.has_value()
-                 ? static_cast<const char*>(bias->data_ptr()) +
-                       v0 * q.bias_stride * bias->element_size()
-                 : nullptr;
+    q.bias = bias_of(bias, v0);
     q.n = (int)p.n;
     q.vp = (int)vp;
     q.dp = (int)p.dp;
@@ -964,27 +1076,29 @@ std::vector<at::Tensor> linear_ce_bwd(
     with_types(p, [&](auto seg, auto bf) {
       constexpr int SEG = decltype(seg)::value;
       constexpr bool BF = decltype(bf)::value;
-      with_row_tile(p.n, [&](auto tile) {
+      with_row_tile(p, [&](auto tile) {
         using C = decltype(tile);
+        if constexpr (reached<C, SEG>()) {
         const int nmt = (int)((p.n + C::BM - 1) / C::BM);
         const int nvt = (int)((vp + C::BN - 1) / C::BN);
         auto launch = [&](auto kernel) {
           allow_lds(kernel, C::LDS_BYTES);
           kernel<<<nmt * nvt, C::THREADS, C::LDS_BYTES, stream>>>(
-              q, lse.data_ptr<float>(), g.template data_ptr<float>(),
-              sc.template data_ptr<float>(), lab, p.v, v0, eps, Gp, ldg, glo,
+              q, reinterpret_cast<const Row*>(rows.data_ptr()),
+              sc.template data_ptr<float>(), p.v, v0, eps, Gp, ldg, glo,
               want_db ? dbp.template data_ptr<float>() : nullptr, nmt, nvt);
           HIP_CHECK_KERNEL();
         };
         if (want_db) {
-          launch(lce_grad_kernel<C, SEG, BF, true>);
+          launch(lce_grad_kernel<C, x_layout<C>(), SEG, BF, true>);
           lce_db_kernel<<<(int)((vp + 255) / 256), 256, 0, stream>>>(
               dbp.template data_ptr<float>(), nmt, ldg, (int)vp,
               static_cast<char*>(db.data_ptr()) + v0 * db.element_size(),
               type_code(db));
           HIP_CHECK_KERNEL();
         } else {
-          launch(lce_grad_kernel<C, SEG, BF, false>);
+          launch(lce_grad_kernel<C, x_layout<C>(), SEG, BF, false>);
+        }
         }
       });
       if (want_dw) {
@@ -997,15 +1111,18 @@ std::vector<at::Tensor> linear_ce_bwd(
           kernel<<<nmt * nnt, C::THREADS, C::LDS_BYTES, stream>>>(
               rows_operand(Gp, nrows, ldg, glo, ldg),
               rows_operand(bits(xpk), p.np, p.dp, p.np * p.dp, p.dp),
-              (int)p.np, sc.template data_ptr<float>(),
+              (int)up(p.n, 64), sc.template data_ptr<float>(),
               s3 ? xinv.data_ptr<float>() : nullptr,
               static_cast<char*>(dw.data_ptr()) +
                   v0 * p.d * dw.element_size(),
               p.type, (int)vp, (int)p.d, nmt, nnt);
           HIP_CHECK_KERNEL();
         };
-        if (p.dp >= 128 && vp >= 8192) {
+        const long cover = ((vp + 255) / 256) * ((p.dp + 255) / 256);
+        if (cover >= 192 && p.dp % 256 == 0) {
           run(Big{});
+        } else if (cover >= 48 && p.dp >= 128) {
+          run(Mid{});
         } else {
           run(Small{});
         }
@@ -1025,7 +1142,9 @@ std::vector<at::Tensor> linear_ce_bwd(
               slices);
           HIP_CHECK_KERNEL();
         };
-        if (dx_big) {
+        if (dx_tile == 256) {
+          run(Big{});
+        } else if (dx_tile == 128) {
           run(Mid{});
         } else {
           run(Small{});

@@ -3,10 +3,14 @@
 // fp32 sums, one workgroup per tile.  The kernel that includes this owns
 // the grid, the operands' scaling and what becomes of the sums.
 //
-//   * An operand lies either k-contiguous ([rows][K], KROWS) or k-strided
-//     ([K][rows], KCOLS).  The first is read from LDS with ds_read_b128, the
-//     second with the transposing ds_read_b64_tr_b16, which hands a lane
-//     four k of one row, so no operand is ever transposed in memory.
+//   * An operand lies k-contiguous ([rows][K], KROWS), k-strided ([K][rows],
+//     KCOLS) or in blocks of 32 k ([K/32][rows][32], KBLOCK).  The first and
+//     the third are read from LDS with ds_read_b128, the second with the
+//     transposing ds_read_b64_tr_b16, which hands a lane four k of one row,
+//     so no operand is ever transposed in memory.  A stage of 32 k takes 64
+//     bytes of a k-contiguous row, half of what memory hands out at a time;
+//     blocks make that one piece (256 x 128 tile, 2560 x 32768 x 512: 86 us
+//     with rows, 74 us with the first operand in blocks).
 //   * SEG = 3 multiplies operands that are split into a high and a low fp16
 //     part (value = hi + lo, 22 bits): the k loop runs over lo*hi, hi*lo and
 //     hi*hi.  The dropped lo*lo is 2^-22 of a product.
@@ -18,7 +22,7 @@
 //     shuffles, and four results go out in one store.
 //
 // LDS layouts (16-byte chunks, permuted so that neither read conflicts):
-//   KROWS  [rows][BK]: chunk c of row r at c ^ sw(r).
+//   KROWS, KBLOCK  [rows][BK]: chunk c of row r at c ^ sw(r).
 //   KCOLS  [BK][rows]: 32-byte segment s of row k at s ^ f(k), f from the
 //          k bits that differ within one transposing read.
 #pragma once
@@ -27,7 +31,7 @@
 
 namespace mm {
 
-enum { KROWS = 0, KCOLS = 1 };
+enum { KROWS = 0, KCOLS = 1, KBLOCK = 2 };
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf8;
 typedef __attribute__((ext_vector_type(8))) _Float16 hf8;
@@ -50,7 +54,8 @@ __device__ __forceinline__ f4 mma(s8 a, s8 b, f4 c) {
 //   p        first element (of the high part)
 //   lo       distance in elements to the low part (SEG = 3)
 //   ld       elements between rows as they lie
-//   rows     rows that may be read (KROWS: of the operand, KCOLS: its k)
+//   rows     rows that may be read (KROWS: of the operand, KCOLS: its k);
+//            KBLOCK: of a block, a multiple of the tile's
 //   cols     KCOLS: operand rows (columns as they lie) that may be read, a
 //            multiple of 8
 // Reads past `rows` and `cols` are clamped to the last ones.
@@ -69,8 +74,14 @@ struct Tile {
   static constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN;
   static constexpr int THREADS = 64 * WAVES_M * WAVES_N;
   static constexpr int FM = WM / 16, FN = WN / 16;
+  // waves on a SIMD that the registers have to leave room for: two
+  // workgroups of four or eight waves on a CU, or one of sixteen
+  static constexpr int OCC = THREADS == 1024 ? 4 : THREADS / 128;
   static constexpr int STAGE_BYTES = (BM + BN) * BK * 2;
-  static constexpr int LDS_BYTES = ST * STAGE_BYTES;
+  // a 16-bit tile on its way out: rows 16 bytes apart from a bank's
+  static constexpr int OUT_ROW = BN * 2 + 16;
+  static constexpr int LDS_BYTES = ST * STAGE_BYTES > BM * OUT_ROW
+                                       ? ST * STAGE_BYTES : BM * OUT_ROW;
 };
 
 template <int BK>
@@ -101,7 +112,8 @@ struct Stager {
   __device__ __forceinline__ void init(const Operand& o, int r0) {
     ld2 = o.ld * 2;
     rows = o.rows;
-    const ushort* base = o.p + (L == KROWS ? (long)r0 * o.ld : (long)r0);
+    const ushort* base =
+        o.p + (L == KROWS ? (long)r0 * o.ld : L == KCOLS ? (long)r0 : 0L);
     const long left = (L == KROWS ? (long)(o.rows - r0) : (long)o.rows) * ld2;
     const int bytes = (int)(left < 0x7fffffffL ? left : 0x7fffffffL);
     rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<ushort*>(base), 0,
@@ -111,7 +123,11 @@ struct Stager {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + i * THREADS;
-      if constexpr (L == KROWS) {
+      if constexpr (L == KBLOCK) {
+        static_assert(BK == 32, "blocks of 32 k");
+        const int r = c / 4;
+        off[i] = (r0 + r) * 64 + (((c % 4) ^ row_swizzle<BK>(r)) * 16);
+      } else if constexpr (L == KROWS) {
         constexpr int S = BK / 8;
         int r = c / S;
         const int src = (c % S) ^ row_swizzle<BK>(r);
@@ -133,7 +149,9 @@ struct Stager {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       int v;
-      if constexpr (L == KROWS) {
+      if constexpr (L == KBLOCK) {
+        v = off[i] + k0 * 2 * rows;
+      } else if constexpr (L == KROWS) {
         v = off[i] + k0 * 2;
       } else {
         int k = (threadIdx.x + i * THREADS) / (R / 8) + k0;
@@ -149,10 +167,19 @@ struct Stager {
   }
 };
 
+// The transposing read.  The compiler knows nothing of its operand and would
+// wait for all loads into LDS before it, also those of the next stage; the
+// restrict gives it the alias information that keeps it from that.  The
+// waits that are needed stand in product().
+typedef __attribute__((address_space(3))) s4 lds_s4;
+__device__ __forceinline__ s4 read_transposed(lds_s4* __restrict__ p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+}
+
 template <int R, int L, int BK>
 __device__ __forceinline__ s8 frag(const char* lds, int r, int kk,
                                    int lane) {
-  if constexpr (L == KROWS) {
+  if constexpr (L != KCOLS) {
     const int row = r + (lane & 15);
     const int c = (kk * 4 + (lane >> 4)) ^ row_swizzle<BK>(row);
     return *reinterpret_cast<const s8*>(lds + row * (BK * 2) + c * 16);
@@ -161,10 +188,8 @@ __device__ __forceinline__ s8 frag(const char* lds, int r, int kk,
     const int k = kk * 32 + (lane >> 4) * 8 + (i >> 2);
     const int seg = (r >> 4) ^ col_swizzle<R>(k);
     const char* at = lds + k * (R * 2) + seg * 32 + (i & 3) * 8;
-    typedef __attribute__((address_space(3))) s4 lds_s4;
-    const s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
-    const s4 v =
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 4 * R * 2));
+    const s4 u = read_transposed((lds_s4*)at);
+    const s4 v = read_transposed((lds_s4*)(at + 4 * R * 2));
     return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
@@ -249,12 +274,61 @@ __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
   barrier();  // the caller may use the LDS
 }
 
+// Writes a tile of 16-bit values, through LDS so that a row goes out in one
+// piece: value(i, j) gives the four values of fragment (i, j) of this lane.
+// Rows and columns from `rows` and `cols` on are left out; `out` and `ld` are
+// multiples of 8 elements, and so is cols unless the tile is cut there.
+template <class C, typename F>
+__device__ __forceinline__ void store_tile(char* lds, ushort* out, long ld,
+                                           int rows, int cols, F value) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int wm = (wave / C::WAVES_N) * C::WM;
+  const int wn = (wave % C::WAVES_N) * C::WN;
+#pragma unroll
+  for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+      *reinterpret_cast<ushort4*>(
+          lds + (wm + i * 16 + (lane & 15)) * C::OUT_ROW +
+          (wn + j * 16 + (lane >> 4) * 4) * 2) = value(i, j);
+  __syncthreads();
+  constexpr int PER_ROW = C::BN / 8;
+#pragma unroll 4
+  for (int c = threadIdx.x; c < C::BM * PER_ROW; c += C::THREADS) {
+    const int r = c / PER_ROW, q = (c % PER_ROW) * 8;
+    if (r >= rows || q >= cols) continue;
+    const s8 v = *reinterpret_cast<const s8*>(lds + r * C::OUT_ROW + q * 2);
+    if (q + 8 <= cols) {
+      *reinterpret_cast<s8*>(out + r * ld + q) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (q + e < cols) out[r * ld + q + e] = (ushort)v[e];
+    }
+  }
+}
+
 // Spreads a flat block id over the 8 dies so that each die works on one
 // contiguous range of tiles: neighbours then share operands in its L2.
 __device__ __forceinline__ int die_contiguous(int bid, int n) {
   const int q = n / 8, r = n % 8;
   const int die = bid % 8, pos = bid / 8;
   return (die < r ? die * (q + 1) : r * (q + 1) + (die - r) * q) + pos;
+}
+
+// sum over the 16 lanes that hold the rows of a fragment
+__device__ __forceinline__ float sum16(float v) {
+  const auto add = [&](int moved) { v += __builtin_bit_cast(float, moved); };
+  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF,
+                                  0xF, true));   // lanes 1 0 3 2
+  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF,
+                                  0xF, true));   // lanes 2 3 0 1
+  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF,
+                                  0xF, true));   // mirrored in 8
+  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF,
+                                  0xF, true));   // mirrored in 16
+  return v;
 }
 
 // hi/lo fp16 parts of a value

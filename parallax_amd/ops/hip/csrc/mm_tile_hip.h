@@ -1,0 +1,348 @@
+// !!! This is a file automatically generated by hipify!!!
+#include "hip/hip_runtime.h"
+// A matrix-product tile for kernels that fuse something into the product:
+// acc[BM x BN] = sum_k A[m, k] * B[n, k], 16-bit operands (bf16 or fp16),
+// fp32 sums, one workgroup per tile.  The kernel that includes this owns
+// the grid, the operands' scaling and what becomes of the sums.
+//
+//   * An operand lies k-contiguous ([rows][K], KROWS), k-strided ([K][rows],
+//     KCOLS) or in blocks of 32 k ([K/32][rows][32], KBLOCK).  The first and
+//     the third are read from LDS with ds_read_b128, the second with the
+//     transposing ds_read_b64_tr_b16, which hands a lane four k of one row,
+//     so no operand is ever transposed in memory.  A stage of 32 k takes 64
+//     bytes of a k-contiguous row, half of what memory hands out at a time;
+//     blocks make that one piece (256 x 128 tile, 2560 x 32768 x 512: 86 us
+//     with rows, 74 us with the first operand in blocks).
+//   * SEG = 3 multiplies operands that are split into a high and a low fp16
+//     part (value = hi + lo, 22 bits): the k loop runs over lo*hi, hi*lo and
+//     hi*hi.  The dropped lo*lo is 2^-22 of a product.
+//   * Operands go from memory to LDS directly (buffer loads, 16 B a lane)
+//     into ST buffers; a wait leaves ST-2 stages in flight, and one barrier
+//     a stage both publishes stage k and frees the buffer of stage k-1.
+//   * The operands are swapped in the matrix instruction, so a lane holds
+//     four neighbouring n of one m: rows reduce over registers and two
+//     shuffles, and four results go out in one store.
+//
+// LDS layouts (16-byte chunks, permuted so that neither read conflicts):
+//   KROWS, KBLOCK  [rows][BK]: chunk c of row r at c ^ sw(r).
+//   KCOLS  [BK][rows]: 32-byte segment s of row k at s ^ f(k), f from the
+//          k bits that differ within one transposing read.
+#pragma once
+
+#include "common.h"
+
+namespace mm {
+
+enum { KROWS = 0, KCOLS = 1, KBLOCK = 2 };
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf8;
+typedef __attribute__((ext_vector_type(8))) _Float16 hf8;
+typedef __attribute__((ext_vector_type(8))) short s8;
+typedef __attribute__((ext_vector_type(4))) short s4;
+typedef __attribute__((ext_vector_type(4))) float f4;
+
+template <bool BF>
+__device__ __forceinline__ f4 mma(s8 a, s8 b, f4 c) {
+  if constexpr (BF) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        __builtin_bit_cast(hf8, a), __builtin_bit_cast(hf8, b), c, 0, 0, 0);
+  }
+}
+
+// One operand of a product.
+//   p        first element (of the high part)
+//   lo       distance in elements to the low part (SEG = 3)
+//   ld       elements between rows as they lie
+//   rows     rows that may be read (KROWS: of the operand, KCOLS: its k);
+//            KBLOCK: of a block, a multiple of the tile's
+//   cols     KCOLS: operand rows (columns as they lie) that may be read, a
+//            multiple of 8
+// Reads past `rows` and `cols` are clamped to the last ones.
+struct Operand {
+  const ushort* p;
+  long lo;
+  int ld;
+  int rows;
+  int cols;
+};
+
+template <int BM_, int BN_, int WM_, int WN_, int BK_, int ST_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BK = BK_, ST = ST_;
+  static constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN;
+  static constexpr int THREADS = 64 * WAVES_M * WAVES_N;
+  static constexpr int FM = WM / 16, FN = WN / 16;
+  // waves on a SIMD that the registers have to leave room for: two
+  // workgroups of four or eight waves on a CU, or one of sixteen
+  static constexpr int OCC = THREADS == 1024 ? 4 : THREADS / 128;
+  static constexpr int STAGE_BYTES = (BM + BN) * BK * 2;
+  // a 16-bit tile on its way out: rows 16 bytes apart from a bank's
+  static constexpr int OUT_ROW = BN * 2 + 16;
+  static constexpr int LDS_BYTES = ST * STAGE_BYTES > BM * OUT_ROW
+                                       ? ST * STAGE_BYTES : BM * OUT_ROW;
+};
+
+template <int BK>
+__device__ __forceinline__ int row_swizzle(int r) {
+  return BK == 32 ? ((-(r >> 2)) & 3) : (r & 7);
+}
+
+template <int R>
+__device__ __forceinline__ int col_swizzle(int k) {
+  if constexpr (R == 64) {
+    return ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
+  } else {
+    return (k & 3) | (((k >> 3) & 1) << 2);
+  }
+}
+
+// Copies one operand's [R x BK] piece of a stage into LDS.
+template <int R, int L, int BK, int THREADS>
+struct Stager {
+  static constexpr int PER = R * BK * 2 / 16 / THREADS;
+  static_assert(PER >= 1 && PER * THREADS * 16 == R * BK * 2,
+                "a stage has to be whole 16-byte pieces for every thread");
+  __amdgpu_buffer_rsrc_t rs, rs_lo;
+  int off[PER];    // KROWS: byte offset; KCOLS: column byte offset
+  int ld2;
+  int rows;
+
+  __device__ __forceinline__ void init(const Operand& o, int r0) {
+    ld2 = o.ld * 2;
+    rows = o.rows;
+    const ushort* base =
+        o.p + (L == KROWS ? (long)r0 * o.ld : L == KCOLS ? (long)r0 : 0L);
+    const long left = (L == KROWS ? (long)(o.rows - r0) : (long)o.rows) * ld2;
+    const int bytes = (int)(left < 0x7fffffffL ? left : 0x7fffffffL);
+    rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<ushort*>(base), 0,
+                                           bytes, 0x00027000);
+    rs_lo = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<ushort*>(base + o.lo), 0, bytes, 0x00027000);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = threadIdx.x + i * THREADS;
+      if constexpr (L == KBLOCK) {
+        static_assert(BK == 32, "blocks of 32 k");
+        const int r = c / 4;
+        off[i] = (r0 + r) * 64 + (((c % 4) ^ row_swizzle<BK>(r)) * 16);
+      } else if constexpr (L == KROWS) {
+        constexpr int S = BK / 8;
+        int r = c / S;
+        const int src = (c % S) ^ row_swizzle<BK>(r);
+        if (r > o.rows - 1 - r0) r = o.rows - 1 - r0;
+        off[i] = r * ld2 + src * 16;
+      } else {
+        constexpr int S = R / 8;
+        const int k = c / S;
+        const int src = (c % S) ^ (col_swizzle<R>(k) << 1);
+        int col = src * 8;
+        if (col > o.cols - 8 - r0) col = o.cols - 8 - r0;
+        off[i] = col * 2;
+      }
+    }
+  }
+
+  // the stage that starts at k0, of the high or the low part
+  __device__ __forceinline__ void load(char* lds, int k0, bool lo) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int v;
+      if constexpr (L == KBLOCK) {
+        v = off[i] + k0 * 2 * rows;
+      } else if constexpr (L == KROWS) {
+        v = off[i] + k0 * 2;
+      } else {
+        int k = (threadIdx.x + i * THREADS) / (R / 8) + k0;
+        if (k > rows - 1) k = rows - 1;
+        v = off[i] + k * ld2;
+      }
+      // each wave writes 1 KiB in lane order from its own base
+      char* dst = lds + i * THREADS * 16 + (threadIdx.x & ~63) * 16;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          lo ? rs_lo : rs,
+          (__attribute__((address_space(3))) void*)dst, 16, v, 0, 0, 0);
+    }
+  }
+};
+
+// The transposing read.  The compiler knows nothing of its operand and would
+// wait for all loads into LDS before it, also those of the next stage; the
+// restrict gives it the alias information that keeps it from that.  The
+// waits that are needed stand in product().
+typedef __attribute__((address_space(3))) s4 lds_s4;
+__device__ __forceinline__ s4 read_transposed(lds_s4* __restrict__ p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+}
+
+template <int R, int L, int BK>
+__device__ __forceinline__ s8 frag(const char* lds, int r, int kk,
+                                   int lane) {
+  if constexpr (L != KCOLS) {
+    const int row = r + (lane & 15);
+    const int c = (kk * 4 + (lane >> 4)) ^ row_swizzle<BK>(row);
+    return *reinterpret_cast<const s8*>(lds + row * (BK * 2) + c * 16);
+  } else {
+    const int i = lane & 15;
+    const int k = kk * 32 + (lane >> 4) * 8 + (i >> 2);
+    const int seg = (r >> 4) ^ col_swizzle<R>(k);
+    const char* at = lds + k * (R * 2) + seg * 32 + (i & 3) * 8;
+    const s4 u = read_transposed((lds_s4*)at);
+    const s4 v = read_transposed((lds_s4*)(at + 4 * R * 2));
+    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// acc[i][j] of wave (wm, wn): element (m, n) with
+//   m = m0 + wm + i*16 + (lane & 15), n = n0 + wn + j*16 + (lane>>4)*4 + r.
+// k runs over [k0, k1), both multiples of BK, of each segment.
+template <class C, int AL, int BL, int SEG, bool BF>
+__device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
+                                        const Operand& b, int n0, int k0,
+                                        int k1, f4 (&acc)[C::FM][C::FN]) {
+  constexpr int BK = C::BK, ST = C::ST, T = C::THREADS;
+  Stager<C::BM, AL, BK, T> sa;
+  Stager<C::BN, BL, BK, T> sb;
+  sa.init(a, m0);
+  sb.init(b, n0);
+  constexpr int LOADS = Stager<C::BM, AL, BK, T>::PER +
+                        Stager<C::BN, BL, BK, T>::PER;
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int wm = (wave / C::WAVES_N) * C::WM;
+  const int wn = (wave % C::WAVES_N) * C::WN;
+  const int per = (k1 - k0) / BK;
+  const int total = per * SEG;
+
+  int ls = 0, lk = k0, lbuf = 0;  // what is staged next
+  auto stage = [&]() {
+    char* at = lds + lbuf * C::STAGE_BYTES;
+    sa.load(at, lk, SEG == 3 && ls == 0);
+    sb.load(at + C::BM * BK * 2, lk, SEG == 3 && ls == 1);
+    lk += BK;
+    if (SEG > 1 && lk == k1) {
+      lk = k0;
+      ++ls;
+    }
+    lbuf = lbuf + 1 == ST ? 0 : lbuf + 1;
+  };
+
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) {
+    if (s < total) stage();
+  }
+  int buf = 0;
+  for (int t = 0; t < total; ++t) {
+    if (t + ST - 1 <= total) {
+      wait_loads<(ST - 2) * LOADS>();
+    } else {
+      wait_loads<0>();
+    }
+    barrier();
+    if (t + ST - 1 < total) stage();
+    const char* pa = lds + buf * C::STAGE_BYTES;
+    const char* pb = pa + C::BM * BK * 2;
+    buf = buf + 1 == ST ? 0 : buf + 1;
+#pragma unroll
+    for (int kk = 0; kk < BK / 32; ++kk) {
+      s8 fa[C::FM], fb[C::FN];
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j)
+        fb[j] = frag<C::BN, BL, BK>(pb, wn + j * 16, kk, lane);
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+        fa[i] = frag<C::BM, AL, BK>(pa, wm + i * 16, kk, lane);
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j)
+          acc[i][j] = mma<BF>(fb[j], fa[i], acc[i][j]);
+    }
+  }
+  barrier();  // the caller may use the LDS
+}
+
+// Writes a tile of 16-bit values, through LDS so that a row goes out in one
+// piece: value(i, j) gives the four values of fragment (i, j) of this lane.
+// Rows and columns from `rows` and `cols` on are left out; `out` and `ld` are
+// multiples of 8 elements, and so is cols unless the tile is cut there.
+template <class C, typename F>
+__device__ __forceinline__ void store_tile(char* lds, ushort* out, long ld,
+                                           int rows, int cols, F value) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int wm = (wave / C::WAVES_N) * C::WM;
+  const int wn = (wave % C::WAVES_N) * C::WN;
+#pragma unroll
+  for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+      *reinterpret_cast<ushort4*>(
+          lds + (wm + i * 16 + (lane & 15)) * C::OUT_ROW +
+          (wn + j * 16 + (lane >> 4) * 4) * 2) = value(i, j);
+  __syncthreads();
+  constexpr int PER_ROW = C::BN / 8;
+#pragma unroll 4
+  for (int c = threadIdx.x; c < C::BM * PER_ROW; c += C::THREADS) {
+    const int r = c / PER_ROW, q = (c % PER_ROW) * 8;
+    if (r >= rows || q >= cols) continue;
+    const s8 v = *reinterpret_cast<const s8*>(lds + r * C::OUT_ROW + q * 2);
+    if (q + 8 <= cols) {
+      *reinterpret_cast<s8*>(out + r * ld + q) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (q + e < cols) out[r * ld + q + e] = (ushort)v[e];
+    }
+  }
+}
+
+// Spreads a flat block id over the 8 dies so that each die works on one
+// contiguous range of tiles: neighbours then share operands in its L2.
+__device__ __forceinline__ int die_contiguous(int bid, int n) {
+  const int q = n / 8, r = n % 8;
+  const int die = bid % 8, pos = bid / 8;
+  return (die < r ? die * (q + 1) : r * (q + 1) + (die - r) * q) + pos;
+}
+
+// sum over the 16 lanes that hold the rows of a fragment
+__device__ __forceinline__ float sum16(float v) {
+  const auto add = [&](int moved) { v += __builtin_bit_cast(float, moved); };
+  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF,
+                                  0xF, true));   // lanes 1 0 3 2
+  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF,
+                                  0xF, true));   // lanes 2 3 0 1
+  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF,
+                                  0xF, true));   // mirrored in 8
+  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF,
+                                  0xF, true));   // mirrored in 16
+  return v;
+}
+
+// hi/lo fp16 parts of a value
+__device__ __forceinline__ void split(float v, ushort& hi, ushort& lo) {
+  const _Float16 h = (_Float16)v;
+  const _Float16 l = (_Float16)(v - (float)h);
+  hi = __builtin_bit_cast(ushort, h);
+  lo = __builtin_bit_cast(ushort, l);
+}
+
+__device__ __forceinline__ float half_bits(ushort h) {
+  return (float)__builtin_bit_cast(_Float16, h);
+}
+
+}  // namespace mm
