@@ -169,9 +169,8 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
 std::vector<at::Tensor> linear_ce_bwd(
     const at::Tensor& dloss, const at::Tensor& x, const at::Tensor& w,
     const c10::optional<at::Tensor>& bias, const at::Tensor& labels,
-    const at::Tensor& lse, const at::Tensor& count, const at::Tensor& tops,
-    int64_t ignore, double smoothing, int64_t reduction, bool want_dx,
-    bool want_dw, bool want_db);
+    const at::Tensor& saved, int64_t ignore, double smoothing,
+    int64_t reduction, bool want_dx, bool want_dw, bool want_db);
 
 // newton_schulz.hip
 void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,

@@ -31,6 +31,9 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <mutex>
+#include <set>
+
 #include "mm_tile.h"
 
 namespace {
@@ -123,48 +126,135 @@ __device__ __forceinline__ float scale_to_half(float top) {
 }
 
 // --- laying out an operand --------------------------------------------------
-// out[rows_out][dp] 16-bit, zeros behind d and behind the rows, and the same
-// in blocks of 32 columns where `blocks` is given; fp32 input: a high and a
-// low fp16 plane, scaled by a power of two.  One wave a row.
-// labels (x only): rows whose label is `ignore` become zeros.
-// fixed: the scale of every row (fp32 only) is found from top[0..ntop);
-// otherwise each row has its own.  inv[r] = 1 / scale.  bmax: the largest
-// |value| of each block, for a later `fixed` call.
-template <int SEG>
-__global__ __launch_bounds__(256) void lce_pack_kernel(
-    const void* __restrict__ src, int type, long rs, long cs, long rows,
-    int d, ushort* __restrict__ out, ushort* __restrict__ blocks, int dp,
-    long rows_out, const int64_t* __restrict__ labels, int64_t ignore, bool fixed,
-    const float* __restrict__ top, int ntop, float* __restrict__ inv,
-    float* __restrict__ bmax) {
+
+// What the gradient needs of a row.  Rows that do not count: an infinite l
+// makes their exponentials 0, and g = 0.
+struct Row {
+  float l;   // log2 e lse
+  float g;   // what the row's G is multiplied by
+  int y;     // label
+  float xs;  // scale to undo
+};
+
+struct Pack {
+  const void* src;
+  int type;
+  long rs, cs;        // strides in elements
+  long rows;          // as they are; zeros up to rows_out
+  int d;              // zeros up to dp
+  bool eight;         // 16-byte pieces can be read
+  int dp;
+  long rows_out;
+  ushort* out;        // [rows_out][dp], fp32: in pairs of parts
+  ushort* blocks;     // [dp / 32][rows_out][32] (16-bit types)
+  const int64_t* labels;  // x only: rows of `ignore` become zeros
+  int64_t ignore;
+  // fp32: the scale of every row is found from top[0..ntop) where given,
+  // else each row has its own; inv[r] = 1 / scale; bmax: the largest value
+  // of each block, for a later call's `top`
+  const float* top;
+  int ntop;
+  float* inv;
+  float* bmax;
+  unsigned* zero;     // a counter to clear
+  // backward: the rows, and sc = {S, 1/S} for 16-bit G
+  Row* row;
+  const float* dloss; // one or (each) of every row
+  bool each;
+  const float* count;
+  const float* lse;
+  long V;
+  float* sc;
+};
+
+__device__ __forceinline__ void load8(const Pack& p, const char* src, long c,
+                                      float (&v)[8]) {
+  if (p.eight && p.type == 2) {
+    const f4 a = *reinterpret_cast<const f4*>(src + c * 4);
+    const f4 b = *reinterpret_cast<const f4*>(src + c * 4 + 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[e];
+      v[4 + e] = b[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v[e] = c + e < p.d ? load_as(src, (c + e) * p.cs, p.type) : 0.f;
+  }
+}
+
+// One wave a row, eight values a lane at a time.
+template <int PARTS>
+__global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
   __shared__ float scratch[PX_BLOCK / WAVE];
   const int lane = threadIdx.x & 63;
+  const int size = PARTS == 2 ? 4 : 2;
   float scale = 1.f, most = 0.f;
-  if (SEG == 3 && fixed) {
+  if (PARTS == 2 && p.top != nullptr) {
     float t = 0.f;
-    for (int i = threadIdx.x; i < ntop; i += blockDim.x) t = fmaxf(t, top[i]);
+    for (int i = threadIdx.x; i < p.ntop; i += blockDim.x)
+      t = fmaxf(t, p.top[i]);
     scale = scale_to_half(block_reduce_max(t, scratch));
   }
-  for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows_out;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (p.zero) *p.zero = 0;
+    if (p.sc && !p.each) {
+      // |softmax - target| <= 1, so S |G| stays below 2^14
+      const float g = p.dloss[0] / (p.count ? p.count[0] : 1.f);
+      const float s = p.type != 0 ? scale_to_half(fabsf(g)) : 1.f;
+      p.sc[0] = s;
+      p.sc[1] = 1.f / s;
+    }
+  }
+  for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < p.rows_out;
        r += (long)gridDim.x * 4) {
-    const bool live =
-        r < rows && (labels == nullptr || labels[r] != ignore);
-    if constexpr (SEG == 1) {
-      for (int c = lane; c < dp; c += 64) {
-        ushort u = 0;
-        if (live && c < d)
-          u = static_cast<const ushort*>(src)[r * rs + c * cs];
-        if (out) out[r * dp + c] = u;
-        if (blocks) blocks[((c >> 5) * rows_out + r) * 32 + (c & 31)] = u;
+    bool live = r < p.rows;
+    if (p.labels && live) {
+      const int64_t y = p.labels[r];
+      live = y != p.ignore;
+      if (p.row && lane == 0) {
+        Row row = {INFINITY, 0.f, 0, 1.f};
+        row.y = (int)(y < 0 ? 0 : (y >= p.V ? p.V - 1 : y));
+        if (live) {
+          row.g = p.dloss[p.each ? r : 0] / (p.count ? p.count[0] : 1.f);
+          row.l = p.lse[r] * kLog2e;
+        }
+        p.row[r] = row;
+      }
+    } else if (p.row && lane == 0) {
+      p.row[r] = Row{INFINITY, 0.f, 0, 1.f};
+    }
+    const char* src = static_cast<const char*>(p.src) + r * p.rs * size;
+    if constexpr (PARTS == 1) {
+      for (int c = lane * 8; c < p.dp; c += 512) {
+        s8 u = {};
+        if (live && p.eight && c < p.d) {
+          u = *reinterpret_cast<const s8*>(src + c * 2);
+        } else if (live) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c + e < p.d)
+              u[e] = reinterpret_cast<const short*>(src)[(c + e) * p.cs];
+        }
+        if (p.out) *reinterpret_cast<s8*>(p.out + r * p.dp + c) = u;
+        if (p.blocks)
+          *reinterpret_cast<s8*>(
+              p.blocks + ((long)(c >> 5) * p.rows_out + r) * 32 + (c & 31)) =
+              u;
       }
     } else {
-      const float* s = static_cast<const float*>(src) + r * rs;
-      if (!fixed) {
+      if (p.top == nullptr) {
         float t = 0.f;
         if (live) {
-          for (int c = lane; c < d; c += 64) {
-            const float v = fabsf(s[c * cs]);
-            if (v < INFINITY) t = fmaxf(t, v);
+          for (int c = lane * 8; c < p.d; c += 512) {
+            float v[8];
+            load8(p, src, c, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float a = fabsf(v[e]);
+              if (a < INFINITY) t = fmaxf(t, a);
+            }
           }
         }
 #pragma unroll
@@ -172,34 +262,57 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(
         most = fmaxf(most, t);
         scale = scale_to_half(t);
       }
-      if (lane == 0) inv[r] = 1.f / scale;
-      for (int c = lane; c < dp; c += 64) {
-        const float v = live && c < d ? s[c * cs] * scale : 0.f;
-        ushort h, l;
-        split(v, h, l);
-        const long at = ((c >> 5) * rows_out + r) * 32 + (c & 31);
-        if (out) {
-          out[r * dp + c] = h;
-          out[rows_out * dp + r * dp + c] = l;
+      if (lane == 0) p.inv[r] = 1.f / scale;
+      for (int c = lane * 8; c < p.dp; c += 512) {
+        float v[8] = {};
+        if (live && c < p.d) load8(p, src, c, v);
+        s8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          ushort hi, lo;
+          split(v[e] * scale, hi, lo);
+          h[e] = hi;
+          l[e] = lo;
         }
-        if (blocks) {
-          blocks[at] = h;
-          blocks[rows_out * dp + at] = l;
-        }
+        ushort* at = p.out + r * p.dp * 2 + (c >> 5) * 64 + (c & 31);
+        *reinterpret_cast<s8*>(at) = h;
+        *reinterpret_cast<s8*>(at + 32) = l;
       }
     }
   }
-  if (SEG == 3 && bmax != nullptr) {
+  if (PARTS == 2 && p.bmax != nullptr) {
     most = block_reduce_max(most, scratch);
-    if (threadIdx.x == 0) bmax[blockIdx.x] = most;
+    if (threadIdx.x == 0) p.bmax[blockIdx.x] = most;
+  }
+}
+
+// sc = {S, 1/S} where every row has a gradient of its own
+__global__ __launch_bounds__(1024) void lce_scale_kernel(
+    const float* __restrict__ dloss, const int64_t* __restrict__ labels,
+    int64_t ignore, int n, bool half, float* __restrict__ sc) {
+  __shared__ float red[16];
+  float most = 0.f;
+  for (int i = threadIdx.x; i < n; i += 1024)
+    if (labels[i] != ignore) most = fmaxf(most, fabsf(dloss[i]));
+  most = block_reduce_max(most, red);
+  if (threadIdx.x == 0) {
+    const float s = half ? scale_to_half(most) : 1.f;
+    sc[0] = s;
+    sc[1] = 1.f / s;
   }
 }
 
 // --- forward ----------------------------------------------------------------
 
+struct Vec {  // a tensor's values by row and column
+  const void* p;
+  int type;
+  long rs, cs;
+};
+
 struct Logits {
   Operand x, w;
-  const float* xinv;  // SEG 3: scales to undo, by row and by word
+  const float* xinv;  // parts: scales to undo, by row and by word
   const float* winv;
   Bias bias;
   int n;     // rows
@@ -208,10 +321,10 @@ struct Logits {
 };
 
 // max, sum of exp and (SMOOTH) total of each row, in powers of 2, over `tpb` tiles of words
-template <class C, int XL, int SEG, bool BF, bool SMOOTH>
+template <class C, int XL, int PARTS, bool BF, bool SMOOTH>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
-    Logits p, float* __restrict__ part, int part_rows, int vb0,
-    int nblocks, int nmt, int nvb, int tpb) {
+    Logits p, float* __restrict__ part, int vb0, int nblocks, int nmt,
+    int nvb, int tpb) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // the row tiles of one block of words run next to each other: the words
   // come from memory once
@@ -229,7 +342,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
     mx[i] = -INFINITY;
     se[i] = tot[i] = 0.f;
     xs[i] = 1.f;
-    if (SEG == 3) {
+    if (PARTS == 2) {
       int m = m0 + wm + i * 16 + (lane & 15);
       if (m > p.n - 1) m = p.n - 1;
       xs[i] = p.xinv[m];
@@ -239,7 +352,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
     const int n0 = (vb * tpb + q) * C::BN;
     if (n0 >= p.vp) break;
     f4 acc[C::FM][C::FN] = {};
-    product<C, XL, KROWS, SEG, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
+    product<C, XL, KROWS, PARTS, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
     float add[C::FN][4], ws[C::FN][4];
 #pragma unroll
     for (int j = 0; j < C::FN; ++j)
@@ -249,7 +362,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int v = n0 + wn + j * 16 + (lane >> 4) * 4 + r;
-        ws[j][r] = SEG == 3 && v < p.vp ? p.winv[v] * kLog2e : kLog2e;
+        ws[j][r] = PARTS == 2 && v < p.vp ? p.winv[v] * kLog2e : kLog2e;
       }
     if (n0 + C::BN > p.vp) {  // words behind the last one
 #pragma unroll
@@ -268,7 +381,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
       for (int j = 0; j < C::FN; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float z = fmaf(SEG == 3 ? acc[i][j][r] * xs[i]
+          const float z = fmaf(PARTS == 2 ? acc[i][j][r] * xs[i]
                                         : acc[i][j][r],
                                ws[j][r], add[j][r]);
           acc[i][j][r] = z;
@@ -323,156 +436,127 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
       m = top;
       t += at[2];
     }
-    // planes [max | sum | total], each [blocks of words][rows]
-    const long at = (long)(vb0 + vb) * part_rows + m0 + r;
-    part[at] = m;
-    part[at + (long)part_rows * nblocks] = s;
-    if (SMOOTH) part[at + 2 * (long)part_rows * nblocks] = t;
+    // of a row next to one another, for the join
+    float* at = part + ((long)(m0 + r) * nblocks + vb0 + vb) * (SMOOTH ? 4 : 2);
+    if (SMOOTH) {
+      *reinterpret_cast<f4*>(at) = f4{m, s, t, 0.f};
+    } else {
+      *reinterpret_cast<float2*>(at) = make_float2(m, s);
+    }
   }
 }
 
-// Joins the partial sums of 16 rows; the label's logit; the loss.
-__global__ __launch_bounds__(256) void lce_join_kernel(
-    const float* __restrict__ part, int nvb, int part_rows,
-    const void* __restrict__ x, int xtype, long xrs, long xcs,
-    const void* __restrict__ w, int wtype, long wrs, long wcs,
-    const void* __restrict__ bias, int btype, long bstride, int d,
-    const int64_t* __restrict__ labels, int64_t ignore, long V, float eps,
-    float* __restrict__ loss, float* __restrict__ lse, int n) {
-  __shared__ float sm[3][16][17];
-  __shared__ float zy[16];
-  const int row = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int r0 = blockIdx.x * 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long plane = (long)part_rows * nvb;
-  float m = -INFINITY, s = 0.f, t = 0.f;
-  if (r0 + row < n) {
-    for (int b = q; b < nvb; b += 16) {
-      const long at = (long)b * part_rows + r0 + row;
-      const float m2 = part[at], s2 = part[at + plane];
-      const float top = fmaxf(m, m2);
-      const float off = top == -INFINITY ? 0.f : top;
-      s = s * exp2_fast(m - off) + s2 * exp2_fast(m2 - off);
-      m = top;
-      if (eps != 0.f) t += part[at + 2 * plane];
-    }
-  }
-  sm[0][row][q] = m;
-  sm[1][row][q] = s;
-  sm[2][row][q] = t;
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + wave * 4 + i;
-    float a = 0.f;
-    if (r < n && labels[r] != ignore) {
-      const int64_t y0 = labels[r];
-      const long y = y0 < 0 ? 0 : (y0 >= V ? V - 1 : y0);
-      for (int c = lane; c < d; c += 64) {
-        a += load_as(x, r * xrs + c * xcs, xtype) *
-             load_as(w, y * wrs + c * wcs, wtype);
+struct Join {
+  const float* part;
+  int nblocks;
+  Vec x, w, bias;
+  int d, n;
+  const int64_t* labels;
+  int64_t ignore;
+  long V;
+  float eps;
+  float* loss;
+  float* lse;
+  int reduction;     // 0: none, 1: mean, 2: sum
+  unsigned* ticket;
+  float* out;        // the scalar
+  float* count;      // rows that count
+};
+
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  const float off = top == -INFINITY ? 0.f : top;
+  s = s * exp2_fast(m - off) + s2 * exp2_fast(m2 - off);
+  m = top;
+}
+
+// One wave a row: joins its partial sums, takes the label's logit as a dot
+// product, and the loss.  The last workgroup to finish adds the losses up,
+// in the rows' order.
+__global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
+  __shared__ double sd[256];
+  __shared__ int sn[256];
+  __shared__ bool last;
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r < p.n) {
+    float m = -INFINITY, s = 0.f, t = 0.f;
+    for (int b = lane; b < p.nblocks; b += 64) {
+      const long at = (long)r * p.nblocks + b;
+      if (p.eps != 0.f) {
+        const f4 v = reinterpret_cast<const f4*>(p.part)[at];
+        join(m, s, v[0], v[1]);
+        t += v[2];
+      } else {
+        const float2 v = reinterpret_cast<const float2*>(p.part)[at];
+        join(m, s, v.x, v.y);
       }
-      a = wave_reduce_sum(a);
-      if (lane == 0 && bias) a += load_as(bias, y * bstride, btype);
     }
-    if (lane == 0) zy[wave * 4 + i] = a;
+    const int64_t y0 = p.labels[r];
+    const bool live = y0 != p.ignore;
+    const long y = y0 < 0 ? 0 : (y0 >= p.V ? p.V - 1 : y0);
+    float a = 0.f;
+    if (live) {
+      for (int c = lane; c < p.d; c += 64)
+        a += load_as(p.x.p, r * p.x.rs + c * p.x.cs, p.x.type) *
+             load_as(p.w.p, y * p.w.rs + c * p.w.cs, p.w.type);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+      t += __shfl_xor(t, o, 64);
+      a += __shfl_xor(a, o, 64);
+    }
+    if (lane == 0) {
+      if (live && p.bias.p) a += load_as(p.bias.p, y * p.bias.rs, p.bias.type);
+      const float l = m * kLn2 + logf(s);
+      p.lse[r] = l;
+      float out = l - (1.f - p.eps) * a;
+      if (p.eps != 0.f) out -= p.eps * (t * kLn2 / (float)p.V);
+      p.loss[r] = live ? out : 0.f;
+    }
   }
+  if (p.reduction == 0) return;
+  __threadfence();
   __syncthreads();
-  if (threadIdx.x < 16 && r0 + row < n) {
-    for (int b = 1; b < 16; ++b) {
-      const float m2 = sm[0][row][b], s2 = sm[1][row][b];
-      const float top = fmaxf(m, m2);
-      const float off = top == -INFINITY ? 0.f : top;
-      s = s * exp2_fast(m - off) + s2 * exp2_fast(m2 - off);
-      m = top;
-      t += sm[2][row][b];
-    }
-    const float l = m * kLn2 + logf(s);
-    const int r = r0 + row;
-    lse[r] = l;
-    float out = l - (1.f - eps) * zy[row];
-    if (eps != 0.f) out -= eps * (t * kLn2 / (float)V);
-    loss[r] = labels[r] == ignore ? 0.f : out;
-  }
-}
-
-// sum and count of the rows that are not ignored; out[0] = sum or mean,
-// out[1] = count.  One workgroup, fixed order.
-__global__ __launch_bounds__(1024) void lce_total_kernel(
-    const float* __restrict__ loss, const int64_t* __restrict__ labels,
-    int64_t ignore, int n, bool mean, float* __restrict__ out) {
-  __shared__ double sd[1024];
-  __shared__ int sc[1024];
+  if (threadIdx.x == 0)
+    last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   double a = 0.;
   int c = 0;
-  for (int i = threadIdx.x; i < n; i += 1024) {
-    a += loss[i];
-    c += labels[i] != ignore;
+  for (int i = threadIdx.x; i < p.n; i += 256) {
+    a += p.loss[i];
+    c += p.labels[i] != p.ignore;
   }
   sd[threadIdx.x] = a;
-  sc[threadIdx.x] = c;
+  sn[threadIdx.x] = c;
   __syncthreads();
-  for (int o = 512; o > 0; o >>= 1) {
+  for (int o = 128; o > 0; o >>= 1) {
     if (threadIdx.x < o) {
       sd[threadIdx.x] += sd[threadIdx.x + o];
-      sc[threadIdx.x] += sc[threadIdx.x + o];
+      sn[threadIdx.x] += sn[threadIdx.x + o];
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    out[0] = (float)(mean ? sd[0] / sc[0] : sd[0]);
-    out[1] = (float)sc[0];
+    p.out[0] = (float)(p.reduction == 1 ? sd[0] / sn[0] : sd[0]);
+    p.count[0] = (float)sn[0];
   }
 }
 
 // --- backward ---------------------------------------------------------------
 
-// What the gradient needs of a row.  Rows that do not count: an infinite l
-// makes their exponentials 0, and g = 0.
-struct Row {
-  float l;   // log2 e lse
-  float g;   // what the row's G is multiplied by
-  int y;     // label
-  float xs;  // scale to undo
-};
-
-// the rows, and sc = {S, 1/S} for 16-bit G
-__global__ __launch_bounds__(1024) void lce_rows_kernel(
-    const float* __restrict__ dloss, bool scalar,
-    const float* __restrict__ count, const int64_t* __restrict__ labels,
-    int64_t ignore, int n, int n_out, bool half,
-    const float* __restrict__ lse, long V, Row* __restrict__ rows,
-    float* __restrict__ sc) {
-  __shared__ float red[16];
-  const float div = count ? count[0] : 1.f;
-  float most = 0.f;
-  for (int i = threadIdx.x; i < n_out; i += 1024) {
-    Row row = {INFINITY, 0.f, 0, 1.f};
-    if (i < n) {
-      const int64_t y = labels[i];
-      row.y = (int)(y < 0 ? 0 : (y >= V ? V - 1 : y));
-      if (y != ignore) {
-        row.g = dloss[scalar ? 0 : i] / div;
-        row.l = lse[i] * kLog2e;
-      }
-    }
-    rows[i] = row;
-    most = fmaxf(most, fabsf(row.g));
-  }
-  most = block_reduce_max(most, red);
-  if (threadIdx.x == 0) {
-    // |softmax - target| <= 1, so S |G| stays below 2^14
-    const float s = half ? scale_to_half(most) : 1.f;
-    sc[0] = s;
-    sc[1] = 1.f / s;
-  }
-}
-
 // G of one piece, [rows padded to BM][ldg]; zeros outside the matrix.
-// DB: column sums of each row tile into dbp[row tile][ldg].
-template <class C, int XL, int SEG, bool BF, bool DB>
+// DB: column sums of each row tile into dbp[row tile][..], or as they are
+// into db where there is one.
+template <class C, int XL, int PARTS, bool BF, bool DB>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     Logits p, const Row* __restrict__ rows, const float* __restrict__ sc,
-    long V, long v0, float eps, ushort* __restrict__ G, int ldg, long glo,
-    float* __restrict__ dbp, int nmt, int nvt) {
+    long V, long v0, float eps, ushort* __restrict__ G, int ldg,
+    float* __restrict__ dbp, long db_ld, void* __restrict__ db, int db_type,
+    int nmt, int nvt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int bid = die_contiguous(blockIdx.x, nmt * nvt);
   const int mt = bid % nmt, vt = bid / nmt;
@@ -482,10 +566,10 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
   f4 acc[C::FM][C::FN] = {};
-  product<C, XL, KROWS, SEG, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
+  product<C, XL, KROWS, PARTS, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
   const int c0 = n0 + wn + (lane >> 4) * 4;
   const float S = sc[0], uni = eps / (float)V;
-  const float xs = SEG == 3 ? p.xinv[0] : 1.f;  // one for all rows
+  const float xs = PARTS == 2 ? p.xinv[0] : 1.f;  // one for all rows
   float add[C::FN][4], ws[C::FN][4];
 #pragma unroll
   for (int j = 0; j < C::FN; ++j) p.bias.load(add[j], c0 + j * 16, p.vp);
@@ -494,7 +578,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int v = c0 + j * 16 + r;
-      ws[j][r] = SEG == 3 && v < p.vp ? p.winv[v] * kLog2e : kLog2e;
+      ws[j][r] = PARTS == 2 && v < p.vp ? p.winv[v] * kLog2e : kLog2e;
     }
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
@@ -506,7 +590,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     for (int j = 0; j < C::FN; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float z = SEG == 3 ? acc[i][j][r] * xs : acc[i][j][r];
+        const float z = PARTS == 2 ? acc[i][j][r] * xs : acc[i][j][r];
         acc[i][j][r] =
             (exp2_fast(fmaf(z, ws[j][r], add[j][r] - l)) - uni) * gm;
       }
@@ -531,22 +615,18 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
           for (int i = 0; i < C::FM; ++i) acc[i][j][r] = 0.f;
         }
   }
-  ushort* at = G + (long)m0 * ldg + n0;
-  store_tile<C>(smem, at, ldg, C::BM, C::BN, [&](int i, int j) {
-    const f4 v = acc[i][j];
-    if (BF)
-      return make_ushort4(bf16_bits(v[0]), bf16_bits(v[1]), bf16_bits(v[2]),
-                          bf16_bits(v[3]));
-    return make_ushort4(fp16_bits(v[0] * S), fp16_bits(v[1] * S),
-                        fp16_bits(v[2] * S), fp16_bits(v[3] * S));
-  });
-  if (SEG == 3) {
-    __syncthreads();
-    store_tile<C>(smem, at + glo, ldg, C::BM, C::BN, [&](int i, int j) {
-      ushort h, l[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) split(acc[i][j][r] * S, h, l[r]);
-      return make_ushort4(l[0], l[1], l[2], l[3]);
+  if constexpr (PARTS == 2) {
+    store_pairs<C>(smem, G + ((long)m0 * ldg + n0) * 2, 2L * ldg,
+                   [&](int i, int j) { return acc[i][j] * S; });
+  } else {
+    store_tile<C>(smem, G + (long)m0 * ldg + n0, ldg, C::BM, C::BN,
+                  [&](int i, int j) {
+      const f4 v = acc[i][j];
+      if (BF)
+        return make_ushort4(bf16_bits(v[0]), bf16_bits(v[1]),
+                            bf16_bits(v[2]), bf16_bits(v[3]));
+      return make_ushort4(fp16_bits(v[0] * S), fp16_bits(v[1] * S),
+                          fp16_bits(v[2] * S), fp16_bits(v[3] * S));
     });
   }
   if (DB) {
@@ -568,23 +648,27 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     for (int c = threadIdx.x; c < C::BN; c += C::THREADS) {
       float s = red[c];
       for (int w = 1; w < C::WAVES_M; ++w) s += red[w * C::BN + c];
-      dbp[(long)mt * ldg + n0 + c] = s;
+      if (nmt > 1) {
+        dbp[mt * db_ld + n0 + c] = s;
+      } else if (n0 + c < p.vp) {
+        store_as(db, n0 + c, db_type, s);
+      }
     }
   }
 }
 
 __global__ __launch_bounds__(256) void lce_db_kernel(
-    const float* __restrict__ dbp, int nmt, int ldg, int vp, void* db,
+    const float* __restrict__ dbp, int nmt, long ld, long words, void* db,
     int type) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= vp) return;
+  const long v = (long)blockIdx.x * 256 + threadIdx.x;
+  if (v >= words) return;
   float s = 0.f;
-  for (int m = 0; m < nmt; ++m) s += dbp[(long)m * ldg + v];
+  for (int m = 0; m < nmt; ++m) s += dbp[m * ld + v];
   store_as(db, v, type, s);
 }
 
 // dw[v, :] = 1/S sum_n G[n, v] x[n, :]  (G and x both k-strided)
-template <class C, int SEG, bool BF>
+template <class C, int PARTS, bool BF>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
     Operand G, Operand x, int kn, const float* __restrict__ sc,
     const float* __restrict__ xinv, void* __restrict__ dw, int type, int vp,
@@ -593,12 +677,12 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
   const int bid = die_contiguous(blockIdx.x, nmt * nnt);
   const int m0 = bid / nnt * C::BM, n0 = bid % nnt * C::BN;
   f4 acc[C::FM][C::FN] = {};
-  product<C, KCOLS, KCOLS, SEG, BF>(smem, G, m0, x, n0, 0, kn, acc);
+  product<C, KCOLS, KCOLS, PARTS, BF>(smem, G, m0, x, n0, 0, kn, acc);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
-  const float back = sc[1] * (SEG == 3 ? xinv[0] : 1.f);
+  const float back = sc[1] * (PARTS == 2 ? xinv[0] : 1.f);
   if (type != 2 && (d & 7) == 0) {
     store_tile<C>(smem, static_cast<ushort*>(dw) + (long)m0 * d + n0, d,
                   vp - m0, d - n0, [&](int i, int j) {
@@ -632,7 +716,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
 }
 
 // part[slice][n, :] (+)= sum over a slice of the piece's words G[n, v] w[v, :]
-template <class C, int SEG, bool BF>
+template <class C, int PARTS, bool BF>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dx_kernel(
     Operand G, Operand w, int kv, int kslice, float* __restrict__ part,
     int n_rows, int dp, bool first, int nmt, int nnt, int slices) {
@@ -644,7 +728,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dx_kernel(
   const int k1 = k0 + kslice < kv ? k0 + kslice : kv;
   f4 acc[C::FM][C::FN] = {};
   if (k0 < k1)
-    product<C, KROWS, KCOLS, SEG, BF>(smem, G, m0, w, n0, k0, k1, acc);
+    product<C, KROWS, KCOLS, PARTS, BF>(smem, G, m0, w, n0, k0, k1, acc);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
@@ -699,20 +783,62 @@ int type_code(const at::Tensor& t) {
   }
 }
 
+// more than 64 KB of LDS has to be asked for, once a kernel and device
 template <typename K>
 void allow_lds(K kernel, int bytes) {
-  hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (bytes <= 64 * 1024) return;
+  static std::mutex lock;
+  static std::set<std::pair<const void*, int>> done;
+  int device = 0;
+  TORCH_CHECK(hipGetDevice(&device) == hipSuccess, "hipGetDevice failed");
+  const auto key = std::make_pair(reinterpret_cast<const void*>(kernel),
+                                  device);
+  std::lock_guard<std::mutex> hold(lock);
+  if (done.count(key)) return;
+  const hipError_t e = hipFuncSetAttribute(
+      key.first, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  TORCH_CHECK(e == hipSuccess, "linear_ce: ", bytes, " bytes of LDS: ",
+              hipGetErrorString(e));
+  done.insert(key);
 }
 
 const ushort* bits(const at::Tensor& t) {
   return reinterpret_cast<const ushort*>(t.data_ptr());
 }
 
+Vec vec_of(const at::Tensor& t) {
+  return Vec{t.data_ptr(), type_code(t), t.stride(0),
+             t.dim() > 1 ? t.stride(1) : 0};
+}
+
+// One allocation for all of a call's scratch memory.
+class Scratch {
+ public:
+  template <typename T>
+  size_t take(long n) {
+    const size_t at = bytes_;
+    bytes_ += (n * sizeof(T) + 255) / 256 * 256;
+    return at;
+  }
+  void allocate(const at::Tensor& like) {
+    t_ = at::empty({(long)bytes_}, like.options().dtype(at::kByte));
+    base_ = static_cast<char*>(t_.data_ptr());
+  }
+  template <typename T>
+  T* at(size_t offset) const {
+    return reinterpret_cast<T*>(base_ + offset);
+  }
+
+ private:
+  size_t bytes_ = 0;
+  at::Tensor t_;
+  char* base_ = nullptr;
+};
+
 // What the products read: x laid out once, w as it is or piece by piece.
 struct Plan {
   long n, v, d, dp, np;
-  int type, seg;
+  int type, parts;
   bool w_direct;   // w's rows can be read in place
   long w_rows;     // words in a piece of w that is laid out
 };
@@ -725,51 +851,51 @@ Plan make_plan(const at::Tensor& x, const at::Tensor& w) {
   p.dp = up(p.d, 64);
   p.np = up(p.n, 256);
   p.type = type_code(x);
-  p.seg = p.type == 2 ? 3 : 1;
-  p.w_direct = p.seg == 1 && p.d == p.dp && w.stride(1) == 1 &&
+  p.parts = p.type == 2 ? 2 : 1;
+  p.w_direct = p.parts == 1 && p.d == p.dp && w.stride(1) == 1 &&
                w.stride(0) % 8 == 0 && w.stride(0) >= p.d &&
                w.stride(0) < (1 << 22) &&
                reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0;
-  const long words = kSplitBytes / (p.dp * 2 * (p.seg == 3 ? 2 : 1));
+  const long words = kSplitBytes / (p.dp * 2 * p.parts);
   p.w_rows = std::min(up(p.v, 256), std::max(256L, words / 256 * 256));
   return p;
 }
 
 int pack_blocks(long rows) {
-  return (int)std::min<long>(1024, (rows + 3) / 4);
+  return (int)std::min<long>(2048, (rows + 3) / 4);
 }
 
-void pack(const at::Tensor& src, long row0, long rows, long rows_out,
-          const Plan& p, at::Tensor& out, at::Tensor& blocks,
-          const int64_t* labels, int64_t ignore, bool fixed, const at::Tensor& top,
-          at::Tensor& inv, float* bmax, hipStream_t stream) {
-  const char* s = static_cast<const char*>(src.data_ptr()) +
-                  row0 * src.stride(0) * src.element_size();
-  auto launch = [&](auto kernel) {
-    kernel<<<pack_blocks(rows_out), 256, 0, stream>>>(
-        s, p.type, src.stride(0), src.stride(1), rows, (int)p.d,
-        out.defined() ? reinterpret_cast<ushort*>(out.data_ptr()) : nullptr,
-        blocks.defined() ? reinterpret_cast<ushort*>(blocks.data_ptr())
-                         : nullptr,
-        (int)p.dp, rows_out,
-        labels, ignore, fixed,
-        top.defined() ? top.data_ptr<float>() : nullptr,
-        top.defined() ? (int)top.numel() : 0,
-        inv.defined() ? inv.data_ptr<float>() : nullptr, bmax);
-    HIP_CHECK_KERNEL();
-  };
-  if (p.seg == 3) {
-    launch(lce_pack_kernel<3>);
+// the layout of rows row0.. of a tensor
+Pack pack_of(const at::Tensor& t, long row0, long rows, long rows_out,
+             const Plan& p, ushort* out) {
+  Pack k = {};
+  const long size = t.element_size();
+  k.src = static_cast<const char*>(t.data_ptr()) + row0 * t.stride(0) * size;
+  k.type = p.type;
+  k.rs = t.stride(0);
+  k.cs = t.stride(1);
+  k.rows = rows;
+  k.d = (int)p.d;
+  k.eight = k.cs == 1 && p.d % 8 == 0 && (k.rs * size) % 16 == 0 &&
+            reinterpret_cast<uintptr_t>(k.src) % 16 == 0;
+  k.dp = (int)p.dp;
+  k.rows_out = rows_out;
+  k.out = out;
+  return k;
+}
+
+void pack(const Pack& k, hipStream_t stream) {
+  if (k.type == 2) {
+    lce_pack_kernel<2><<<pack_blocks(k.rows_out), 256, 0, stream>>>(k);
   } else {
-    launch(lce_pack_kernel<1>);
+    lce_pack_kernel<1><<<pack_blocks(k.rows_out), 256, 0, stream>>>(k);
   }
+  HIP_CHECK_KERNEL();
 }
 
-Operand rows_operand(const ushort* p, long rows, long ld, long lo,
-                     long cols) {
+Operand operand(const ushort* p, long rows, long ld, long cols) {
   Operand o;
   o.p = p;
-  o.lo = lo;
   o.ld = (int)ld;
   o.rows = (int)std::min<long>(rows, 0x7fffffffL);
   o.cols = (int)cols;
@@ -816,7 +942,7 @@ void check(const at::Tensor& x, const at::Tensor& w,
   }
 }
 
-// calls f(tile, seg, bf16) with compile-time arguments
+// calls f(parts, bf16) with compile-time arguments
 template <typename F>
 void with_types(const Plan& p, F f) {
   if (p.type == 0) {
@@ -824,7 +950,7 @@ void with_types(const Plan& p, F f) {
   } else if (p.type == 1) {
     f(std::integral_constant<int, 1>{}, std::false_type{});
   } else {
-    f(std::integral_constant<int, 3>{}, std::false_type{});
+    f(std::integral_constant<int, 2>{}, std::false_type{});
   }
 }
 
@@ -839,14 +965,14 @@ constexpr int x_layout() {
 }
 
 // two-part operands never meet that tile: its registers do not hold them
-template <class C, int SEG>
+template <class C, int PARTS>
 constexpr bool reached() {
-  return !(std::is_same<C, Logit>::value && SEG == 3);
+  return !(std::is_same<C, Logit>::value && PARTS == 2);
 }
 
 bool blocked(const Plan& p) {
   // not where 256-row tiles would be empty by more than they gain
-  return p.seg == 1 && p.n > 64 && up(p.n, 256) * 100 <= up(p.n, 128) * 115;
+  return p.parts == 1 && p.n > 64 && up(p.n, 256) * 100 <= up(p.n, 128) * 115;
 }
 
 template <typename F>
@@ -862,7 +988,8 @@ void with_row_tile(const Plan& p, F f) {
 
 }  // namespace
 
-// {loss (scalar or [N]), lse [N], count [1], top |w| of blocks (fp32)}
+// {loss (scalar or [N]), what the backward needs: lse [N], the count, and
+// (fp32) the largest |w| of blocks}
 std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
                                       const at::Tensor& w,
                                       const c10::optional<at::Tensor>& bias,
@@ -874,30 +1001,18 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
   auto stream = at::cuda::getCurrentCUDAStream();
   const Plan p = make_plan(x, w);
   auto f32 = x.options().dtype(at::kFloat);
-  auto u16 = x.options().dtype(at::kShort);
   const auto* lab = labels.data_ptr<int64_t>();
   const float eps = (float)smoothing;
-
   const bool blk = blocked(p);
-  auto xpk = at::empty({p.seg == 3 ? 2 * p.np : p.np, p.dp}, u16);
-  at::Tensor xinv, winv, none, tops, wpk;
-  if (p.seg == 3) xinv = at::empty({p.np}, f32);
-  pack(x, 0, p.n, p.np, p, blk ? none : xpk, blk ? xpk : none, lab, ignore, false, none, xinv, nullptr,
-       stream);
-
   const long piece = p.w_direct ? p.v : p.w_rows;
   const long pieces = (p.v + piece - 1) / piece;
   const int wblocks = pack_blocks(p.w_rows);
-  if (!p.w_direct) {
-    wpk = at::empty({p.seg == 3 ? 2 * p.w_rows : p.w_rows, p.dp}, u16);
-    if (p.seg == 3) {
-      winv = at::empty({p.w_rows}, f32);
-      tops = at::empty({pieces * wblocks}, f32);
-    }
-  }
-  auto loss = at::empty({p.n}, f32);
-  auto lse = at::empty({p.n}, f32);
-  auto total = at::empty({2}, f32);
+  const long ntop = p.parts == 2 ? pieces * wblocks : 0;
+  auto out = reduction == 0 ? at::empty({p.n}, f32) : at::empty({}, f32);
+  auto saved = at::empty({p.n + 1 + ntop}, f32);
+  float* lse = saved.data_ptr<float>();
+  float* tops = lse + p.n + 1;
+
   with_row_tile(p, [&](auto tile) {
     using C = decltype(tile);
     const int nmt = (int)((p.n + C::BM - 1) / C::BM);
@@ -905,82 +1020,104 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
     // a workgroup takes several tiles of words as long as ~2000 are left
     int tpb = (int)std::min<long>(8, piece_tiles * nmt / 2048);
     if (tpb < 1) tpb = 1;
-    std::vector<int> first;
-    int blocks = 0;
-    for (long i = 0; i < pieces; ++i) {
-      const long vp = std::min(piece, p.v - i * piece);
-      first.push_back(blocks);
-      blocks += (int)((vp + (long)C::BN * tpb - 1) / ((long)C::BN * tpb));
-    }
-    const int part_rows = (int)up(p.n, 16);
-    auto part = at::empty({eps != 0.f ? 3 : 2, blocks, part_rows}, f32);
+    const long span = (long)C::BN * tpb;
+    const int nvb = (int)((std::min(piece, p.v) + span - 1) / span);
+    const long rest = p.v - (pieces - 1) * piece;
+    const int blocks = (int)((pieces - 1) * nvb + (rest + span - 1) / span);
+
+    Scratch mem;
+    const auto o_x = mem.take<ushort>(p.np * p.dp * p.parts);
+    const auto o_xinv = mem.take<float>(p.parts == 2 ? p.np : 0);
+    const auto o_w =
+        mem.take<ushort>(p.w_direct ? 0 : p.w_rows * p.dp * p.parts);
+    const auto o_winv = mem.take<float>(p.parts == 2 ? p.w_rows : 0);
+    const auto o_part = mem.take<float>(p.n * blocks * (eps != 0.f ? 4 : 2));
+    const auto o_loss = mem.take<float>(reduction == 0 ? 0 : p.n);
+    const auto o_ticket = mem.take<unsigned>(1);
+    mem.allocate(x);
+
+    Pack kx = pack_of(x, 0, p.n, p.np, p,
+                      blk ? nullptr : mem.at<ushort>(o_x));
+    if (blk) kx.blocks = mem.at<ushort>(o_x);
+    kx.labels = lab;
+    kx.ignore = ignore;
+    kx.inv = mem.at<float>(o_xinv);
+    kx.zero = mem.at<unsigned>(o_ticket);
+    pack(kx, stream);
     for (long i = 0; i < pieces; ++i) {
       const long v0 = i * piece, vp = std::min(piece, p.v - v0);
       Logits q;
-      q.x = rows_operand(bits(xpk), p.np, p.dp, p.np * p.dp, p.dp);
+      q.x = operand(mem.at<ushort>(o_x), p.np, p.dp * p.parts, p.dp);
       if (p.w_direct) {
-        q.w = rows_operand(bits(w), vp, w.stride(0), 0, p.dp);
+        q.w = operand(bits(w), vp, w.stride(0), p.dp);
       } else {
-        pack(w, v0, vp, p.w_rows, p, wpk, none, nullptr, 0, false, none, winv,
-             p.seg == 3 ? tops.data_ptr<float>() + i * wblocks : nullptr,
-             stream);
-        q.w = rows_operand(bits(wpk), p.w_rows, p.dp, p.w_rows * p.dp, p.dp);
+        Pack kw = pack_of(w, v0, vp, up(vp, 64), p, mem.at<ushort>(o_w));
+        kw.inv = mem.at<float>(o_winv);
+        if (p.parts == 2) {
+          kw.bmax = tops + i * wblocks;
+          kw.rows_out = p.w_rows;  // every block has its largest value
+        }
+        pack(kw, stream);
+        q.w = operand(mem.at<ushort>(o_w), kw.rows_out, p.dp * p.parts,
+                      p.dp);
       }
-      q.xinv = p.seg == 3 ? xinv.data_ptr<float>() : nullptr;
-      q.winv = p.seg == 3 ? winv.data_ptr<float>() : nullptr;
+      q.xinv = mem.at<float>(o_xinv);
+      q.winv = mem.at<float>(o_winv);
       q.bias = bias_of(bias, v0);
       q.n = (int)p.n;
       q.vp = (int)vp;
       q.dp = (int)p.dp;
-      const int nvb =
-          (int)((vp + (long)C::BN * tpb - 1) / ((long)C::BN * tpb));
-      with_types(p, [&](auto seg, auto bf) {
-        if constexpr (reached<C, decltype(seg)::value>()) {
-        auto launch = [&](auto kernel) {
-          allow_lds(kernel, C::LDS_BYTES);
-          kernel<<<nmt * nvb, C::THREADS, C::LDS_BYTES, stream>>>(
-              q, part.template data_ptr<float>(), part_rows, first[i],
-              blocks, nmt, nvb, tpb);
-          HIP_CHECK_KERNEL();
-        };
-        if (eps != 0.f) {
-          launch(lce_fwd_kernel<C, x_layout<C>(), decltype(seg)::value,
-                                decltype(bf)::value, true>);
-        } else {
-          launch(lce_fwd_kernel<C, x_layout<C>(), decltype(seg)::value,
-                                decltype(bf)::value, false>);
-        }
+      const int here = (int)((vp + span - 1) / span);
+      with_types(p, [&](auto parts, auto bf) {
+        constexpr int PARTS = decltype(parts)::value;
+        constexpr bool BF = decltype(bf)::value;
+        if constexpr (reached<C, PARTS>()) {
+          auto launch = [&](auto kernel) {
+            constexpr int lds = C::template lds<1>();
+            allow_lds(kernel, lds);
+            kernel<<<nmt * here, C::THREADS, lds, stream>>>(
+                q, mem.at<float>(o_part), (int)i * nvb, blocks, nmt, here,
+                tpb);
+            HIP_CHECK_KERNEL();
+          };
+          if (eps != 0.f) {
+            launch(lce_fwd_kernel<C, x_layout<C>(), PARTS, BF, true>);
+          } else {
+            launch(lce_fwd_kernel<C, x_layout<C>(), PARTS, BF, false>);
+          }
         }
       });
     }
-    lce_join_kernel<<<(int)((p.n + 15) / 16), 256, 0, stream>>>(
-        part.template data_ptr<float>(), blocks, part_rows, x.data_ptr(),
-        p.type, x.stride(0), x.stride(1), w.data_ptr(), p.type, w.stride(0),
-        w.stride(1), bias.has_value() ? bias->data_ptr() : nullptr,
-        bias.has_value() ? type_code(*bias) : 0,
-        bias.has_value() ? bias->stride(0) : 0, (int)p.d, lab, ignore, p.v,
-        eps, loss.data_ptr<float>(), lse.data_ptr<float>(), (int)p.n);
+    Join j = {};
+    j.part = mem.at<float>(o_part);
+    j.nblocks = blocks;
+    j.x = vec_of(x);
+    j.w = vec_of(w);
+    if (bias.has_value()) j.bias = vec_of(*bias);
+    j.d = (int)p.d;
+    j.n = (int)p.n;
+    j.labels = lab;
+    j.ignore = ignore;
+    j.V = p.v;
+    j.eps = eps;
+    j.loss = reduction == 0 ? out.data_ptr<float>() : mem.at<float>(o_loss);
+    j.lse = lse;
+    j.reduction = (int)reduction;
+    j.ticket = mem.at<unsigned>(o_ticket);
+    j.out = out.data_ptr<float>();
+    j.count = lse + p.n;
+    lce_join_kernel<<<(int)((p.n + 3) / 4), 256, 0, stream>>>(j);
     HIP_CHECK_KERNEL();
   });
-  at::Tensor out = loss;
-  if (reduction != 0) {
-    lce_total_kernel<<<1, 1024, 0, stream>>>(
-        loss.data_ptr<float>(), lab, ignore, (int)p.n, reduction == 1,
-        total.data_ptr<float>());
-    HIP_CHECK_KERNEL();
-    out = total[0];
-  }
-  if (!tops.defined()) tops = at::empty({0}, f32);
-  return {out, lse, total, tops};
+  return {out, saved};
 }
 
 // {dx, dw, db}; an empty tensor for what is not wanted
 std::vector<at::Tensor> linear_ce_bwd(
     const at::Tensor& dloss, const at::Tensor& x, const at::Tensor& w,
     const c10::optional<at::Tensor>& bias, const at::Tensor& labels,
-    const at::Tensor& lse, const at::Tensor& count, const at::Tensor& tops,
-    int64_t ignore, double smoothing, int64_t reduction, bool want_dx,
-    bool want_dw, bool want_db) {
+    const at::Tensor& saved, int64_t ignore, double smoothing,
+    int64_t reduction, bool want_dx, bool want_dw, bool want_db) {
   check(x, w, bias, labels);
   TORCH_CHECK(dloss.scalar_type() == at::kFloat && dloss.is_cuda() &&
                   dloss.is_contiguous() &&
@@ -989,175 +1126,198 @@ std::vector<at::Tensor> linear_ce_bwd(
   const c10::cuda::CUDAGuard guard(x.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   const Plan p = make_plan(x, w);
-  auto f32 = x.options().dtype(at::kFloat);
-  auto u16 = x.options().dtype(at::kShort);
   const auto* lab = labels.data_ptr<int64_t>();
   const float eps = (float)smoothing;
-  const bool s3 = p.seg == 3;
-
-  const long nrows = up(p.n, 256);
-  auto rows = at::empty({nrows, 4}, f32);
-  auto sc = at::empty({2}, f32);
-  lce_rows_kernel<<<1, 1024, 0, stream>>>(
-      dloss.data_ptr<float>(), reduction != 0,
-      reduction == 1 ? count.data_ptr<float>() + 1 : nullptr, lab, ignore,
-      (int)p.n, (int)nrows, p.type != 0, lse.data_ptr<float>(), p.v,
-      reinterpret_cast<Row*>(rows.data_ptr()), sc.data_ptr<float>());
-  HIP_CHECK_KERNEL();
-
-  at::Tensor xpk = at::empty({s3 ? 2 * p.np : p.np, p.dp}, u16);
-  at::Tensor xinv, winv, none, xtop, wpk, xblk;
-  if (blocked(p)) xblk = at::empty_like(xpk);
-  if (s3) {
-    // one scale for all rows, as the rows are summed over: the first call
-    // only finds the largest value
-    xinv = at::empty({p.np}, f32);
-    xtop = at::empty({pack_blocks(p.np)}, f32);
-    pack(x, 0, p.n, p.np, p, xpk, none, lab, ignore, false, none, xinv,
-         xtop.data_ptr<float>(), stream);
-  }
-  pack(x, 0, p.n, p.np, p, xpk, xblk, lab, ignore, s3, xtop, xinv, nullptr,
-       stream);
+  const bool two = p.parts == 2, blk = blocked(p);
+  const float* lse = saved.data_ptr<float>();
+  const float* tops = lse + p.n + 1;
+  const int ntop = (int)(saved.numel() - p.n - 1);
 
   // words for which the tiles of dw fill the chip's 256 CUs once
   const long wave_of_words = 256 * 256 / ((p.dp + 255) / 256);
-  long piece = kPieceBytes / (nrows * (s3 ? 4 : 2));
+  long piece = kPieceBytes / (p.np * 2 * p.parts);
   piece = piece >= wave_of_words ? piece / wave_of_words * wave_of_words
                                  : piece / 256 * 256;
   piece = std::max(256L, std::min(piece, up(p.v, 256)));
   if (!p.w_direct) piece = std::min(piece, p.w_rows);
   // offsets inside a piece of w stay below 2^31
-  const long w_ld = p.w_direct ? w.stride(0) : p.dp;
+  const long w_ld = p.w_direct ? w.stride(0) : p.dp * p.parts;
   piece = std::max(256L, std::min(piece, (1L << 30) / w_ld / 256 * 256));
   const int ldg = (int)piece;
-  const long glo = nrows * ldg;
-  auto G = at::empty({s3 ? 2 * nrows : nrows, ldg}, u16);
-  if (!p.w_direct) {
-    wpk = at::empty({s3 ? 2 * piece : piece, p.dp}, u16);
-    if (s3) winv = at::empty({piece}, f32);
-  }
-  at::Tensor dx, dw, db, part, dbp;
-  if (want_dx) dx = at::empty({p.n, p.d}, x.options());
-  if (want_dw) dw = at::empty({p.v, p.d}, w.options());
-  if (want_db) {
-    db = at::empty({p.v}, bias->options());
-    dbp = at::empty({(p.n + 63) / 64, ldg}, f32);
-  }
   // dx: few tiles and a long k, so k is cut until the chip is full
-  const int dx_tile = p.n > 128 && p.dp >= 128 ? (getenv("DXBIG") && p.dp>=256 ? 256:128) : 64;
+  const int dx_tile = p.n > 128 && p.dp >= 128 ? 128 : 64;
   const long dx_tiles = ((p.n + dx_tile - 1) / dx_tile) *
                         ((p.dp + dx_tile - 1) / dx_tile);
-  const int slices = (int)std::min<long>(
-      std::max(1L, (dx_tile == 256 ? 256 : 512) / dx_tiles),
-      std::max(1L, piece / 512));
-  if (want_dx) part = at::empty({slices, p.n, p.dp}, f32);
+  const int slices = (int)std::min<long>(std::max(1L, 512 / dx_tiles),
+                                         std::max(1L, piece / 512));
+  at::Tensor dx, dw, db;
+  if (want_dx) dx = at::empty({p.n, p.d}, x.options());
+  if (want_dw) dw = at::empty({p.v, p.d}, w.options());
+  if (want_db) db = at::empty({p.v}, bias->options());
 
-  for (long v0 = 0; v0 < p.v; v0 += piece) {
-    const long vp = std::min(piece, p.v - v0);
-    Logits q;
-    q.x = rows_operand(bits(xblk.defined() ? xblk : xpk), p.np, p.dp,
-                       p.np * p.dp, p.dp);
-    if (p.w_direct) {
-      q.w = rows_operand(bits(w) + v0 * w.stride(0), vp, w.stride(0), 0,
-                         p.dp);
-    } else {
-      pack(w, v0, vp, up(vp, 64), p, wpk, none, nullptr, 0, s3, tops, winv,
-           nullptr, stream);
-      q.w = rows_operand(bits(wpk), up(vp, 64), p.dp, up(vp, 64) * p.dp,
-                         p.dp);
+  with_row_tile(p, [&](auto row_tile) {
+    using R = decltype(row_tile);
+    const int nmt = (int)((p.n + R::BM - 1) / R::BM);
+    // column sums of all pieces are joined at the end where they are small
+    const bool db_late = up(p.v, 256) * nmt <= (16L << 20);
+    const long db_ld = db_late ? up(p.v, 256) : ldg;
+
+    Scratch mem;
+    const auto o_rows = mem.take<Row>(p.np);
+    const auto o_sc = mem.take<float>(2);
+    const auto o_x = mem.take<ushort>(p.np * p.dp * p.parts);
+    const auto o_xblk = mem.take<ushort>(blk ? p.np * p.dp : 0);
+    const auto o_xinv = mem.take<float>(two ? p.np : 0);
+    const auto o_xtop = mem.take<float>(two ? pack_blocks(p.np) : 0);
+    const auto o_w = mem.take<ushort>(p.w_direct ? 0
+                                                 : piece * p.dp * p.parts);
+    const auto o_winv = mem.take<float>(two ? piece : 0);
+    const auto o_G = mem.take<ushort>(p.np * ldg * p.parts);
+    const auto o_part =
+        mem.take<float>(want_dx ? slices * p.n * p.dp : 0);
+    const auto o_dbp = mem.take<float>(want_db && nmt > 1 ? nmt * db_ld : 0);
+    mem.allocate(x);
+
+    Pack kx = pack_of(x, 0, p.n, p.np, p, mem.at<ushort>(o_x));
+    kx.labels = lab;
+    kx.ignore = ignore;
+    kx.inv = mem.at<float>(o_xinv);
+    if (two) {
+      // one scale for all rows, as the rows are summed over: the first call
+      // only finds the largest value
+      kx.bmax = mem.at<float>(o_xtop);
+      pack(kx, stream);
+      kx.bmax = nullptr;
+      kx.top = mem.at<float>(o_xtop);
+      kx.ntop = pack_blocks(p.np);
     }
-    q.xinv = s3 ? xinv.data_ptr<float>() : nullptr;
-    q.winv = s3 ? winv.data_ptr<float>() : nullptr;
-    q.bias = bias_of(bias, v0);
-    q.n = (int)p.n;
-    q.vp = (int)vp;
-    q.dp = (int)p.dp;
-    auto* Gp = reinterpret_cast<ushort*>(G.data_ptr());
-    with_types(p, [&](auto seg, auto bf) {
-      constexpr int SEG = decltype(seg)::value;
-      constexpr bool BF = decltype(bf)::value;
-      with_row_tile(p, [&](auto tile) {
-        using C = decltype(tile);
-        if constexpr (reached<C, SEG>()) {
-        const int nmt = (int)((p.n + C::BM - 1) / C::BM);
-        const int nvt = (int)((vp + C::BN - 1) / C::BN);
-        auto launch = [&](auto kernel) {
-          allow_lds(kernel, C::LDS_BYTES);
-          kernel<<<nmt * nvt, C::THREADS, C::LDS_BYTES, stream>>>(
-              q, reinterpret_cast<const Row*>(rows.data_ptr()),
-              sc.template data_ptr<float>(), p.v, v0, eps, Gp, ldg, glo,
-              want_db ? dbp.template data_ptr<float>() : nullptr, nmt, nvt);
-          HIP_CHECK_KERNEL();
-        };
-        if (want_db) {
-          launch(lce_grad_kernel<C, x_layout<C>(), SEG, BF, true>);
-          lce_db_kernel<<<(int)((vp + 255) / 256), 256, 0, stream>>>(
-              dbp.template data_ptr<float>(), nmt, ldg, (int)vp,
-              static_cast<char*>(db.data_ptr()) + v0 * db.element_size(),
-              type_code(db));
-          HIP_CHECK_KERNEL();
-        } else {
-          launch(lce_grad_kernel<C, x_layout<C>(), SEG, BF, false>);
+    if (blk) kx.blocks = mem.at<ushort>(o_xblk);
+    kx.row = mem.at<Row>(o_rows);
+    kx.dloss = dloss.data_ptr<float>();
+    kx.each = reduction == 0;
+    kx.count = reduction == 1 ? lse + p.n : nullptr;
+    kx.lse = lse;
+    kx.V = p.v;
+    kx.sc = mem.at<float>(o_sc);
+    pack(kx, stream);
+    if (kx.each) {
+      lce_scale_kernel<<<1, 1024, 0, stream>>>(
+          kx.dloss, lab, ignore, (int)p.n, p.type != 0, kx.sc);
+      HIP_CHECK_KERNEL();
+    }
+    auto* G = mem.at<ushort>(o_G);
+    const float* sc = kx.sc;
+    const float* xinv = two ? kx.inv : nullptr;
+    const float* winv = two ? mem.at<float>(o_winv) : nullptr;
+    const Operand xr = operand(mem.at<ushort>(o_x), p.np, p.dp * p.parts,
+                               p.dp);
+
+    for (long v0 = 0; v0 < p.v; v0 += piece) {
+      const long vp = std::min(piece, p.v - v0);
+      Logits q;
+      q.x = blk ? operand(mem.at<ushort>(o_xblk), p.np, p.dp, p.dp) : xr;
+      if (p.w_direct) {
+        q.w = operand(bits(w) + v0 * w.stride(0), vp, w.stride(0), p.dp);
+      } else {
+        Pack kw = pack_of(w, v0, vp, up(vp, 64), p, mem.at<ushort>(o_w));
+        kw.inv = mem.at<float>(o_winv);
+        kw.top = two ? tops : nullptr;
+        kw.ntop = ntop;
+        pack(kw, stream);
+        q.w = operand(mem.at<ushort>(o_w), kw.rows_out, p.dp * p.parts,
+                      p.dp);
+      }
+      q.xinv = xinv;
+      q.winv = winv;
+      q.bias = bias_of(bias, v0);
+      q.n = (int)p.n;
+      q.vp = (int)vp;
+      q.dp = (int)p.dp;
+      with_types(p, [&](auto parts, auto bf) {
+        constexpr int PARTS = decltype(parts)::value;
+        constexpr bool BF = decltype(bf)::value;
+        if constexpr (reached<R, PARTS>()) {
+          const int nvt = (int)((vp + R::BN - 1) / R::BN);
+          float* dbp = mem.at<float>(o_dbp) + (db_late ? v0 : 0);
+          void* db_at = want_db ? static_cast<char*>(db.data_ptr()) +
+                                      v0 * db.element_size()
+                                : nullptr;
+          auto launch = [&](auto kernel) {
+            constexpr int lds = R::template lds<PARTS>();
+            allow_lds(kernel, lds);
+            kernel<<<nmt * nvt, R::THREADS, lds, stream>>>(
+                q, mem.at<Row>(o_rows), sc, p.v, v0, eps, G, ldg, dbp, db_ld,
+                db_at, want_db ? type_code(db) : 0, nmt, nvt);
+            HIP_CHECK_KERNEL();
+          };
+          if (want_db) {
+            launch(lce_grad_kernel<R, x_layout<R>(), PARTS, BF, true>);
+          } else {
+            launch(lce_grad_kernel<R, x_layout<R>(), PARTS, BF, false>);
+          }
+          const bool done = v0 + piece >= p.v;
+          if (want_db && nmt > 1 && (!db_late || done)) {
+            const long words = db_late ? p.v : vp;
+            lce_db_kernel<<<(int)((words + 255) / 256), 256, 0, stream>>>(
+                mem.at<float>(o_dbp), nmt, db_ld, words,
+                db_late ? db.data_ptr() : db_at, type_code(db));
+            HIP_CHECK_KERNEL();
+          }
         }
+        const Operand g_rows = operand(G, p.np, (long)ldg * PARTS, ldg);
+        if (want_dw) {
+          auto run = [&](auto tile) {
+            using C = decltype(tile);
+            const int mt = (int)((vp + C::BM - 1) / C::BM);
+            const int nt = (int)((p.d + C::BN - 1) / C::BN);
+            auto kernel = lce_dw_kernel<C, PARTS, BF>;
+            constexpr int lds = C::template lds<1>();
+            allow_lds(kernel, lds);
+            kernel<<<mt * nt, C::THREADS, lds, stream>>>(
+                g_rows, xr, (int)up(p.n, 64), sc, xinv,
+                static_cast<char*>(dw.data_ptr()) +
+                    v0 * p.d * dw.element_size(),
+                p.type, (int)vp, (int)p.d, mt, nt);
+            HIP_CHECK_KERNEL();
+          };
+          const long cover = ((vp + 255) / 256) * ((p.dp + 255) / 256);
+          if (cover >= 192 && p.dp % 256 == 0) {
+            run(Big{});
+          } else if (cover >= 48 && p.dp >= 128) {
+            run(Mid{});
+          } else {
+            run(Small{});
+          }
+        }
+        if (want_dx) {
+          auto run = [&](auto tile) {
+            using C = decltype(tile);
+            const int mt = (int)((p.n + C::BM - 1) / C::BM);
+            const int nt = (int)((p.dp + C::BN - 1) / C::BN);
+            const int kv = (int)up(vp, 64);
+            const int kslice = (int)up((kv + slices - 1) / slices, 64);
+            auto kernel = lce_dx_kernel<C, PARTS, BF>;
+            constexpr int lds = C::template lds<1>();
+            allow_lds(kernel, lds);
+            kernel<<<mt * nt * slices, C::THREADS, lds, stream>>>(
+                g_rows, q.w, kv, kslice, mem.at<float>(o_part), (int)p.n,
+                (int)p.dp, v0 == 0, mt, nt, slices);
+            HIP_CHECK_KERNEL();
+          };
+          if (dx_tile == 128) {
+            run(Mid{});
+          } else {
+            run(Small{});
+          }
         }
       });
-      if (want_dw) {
-        auto run = [&](auto tile) {
-          using C = decltype(tile);
-          const int nmt = (int)((vp + C::BM - 1) / C::BM);
-          const int nnt = (int)((p.d + C::BN - 1) / C::BN);
-          auto kernel = lce_dw_kernel<C, SEG, BF>;
-          allow_lds(kernel, C::LDS_BYTES);
-          kernel<<<nmt * nnt, C::THREADS, C::LDS_BYTES, stream>>>(
-              rows_operand(Gp, nrows, ldg, glo, ldg),
-              rows_operand(bits(xpk), p.np, p.dp, p.np * p.dp, p.dp),
-              (int)up(p.n, 64), sc.template data_ptr<float>(),
-              s3 ? xinv.data_ptr<float>() : nullptr,
-              static_cast<char*>(dw.data_ptr()) +
-                  v0 * p.d * dw.element_size(),
-              p.type, (int)vp, (int)p.d, nmt, nnt);
-          HIP_CHECK_KERNEL();
-        };
-        const long cover = ((vp + 255) / 256) * ((p.dp + 255) / 256);
-        if (cover >= 192 && p.dp % 256 == 0) {
-          run(Big{});
-        } else if (cover >= 48 && p.dp >= 128) {
-          run(Mid{});
-        } else {
-          run(Small{});
-        }
-      }
-      if (want_dx) {
-        auto run = [&](auto tile) {
-          using C = decltype(tile);
-          const int nmt = (int)((p.n + C::BM - 1) / C::BM);
-          const int nnt = (int)((p.dp + C::BN - 1) / C::BN);
-          const int kv = (int)up(vp, 64);
-          const int kslice = (int)up((kv + slices - 1) / slices, 64);
-          auto kernel = lce_dx_kernel<C, SEG, BF>;
-          allow_lds(kernel, C::LDS_BYTES);
-          kernel<<<nmt * nnt * slices, C::THREADS, C::LDS_BYTES, stream>>>(
-              rows_operand(Gp, nrows, ldg, glo, ldg), q.w, kv, kslice,
-              part.data_ptr<float>(), (int)p.n, (int)p.dp, v0 == 0, nmt, nnt,
-              slices);
-          HIP_CHECK_KERNEL();
-        };
-        if (dx_tile == 256) {
-          run(Big{});
-        } else if (dx_tile == 128) {
-          run(Mid{});
-        } else {
-          run(Small{});
-        }
-      }
-    });
-  }
-  if (want_dx) {
-    lce_dx_sum_kernel<<<px_grid(p.n * p.d), 256, 0, stream>>>(
-        part.data_ptr<float>(), slices, p.n, (int)p.d, (int)p.dp,
-        sc.data_ptr<float>(), s3 ? winv.data_ptr<float>() : nullptr,
-        dx.data_ptr(), p.type);
-    HIP_CHECK_KERNEL();
-  }
+    }
+    if (want_dx) {
+      lce_dx_sum_kernel<<<px_grid(p.n * p.d), 256, 0, stream>>>(
+          mem.at<float>(o_part), slices, p.n, (int)p.d, (int)p.dp, sc, winv,
+          dx.data_ptr(), p.type);
+      HIP_CHECK_KERNEL();
+    }
+  });
   return {dx, dw, db};
 }

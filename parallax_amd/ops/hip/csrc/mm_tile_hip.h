@@ -13,9 +13,11 @@
 //     bytes of a k-contiguous row, half of what memory hands out at a time;
 //     blocks make that one piece (256 x 128 tile, 2560 x 32768 x 512: 86 us
 //     with rows, 74 us with the first operand in blocks).
-//   * SEG = 3 multiplies operands that are split into a high and a low fp16
-//     part (value = hi + lo, 22 bits): the k loop runs over lo*hi, hi*lo and
-//     hi*hi.  The dropped lo*lo is 2^-22 of a product.
+//   * PARTS = 2 multiplies operands that are split into a high and a low
+//     fp16 part (value = hi + lo, 22 bits): lo*hi, hi*lo and hi*hi are added
+//     up, the dropped lo*lo is 2^-22 of a product.  Such an operand lies in
+//     pairs: each 32 values of a row are 32 high parts and 32 low parts, so
+//     a stage is 32 k of both, and three products come of four reads.
 //   * Operands go from memory to LDS directly (buffer loads, 16 B a lane)
 //     into ST buffers; a wait leaves ST-2 stages in flight, and one barrier
 //     a stage both publishes stage k and frees the buffer of stage k-1.
@@ -53,17 +55,15 @@ __device__ __forceinline__ f4 mma(s8 a, s8 b, f4 c) {
 }
 
 // One operand of a product.
-//   p        first element (of the high part)
-//   lo       distance in elements to the low part (SEG = 3)
-//   ld       elements between rows as they lie
+//   p        first element
+//   ld       elements between rows as they lie (pairs: both parts counted)
 //   rows     rows that may be read (KROWS: of the operand, KCOLS: its k);
 //            KBLOCK: of a block, a multiple of the tile's
 //   cols     KCOLS: operand rows (columns as they lie) that may be read, a
-//            multiple of 8
+//            multiple of 8, of 32 in pairs
 // Reads past `rows` and `cols` are clamped to the last ones.
 struct Operand {
   const ushort* p;
-  long lo;
   int ld;
   int rows;
   int cols;
@@ -80,10 +80,17 @@ struct Tile {
   // workgroups of four or eight waves on a CU, or one of sixteen
   static constexpr int OCC = THREADS == 1024 ? 4 : THREADS / 128;
   static constexpr int STAGE_BYTES = (BM + BN) * BK * 2;
-  // a 16-bit tile on its way out: rows 16 bytes apart from a bank's
-  static constexpr int OUT_ROW = BN * 2 + 16;
-  static constexpr int LDS_BYTES = ST * STAGE_BYTES > BM * OUT_ROW
-                                       ? ST * STAGE_BYTES : BM * OUT_ROW;
+  // a tile on its way out, of 16-bit values or of pairs of parts: rows 16
+  // bytes apart from a bank's, in two goes where 160 KB do not hold it
+  static constexpr int OUT_ROW = BN * 2 + 16, PAIR_ROW = BN * 4 + 16;
+  static constexpr int PAIR_GOES = BM * PAIR_ROW > 160 * 1024 ? 2 : 1;
+  static constexpr int lds_bytes(int out) {
+    return ST * STAGE_BYTES > out ? ST * STAGE_BYTES : out;
+  }
+  template <int PARTS>
+  static constexpr int lds() {
+    return lds_bytes(PARTS == 2 ? BM * PAIR_ROW / PAIR_GOES : BM * OUT_ROW);
+  }
 };
 
 template <int BK>
@@ -101,12 +108,13 @@ __device__ __forceinline__ int col_swizzle(int k) {
 }
 
 // Copies one operand's [R x BK] piece of a stage into LDS.
-template <int R, int L, int BK, int THREADS>
+template <int R, int L, int BK, int THREADS, int PARTS>
 struct Stager {
   static constexpr int PER = R * BK * 2 / 16 / THREADS;
   static_assert(PER >= 1 && PER * THREADS * 16 == R * BK * 2,
                 "a stage has to be whole 16-byte pieces for every thread");
-  __amdgpu_buffer_rsrc_t rs, rs_lo;
+  static_assert(PARTS == 1 || BK == 64, "pairs of 32");
+  __amdgpu_buffer_rsrc_t rs;
   int off[PER];    // KROWS: byte offset; KCOLS: column byte offset
   int ld2;
   int rows;
@@ -114,19 +122,18 @@ struct Stager {
   __device__ __forceinline__ void init(const Operand& o, int r0) {
     ld2 = o.ld * 2;
     rows = o.rows;
-    const ushort* base =
-        o.p + (L == KROWS ? (long)r0 * o.ld : L == KCOLS ? (long)r0 : 0L);
+    const ushort* base = o.p + (L == KROWS ? (long)r0 * o.ld
+                                : L == KCOLS ? (long)r0 * PARTS : 0L);
     const long left = (L == KROWS ? (long)(o.rows - r0) : (long)o.rows) * ld2;
     const int bytes = (int)(left < 0x7fffffffL ? left : 0x7fffffffL);
     rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<ushort*>(base), 0,
                                            bytes, 0x00027000);
-    rs_lo = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<ushort*>(base + o.lo), 0, bytes, 0x00027000);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + i * THREADS;
       if constexpr (L == KBLOCK) {
-        static_assert(BK == 32, "blocks of 32 k");
+        static_assert(L != KBLOCK || (BK == 32 && PARTS == 1),
+                      "blocks of 32 k");
         const int r = c / 4;
         off[i] = (r0 + r) * 64 + (((c % 4) ^ row_swizzle<BK>(r)) * 16);
       } else if constexpr (L == KROWS) {
@@ -141,30 +148,32 @@ struct Stager {
         const int src = (c % S) ^ (col_swizzle<R>(k) << 1);
         int col = src * 8;
         if (col > o.cols - 8 - r0) col = o.cols - 8 - r0;
-        off[i] = col * 2;
+        off[i] = PARTS == 2
+                     ? ((col >> 5) * 64 + (col & 31) + (k & 32)) * 2
+                     : col * 2;
       }
     }
   }
 
-  // the stage that starts at k0, of the high or the low part
-  __device__ __forceinline__ void load(char* lds, int k0, bool lo) const {
+  // the stage that starts at k0
+  __device__ __forceinline__ void load(char* lds, int k0) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       int v;
       if constexpr (L == KBLOCK) {
         v = off[i] + k0 * 2 * rows;
       } else if constexpr (L == KROWS) {
-        v = off[i] + k0 * 2;
+        v = off[i] + k0 * 2 * PARTS;
       } else {
-        int k = (threadIdx.x + i * THREADS) / (R / 8) + k0;
+        int k = (threadIdx.x + i * THREADS) / (R / 8);
+        k = (PARTS == 2 ? k & 31 : k) + k0;
         if (k > rows - 1) k = rows - 1;
         v = off[i] + k * ld2;
       }
       // each wave writes 1 KiB in lane order from its own base
       char* dst = lds + i * THREADS * 16 + (threadIdx.x & ~63) * 16;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          lo ? rs_lo : rs,
-          (__attribute__((address_space(3))) void*)dst, 16, v, 0, 0, 0);
+          rs, (__attribute__((address_space(3))) void*)dst, 16, v, 0, 0, 0);
     }
   }
 };
@@ -209,41 +218,42 @@ __device__ __forceinline__ void barrier() {
 
 // acc[i][j] of wave (wm, wn): element (m, n) with
 //   m = m0 + wm + i*16 + (lane & 15), n = n0 + wn + j*16 + (lane>>4)*4 + r.
-// k runs over [k0, k1), both multiples of BK, of each segment.
-template <class C, int AL, int BL, int SEG, bool BF>
+// k runs over [k0, k1), both multiples of BK, of 32 in pairs.
+template <class C, int AL, int BL, int PARTS, bool BF>
 __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
                                         const Operand& b, int n0, int k0,
                                         int k1, f4 (&acc)[C::FM][C::FN]) {
   constexpr int BK = C::BK, ST = C::ST, T = C::THREADS;
-  Stager<C::BM, AL, BK, T> sa;
-  Stager<C::BN, BL, BK, T> sb;
+  constexpr int STEP = PARTS == 2 ? 32 : BK;
+  Stager<C::BM, AL, BK, T, PARTS> sa;
+  Stager<C::BN, BL, BK, T, PARTS> sb;
   sa.init(a, m0);
   sb.init(b, n0);
-  constexpr int LOADS = Stager<C::BM, AL, BK, T>::PER +
-                        Stager<C::BN, BL, BK, T>::PER;
+  constexpr int LOADS = sa.PER + sb.PER;
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
-  const int per = (k1 - k0) / BK;
-  const int total = per * SEG;
+  const int total = (k1 - k0) / STEP;
 
-  int ls = 0, lk = k0, lbuf = 0;  // what is staged next
-  auto stage = [&]() {
+  int lbuf = 0;  // where the next stage goes
+  auto stage = [&](int t) {
     char* at = lds + lbuf * C::STAGE_BYTES;
-    sa.load(at, lk, SEG == 3 && ls == 0);
-    sb.load(at + C::BM * BK * 2, lk, SEG == 3 && ls == 1);
-    lk += BK;
-    if (SEG > 1 && lk == k1) {
-      lk = k0;
-      ++ls;
-    }
+    sa.load(at, k0 + t * STEP);
+    sb.load(at + C::BM * BK * 2, k0 + t * STEP);
     lbuf = lbuf + 1 == ST ? 0 : lbuf + 1;
+  };
+  auto multiply = [&](const s8 (&fa)[C::FM], const s8 (&fb)[C::FN]) {
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j)
+        acc[i][j] = mma<BF>(fb[j], fa[i], acc[i][j]);
   };
 
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) {
-    if (s < total) stage();
+    if (s < total) stage(s);
   }
   int buf = 0;
   for (int t = 0; t < total; ++t) {
@@ -253,27 +263,52 @@ __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
       wait_loads<0>();
     }
     barrier();
-    if (t + ST - 1 < total) stage();
+    if (t + ST - 1 < total) stage(t + ST - 1);
     const char* pa = lds + buf * C::STAGE_BYTES;
     const char* pb = pa + C::BM * BK * 2;
     buf = buf + 1 == ST ? 0 : buf + 1;
+    auto read_a = [&](s8 (&f)[C::FM], int kk) {
 #pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      s8 fa[C::FM], fb[C::FN];
+      for (int i = 0; i < C::FM; ++i)
+        f[i] = frag<C::BM, AL, BK>(pa, wm + i * 16, kk, lane);
+    };
+    auto read_b = [&](s8 (&f)[C::FN], int kk) {
 #pragma unroll
       for (int j = 0; j < C::FN; ++j)
-        fb[j] = frag<C::BN, BL, BK>(pb, wn + j * 16, kk, lane);
+        f[j] = frag<C::BN, BL, BK>(pb, wn + j * 16, kk, lane);
+    };
+    if constexpr (PARTS == 2) {
+      s8 ah[C::FM], al[C::FM], bh[C::FN], bl[C::FN];
+      read_b(bh, 0);
+      read_a(al, 1);
+      multiply(al, bh);
+      read_a(ah, 0);
+      multiply(ah, bh);
+      read_b(bl, 1);
+      multiply(ah, bl);
+    } else {
 #pragma unroll
-      for (int i = 0; i < C::FM; ++i)
-        fa[i] = frag<C::BM, AL, BK>(pa, wm + i * 16, kk, lane);
-#pragma unroll
-      for (int i = 0; i < C::FM; ++i)
-#pragma unroll
-        for (int j = 0; j < C::FN; ++j)
-          acc[i][j] = mma<BF>(fb[j], fa[i], acc[i][j]);
+      for (int kk = 0; kk < BK / 32; ++kk) {
+        s8 fa[C::FM], fb[C::FN];
+        read_b(fb, kk);
+        read_a(fa, kk);
+        multiply(fa, fb);
+      }
     }
   }
   barrier();  // the caller may use the LDS
+}
+
+// hi/lo fp16 parts of a value
+__device__ __forceinline__ void split(float v, ushort& hi, ushort& lo) {
+  const _Float16 h = (_Float16)v;
+  const _Float16 l = (_Float16)(v - (float)h);
+  hi = __builtin_bit_cast(ushort, h);
+  lo = __builtin_bit_cast(ushort, l);
+}
+
+__device__ __forceinline__ float half_bits(ushort h) {
+  return (float)__builtin_bit_cast(_Float16, h);
 }
 
 // Writes a tile of 16-bit values, through LDS so that a row goes out in one
@@ -311,6 +346,47 @@ __device__ __forceinline__ void store_tile(char* lds, ushort* out, long ld,
   }
 }
 
+// The same for values in pairs of parts: value(i, j) in fp32, scaled; `out`
+// is at a multiple of 32 values, `ld` counts both parts, all is written.
+template <class C, typename F>
+__device__ __forceinline__ void store_pairs(char* lds, ushort* out, long ld,
+                                            F value) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int wm = (wave / C::WAVES_N) * C::WM;
+  const int wn = (wave % C::WAVES_N) * C::WN;
+  constexpr int HALF = C::BM / C::PAIR_GOES, PER_ROW = C::BN / 4;
+#pragma unroll
+  for (int go = 0; go < C::PAIR_GOES; ++go) {
+    if (go) __syncthreads();
+    if (wm / HALF == go) {
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j) {
+          const f4 v = value(i, j);
+          ushort h[4], l[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) split(v[r], h[r], l[r]);
+          const int n = wn + j * 16 + (lane >> 4) * 4;
+          char* at = lds + (wm % HALF + i * 16 + (lane & 15)) * C::PAIR_ROW +
+                     ((n >> 5) * 64 + (n & 31)) * 2;
+          *reinterpret_cast<ushort4*>(at) =
+              make_ushort4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<ushort4*>(at + 64) =
+              make_ushort4(l[0], l[1], l[2], l[3]);
+        }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int c = threadIdx.x; c < HALF * PER_ROW; c += C::THREADS) {
+      const int r = c / PER_ROW, q = (c % PER_ROW) * 8;
+      *reinterpret_cast<s8*>(out + (go * HALF + r) * ld + q) =
+          *reinterpret_cast<const s8*>(lds + r * C::PAIR_ROW + q * 2);
+    }
+  }
+}
+
 // Spreads a flat block id over the 8 dies so that each die works on one
 // contiguous range of tiles: neighbours then share operands in its L2.
 __device__ __forceinline__ int die_contiguous(int bid, int n) {
@@ -331,18 +407,6 @@ __device__ __forceinline__ float sum16(float v) {
   add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF,
                                   0xF, true));   // mirrored in 16
   return v;
-}
-
-// hi/lo fp16 parts of a value
-__device__ __forceinline__ void split(float v, ushort& hi, ushort& lo) {
-  const _Float16 h = (_Float16)v;
-  const _Float16 l = (_Float16)(v - (float)h);
-  hi = __builtin_bit_cast(ushort, h);
-  lo = __builtin_bit_cast(ushort, l);
-}
-
-__device__ __forceinline__ float half_bits(ushort h) {
-  return (float)__builtin_bit_cast(_Float16, h);
 }
 
 }  // namespace mm

@@ -29,6 +29,9 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <mutex>
+#include <set>
+
 #include "mm_tile.h"
 
 namespace {
@@ -77,21 +80,69 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(
   if (threadIdx.x == 0) part[(long)blockIdx.y * blocks + blockIdx.x] = red[0];
 }
 
+// How X, A and B lie between the products: in pairs of parts for products of
+// two-part operands; else a plane of high parts and, for X, one of low parts
+// behind it.  All are padded with zeros to whole tiles.
+struct Matrix {
+  ushort* p;
+  long stride;   // between the matrices of a batch
+  int rows, cols;
+  bool pairs;
+
+  __device__ __forceinline__ Matrix of(int batch) const {
+    Matrix m = *this;
+    m.p += batch * stride;
+    return m;
+  }
+  __host__ __device__ __forceinline__ Operand operand() const {
+    Operand o;
+    o.p = p;
+    o.ld = pairs ? 2 * cols : cols;
+    o.rows = rows;
+    o.cols = cols;
+    return o;
+  }
+  __device__ __forceinline__ long at(int r, int c) const {
+    return pairs ? (long)r * cols * 2 + (c >> 5) * 64 + (c & 31)
+                 : (long)r * cols + c;
+  }
+  // four values of a row; LO: with the low parts
+  template <bool LO>
+  __device__ __forceinline__ f4 four(int r, int c) const {
+    const long i = at(r, c);
+    const ushort4 h = *reinterpret_cast<const ushort4*>(p + i);
+    f4 v = {half_bits(h.x), half_bits(h.y), half_bits(h.z), half_bits(h.w)};
+    if (LO) {
+      const ushort4 l = *reinterpret_cast<const ushort4*>(
+          p + i + (pairs ? 32L : (long)rows * cols));
+      v += f4{half_bits(l.x), half_bits(l.y), half_bits(l.z),
+              half_bits(l.w)};
+    }
+    return v;
+  }
+};
+
 // X0 in 64 x 64 tiles, transposed where the matrix is tall, zeros behind it.
-// g is [rows, cols]; X is [mp][np].
 __global__ __launch_bounds__(256) void ns_start_kernel(
     const void* __restrict__ g, int type, int rows, int cols, bool flip,
-    const double* __restrict__ part, int blocks, double eps, int mp, int np,
-    ushort* __restrict__ X, long xlo) {
+    const double* __restrict__ part, int blocks, double eps, Matrix X,
+    unsigned* __restrict__ tickets, int ntickets) {
   __shared__ float tile[64][65];
-  __shared__ double total;
-  if (threadIdx.x == 0) {
-    double s = 0.;
-    for (int i = 0; i < blocks; ++i) s += part[(long)blockIdx.z * blocks + i];
-    total = s;
+  __shared__ double red[64];
+  if (threadIdx.x < 64) {
+    red[threadIdx.x] = threadIdx.x < blocks
+                           ? part[(long)blockIdx.z * blocks + threadIdx.x]
+                           : 0.;
+  }
+  if (blockIdx.x + blockIdx.y == 0) {
+    for (int i = threadIdx.x; i < ntickets; i += 256)
+      tickets[(long)blockIdx.z * ntickets + i] = 0;
   }
   __syncthreads();
+  double total = 0.;
+  for (int i = 0; i < blocks; ++i) total += red[i];
   const double scale = kScale / (sqrt(total) + eps);
+  X = X.of(blockIdx.z);
   const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
   const int r0 = flip ? n0 : m0, c0 = flip ? m0 : n0;
   const long base = (long)blockIdx.z * rows * cols;
@@ -103,139 +154,272 @@ __global__ __launch_bounds__(256) void ns_start_kernel(
     tile[i >> 6][i & 63] = v;
   }
   __syncthreads();
-  ushort* out = X + (long)blockIdx.z * xlo * 2;
   for (int i = threadIdx.x; i < 4096; i += 256) {
     const int r = i >> 6, c = i & 63;
     const float v = flip ? tile[c][r] : tile[r][c];
     ushort h, l;
     split(v, h, l);
-    const long at = (long)(m0 + r) * np + n0 + c;
-    out[at] = h;
-    out[xlo + at] = l;
+    const long at = X.at(m0 + r, n0 + c);
+    X.p[at] = h;
+    X.p[at + (X.pairs ? 32L : (long)X.rows * X.cols)] = l;
   }
 }
 
-__device__ __forceinline__ void put(ushort* out, long lo, bool lo_too,
-                                    long at, float v) {
-  ushort h, l;
-  split(v, h, l);
-  out[at] = h;
-  if (lo_too) out[lo + at] = l;
+// A tile of values at (m0, n0) of `out`, whole.
+template <class C, int PARTS, bool LO, typename F>
+__device__ __forceinline__ void put_tile(char* lds, const Matrix& out, int m0,
+                                         int n0, F value) {
+  ushort* at = out.p + out.at(m0, n0);
+  if constexpr (PARTS == 2) {
+    store_pairs<C>(lds, at, 2L * out.cols, value);
+  } else {
+    store_tile<C>(lds, at, out.cols, C::BM, C::BN, [&](int i, int j) {
+      const f4 v = value(i, j);
+      ushort h[4], l;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) split(v[r], h[r], l);
+      return make_ushort4(h[0], h[1], h[2], h[3]);
+    });
+    if (LO) {
+      __syncthreads();
+      store_tile<C>(lds, at + (long)out.rows * out.cols, out.cols, C::BM,
+                    C::BN, [&](int i, int j) {
+        const f4 v = value(i, j);
+        ushort h, l[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) split(v[r], h, l[r]);
+        return make_ushort4(l[0], l[1], l[2], l[3]);
+      });
+    }
+  }
 }
 
 // One symmetric product [mp, mp]: S = sum_k P[i, k] P[j, k].
 //   SECOND = false: out = S                (P = X, S = A)
 //   SECOND = true:  out = b P + c S        (P = A, S = A A)
-template <class C, int SEG, bool SECOND>
-__global__ __launch_bounds__(C::THREADS, 2) void ns_sym_kernel(
-    const ushort* __restrict__ P, int ld, long plo, int kp, float b, float c,
-    int mp, ushort* __restrict__ out, long olo, bool old_lo, bool new_lo,
-    int tiles) {
+// Where there are few tiles, k is cut into `cuts`: each workgroup leaves its
+// sums in `part`, and the last one of a tile adds them up, in order.
+template <class C, int PARTS, bool SECOND>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
+    Matrix P, int kp, float b, float c, Matrix out, int tiles, int cuts,
+    float* __restrict__ part, unsigned* __restrict__ tickets) {
   static_assert(C::BM == C::BN, "square tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ bool last;
   // tile pairs on and above the diagonal, row by row
-  int t = blockIdx.x, ti = 0;
+  const int pairs = tiles * (tiles + 1) / 2;
+  const int cut = blockIdx.x / pairs, pair = blockIdx.x % pairs;
+  int t = pair, ti = 0;
   while (t >= tiles - ti) {
     t -= tiles - ti;
     ++ti;
   }
   const int m0 = ti * C::BM, n0 = (ti + t) * C::BN;
-  P += (long)blockIdx.y * plo * 2;
-  out += (long)blockIdx.y * olo * 2;
-  Operand o;
-  o.p = P;
-  o.lo = plo;
-  o.ld = ld;
-  o.rows = mp;
-  o.cols = ld;
+  P = P.of(blockIdx.y);
+  out = out.of(blockIdx.y);
+  const int each = (kp / 64 + cuts - 1) / cuts * 64;
+  const int k0 = cut * each, k1 = k0 + each < kp ? k0 + each : kp;
   f4 acc[C::FM][C::FN] = {};
-  product<C, KROWS, KROWS, SEG, false>(smem, o, m0, o, n0, 0, kp, acc);
+  if (k0 < k1) {
+    const Operand o = P.operand();
+    product<C, KROWS, KROWS, PARTS, false>(smem, o, m0, o, n0, k0, k1, acc);
+  }
+  if (cuts > 1) {
+    const long size = C::BM * C::BN;
+    f4* mine = reinterpret_cast<f4*>(
+        part + (((long)blockIdx.y * pairs + pair) * cuts) * size);
+    // in the order of the registers: 16 bytes of each thread next to one
+    // another
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j)
+        mine[cut * (size / 4) + (i * C::FN + j) * C::THREADS + threadIdx.x] =
+            acc[i][j];
+    __threadfence();
+    __syncthreads();
+    unsigned* ticket = tickets + (long)blockIdx.y * pairs + pair;
+    if (threadIdx.x == 0)
+      last = atomicAdd(ticket, 1u) == (unsigned)cuts - 1;
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) *ticket = 0;  // for the next product
+    __threadfence();
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) {
+        f4 v = {};
+        for (int q = 0; q < cuts; ++q)
+          v += mine[q * (size / 4) + (i * C::FN + j) * C::THREADS +
+                    threadIdx.x];
+        acc[i][j] = v;
+      }
+  }
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
 #pragma unroll
-  for (int i = 0; i < C::FM; ++i) {
-    const int m = m0 + wm + i * 16 + (lane & 15);
-    if (m >= mp) continue;
+  for (int i = 0; i < C::FM; ++i)
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) {
-      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (n >= mp) continue;
+      f4 v = acc[i][j] * (1.f / kScale);
+      if (SECOND)
+        v = b * P.four<PARTS == 2>(m0 + wm + i * 16 + (lane & 15),
+                                   n0 + wn + j * 16 + (lane >> 4) * 4) +
+            c * v;
+      acc[i][j] = v;
+    }
+  put_tile<C, PARTS, false>(smem, out, m0, n0,
+                            [&](int i, int j) { return acc[i][j]; });
+  if (m0 == n0) return;
+  // the mirrored tile, turned over in LDS
+  constexpr int ROW = PARTS == 2 ? C::PAIR_ROW : C::OUT_ROW;
+  constexpr int GOES = PARTS == 2 ? C::PAIR_GOES : 1;
+  constexpr int HALF = C::BM / GOES;
+  constexpr int PER_ROW = C::BN * PARTS / 8;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = acc[i][j][r] * (1.f / kScale);
-        if (SECOND) {
-          const long at = (long)m * ld + n + r;
-          float a = half_bits(P[at]);
-          if (old_lo) a += half_bits(P[plo + at]);
-          v = b * a + c * v;
-        }
-        put(out, olo, new_lo, (long)m * mp + n + r, v);
-        if (m0 != n0) put(out, olo, new_lo, (long)(n + r) * mp + m, v);
+  for (int go = 0; go < GOES; ++go) {
+    __syncthreads();
+    if (wn / HALF == go) {
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) {
+        const int m = wm + i * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            ushort h, l;
+            split(acc[i][j][r], h, l);
+            char* row =
+                smem + (wn % HALF + j * 16 + (lane >> 4) * 4 + r) * ROW;
+            if (PARTS == 2) {
+              ushort* at = reinterpret_cast<ushort*>(row) + (m >> 5) * 64 +
+                           (m & 31);
+              at[0] = h;
+              at[32] = l;
+            } else {
+              reinterpret_cast<ushort*>(row)[m] = h;
+            }
+          }
       }
+    }
+    __syncthreads();
+    ushort* to = out.p + out.at(n0 + go * HALF, m0);
+#pragma unroll 4
+    for (int q = threadIdx.x; q < HALF * PER_ROW; q += C::THREADS) {
+      const int r = q / PER_ROW, e = (q % PER_ROW) * 8;
+      *reinterpret_cast<s8*>(to + (long)r * out.cols * PARTS + e) =
+          *reinterpret_cast<const s8*>(smem + r * ROW + e * 2);
     }
   }
 }
 
 // X' = a X + B X; the last one goes to the result.
-template <class C, int SEG>
-__global__ __launch_bounds__(C::THREADS, 2) void ns_next_kernel(
-    const ushort* __restrict__ B, long blo, const ushort* __restrict__ X,
-    long xlo, float a, int mp, int np, ushort* __restrict__ out,
-    void* __restrict__ last, int type, int rows, int cols,
-    bool flip, int nnt) {
+template <class C, int PARTS>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void ns_next_kernel(
+    Matrix B, int kp, Matrix X, float a, Matrix out, void* __restrict__ last,
+    int type, int rows, int cols, bool flip, int nnt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int m0 = blockIdx.x / nnt * C::BM, n0 = blockIdx.x % nnt * C::BN;
-  B += (long)blockIdx.y * blo * 2;
-  X += (long)blockIdx.y * xlo * 2;
-  out += (long)blockIdx.y * xlo * 2;
-  Operand ob, ox;
-  ob.p = B;
-  ob.lo = blo;
-  ob.ld = mp;
-  ob.rows = mp;
-  ob.cols = mp;
-  ox.p = X;
-  ox.lo = xlo;
-  ox.ld = np;
-  ox.rows = mp;
-  ox.cols = np;
+  const int bid = die_contiguous(blockIdx.x, gridDim.x);
+  const int m0 = bid / nnt * C::BM, n0 = bid % nnt * C::BN;
+  B = B.of(blockIdx.y);
+  X = X.of(blockIdx.y);
   f4 acc[C::FM][C::FN] = {};
-  product<C, KROWS, KCOLS, SEG, false>(smem, ob, m0, ox, n0, 0, mp, acc);
+  product<C, KROWS, KCOLS, PARTS, false>(smem, B.operand(), m0, X.operand(),
+                                         n0, 0, kp, acc);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
+#pragma unroll
+  for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+      acc[i][j] = a * X.four<true>(m0 + wm + i * 16 + (lane & 15),
+                                   n0 + wn + j * 16 + (lane >> 4) * 4) +
+                  acc[i][j] * (1.f / kScale);
+  const auto value = [&](int i, int j) { return acc[i][j]; };
+  if (last == nullptr) {
+    out = out.of(blockIdx.y);
+    if (out.pairs) {
+      put_tile<C, 2, true>(smem, out, m0, n0, value);
+    } else {
+      put_tile<C, 1, true>(smem, out, m0, n0, value);
+    }
+    return;
+  }
   const long base = (long)blockIdx.y * rows * cols;
+  if (type != 2 && !flip && cols % 8 == 0) {
+    store_tile<C>(smem, static_cast<ushort*>(last) + base + (long)m0 * cols +
+                            n0,
+                  cols, rows - m0, cols - n0, [&](int i, int j) {
+      ushort u[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        store_as(u, r, type, acc[i][j][r] * (1.f / kScale));
+      return make_ushort4(u[0], u[1], u[2], u[3]);
+    });
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
     const int m = m0 + wm + i * 16 + (lane & 15);
-    if (m >= mp) continue;
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) {
       const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (n >= np) continue;
+      if (type == 2 && !flip && cols % 4 == 0) {
+        if (m < rows && n < cols)
+          *reinterpret_cast<f4*>(static_cast<float*>(last) + base +
+                                 (long)m * cols + n) =
+              acc[i][j] * (1.f / kScale);
+        continue;
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const long at = (long)m * np + n + r;
-        const float x = half_bits(X[at]) + half_bits(X[xlo + at]);
-        const float v = a * x + acc[i][j][r] * (1.f / kScale);
-        if (last == nullptr) {
-          put(out, xlo, true, at, v);
-        } else {
-          const int row = flip ? n + r : m, col = flip ? m : n + r;
-          if (row < rows && col < cols)
-            store_as(last, base + (long)row * cols + col, type,
-                     v * (1.f / kScale));
-        }
+        const int row = flip ? n + r : m, col = flip ? m : n + r;
+        if (row < rows && col < cols)
+          store_as(last, base + (long)row * cols + col, type,
+                   acc[i][j][r] * (1.f / kScale));
       }
     }
   }
 }
 
-using Wide = Tile<128, 128, 64, 64, 32, 3>;
-using Small = Tile<64, 64, 32, 32, 32, 3>;
+using Big = Tile<256, 256, 64, 64, 64, 2>;
+using Mid = Tile<128, 128, 64, 64, 64, 2>;
+using Small = Tile<64, 64, 32, 32, 64, 2>;
+
+template <typename K>
+void allow_lds(K kernel, int bytes) {
+  if (bytes <= 64 * 1024) return;
+  static std::mutex lock;
+  static std::set<std::pair<const void*, int>> done;
+  int device = 0;
+  TORCH_CHECK(hipGetDevice(&device) == hipSuccess, "hipGetDevice failed");
+  const auto key = std::make_pair(reinterpret_cast<const void*>(kernel),
+                                  device);
+  std::lock_guard<std::mutex> hold(lock);
+  if (done.count(key)) return;
+  const hipError_t e = hipFuncSetAttribute(
+      key.first, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  TORCH_CHECK(e == hipSuccess, "newton_schulz: ", bytes, " bytes of LDS: ",
+              hipGetErrorString(e));
+  done.insert(key);
+}
+
+// f(tile) for a tile size of 64, 128 or 256
+template <typename F>
+void with_tile(int size, F f) {
+  if (size == 256) {
+    f(Big{});
+  } else if (size == 128) {
+    f(Mid{});
+  } else {
+    f(Small{});
+  }
+}
 
 }  // namespace
 
@@ -262,78 +446,116 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
   const long batch = g.size(0), rows = g.size(1), cols = g.size(2);
   TORCH_CHECK(steps >= 1 && steps <= 64, "newton_schulz: 1 to 64 steps");
   TORCH_CHECK(batch <= 65535, "newton_schulz: at most 65535 matrices");
-  TORCH_CHECK(rows <= 32768 && cols <= 32768 &&
-                  std::min(rows, cols) <= 16384,
-              "newton_schulz: matrices up to 16384 x 32768");
+  TORCH_CHECK(rows <= 32768 && cols <= 32768 && rows * cols <= (1L << 28),
+              "newton_schulz: matrices of up to 32768 rows and columns and "
+              "2^28 values");
   if (g.numel() == 0) return;
   const c10::cuda::CUDAGuard guard(g.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool flip = rows > cols;
-  const int mp = (int)up(std::min(rows, cols), 64);
-  const int np = (int)up(std::max(rows, cols), 64);
-  const long xlo = (long)mp * np, alo = (long)mp * mp;
-  auto u16 = g.options().dtype(at::kShort);
-  const int blocks = (int)std::min<long>(64, (rows * cols + 2047) / 2048);
-  auto part = at::empty({batch, blocks}, g.options().dtype(at::kDouble));
-  // a high and a low plane for each matrix
-  auto xa = at::empty({batch, 2, mp, np}, u16);
-  auto xb = at::empty({batch, 2, mp, np}, u16);
-  auto A = at::empty({batch, 2, mp, mp}, u16);
-  auto B = at::empty({batch, 2, mp, mp}, u16);
-  auto ptr = [](at::Tensor& t) {
-    return reinterpret_cast<ushort*>(t.data_ptr());
-  };
-  ns_norm_kernel<<<dim3(blocks, batch), 256, 0, stream>>>(
-      g.data_ptr(), type, rows * cols, part.data_ptr<double>(), blocks);
-  HIP_CHECK_KERNEL();
-  const bool every = exact || std::min(rows, cols) < 256;
+  const long small = std::min(rows, cols), large = std::max(rows, cols);
+  const bool every = exact || small < 256;
   auto fine = [&](int64_t i) { return every || i >= steps - 3; };
-  ns_start_kernel<<<dim3(np / 64, mp / 64, batch), 256, 0, stream>>>(
-      g.data_ptr(), type, (int)rows, (int)cols, flip,
-      part.data_ptr<double>(), blocks, eps, mp, np, ptr(xa), xlo);
+
+  // The largest tile that still gives the chip's 256 CUs something to do;
+  // the symmetric products may cut k as well.
+  auto full_tiles = [&](long t) {
+    return (small + t - 1) / t * ((large + t - 1) / t) * batch;
+  };
+  auto sym_tiles = [&](long t) {
+    const long n = (small + t - 1) / t;
+    return n * (n + 1) / 2 * batch;
+  };
+  const int full = full_tiles(256) >= 200 ? 256
+                   : full_tiles(128) >= 128 ? 128 : 64;
+  const int sym = sym_tiles(256) >= 200 ? 256
+                  : sym_tiles(128) >= 30 ? 128 : 64;
+  auto cuts_of = [&](long k) {
+    const long slots = sym == 256 ? 256 : 512;
+    return (int)std::max(1L, std::min({slots / sym_tiles(sym), k / 512,
+                                       8L}));
+  };
+  const int tile = std::max(full, sym);
+  const int mp = (int)up(small, tile), np = (int)up(large, tile);
+  const int km = (int)up(small, 64), kn = (int)up(large, 64);
+  const long pairs = (long)(mp / sym) * (mp / sym + 1) / 2;
+  const int cuts = std::max(cuts_of(kn), cuts_of(km));
+  const int blocks = (int)std::min<long>(64, (rows * cols + 2047) / 2048);
+
+  // one allocation: two X, A, B, the norm's partial sums, the cut sums
+  const long xs = 2L * mp * np, as = 2L * mp * mp;
+  size_t bytes = 0;
+  auto take = [&](size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  const size_t o_x0 = take(batch * xs * 2), o_x1 = take(batch * xs * 2);
+  const size_t o_a = take(batch * as * 2), o_b = take(batch * as * 2);
+  const size_t o_norm = take(batch * blocks * sizeof(double));
+  const size_t o_part =
+      take(cuts > 1 ? batch * pairs * cuts * sym * sym * 4 : 0);
+  const size_t o_ticket = take(batch * pairs * 4);
+  auto mem = at::empty({(long)bytes}, g.options().dtype(at::kByte));
+  char* base = static_cast<char*>(mem.data_ptr());
+  auto matrix = [&](size_t at, long stride, int r, int c, bool in_pairs) {
+    return Matrix{reinterpret_cast<ushort*>(base + at), stride, r, c,
+                  in_pairs};
+  };
+  double* norm = reinterpret_cast<double*>(base + o_norm);
+  float* part = reinterpret_cast<float*>(base + o_part);
+  unsigned* tickets = reinterpret_cast<unsigned*>(base + o_ticket);
+
+  ns_norm_kernel<<<dim3(blocks, batch), 256, 0, stream>>>(
+      g.data_ptr(), type, rows * cols, norm, blocks);
   HIP_CHECK_KERNEL();
-  auto run = [&](auto tile) {
-    using C = decltype(tile);
-    const int tiles = (mp + C::BM - 1) / C::BM;
-    const int nnt = (np + C::BN - 1) / C::BN;
-    const dim3 sym(tiles * (tiles + 1) / 2, batch), full(tiles * nnt, batch);
-    for (int64_t i = 0; i < steps; ++i) {
-      const bool f = fine(i);
-      auto first = [&](auto kernel) {
-        kernel<<<sym, C::THREADS, C::LDS_BYTES, stream>>>(
-            ptr(xa), np, xlo, np, 0.f, 0.f, mp, ptr(A), alo, false, f, tiles);
+  ns_start_kernel<<<dim3(np / 64, mp / 64, batch), 256, 0, stream>>>(
+      g.data_ptr(), type, (int)rows, (int)cols, flip, norm, blocks, eps,
+      matrix(o_x0, xs, mp, np, fine(0)), tickets, (int)pairs);
+  HIP_CHECK_KERNEL();
+  for (int64_t i = 0; i < steps; ++i) {
+    const bool f = fine(i);
+    const Matrix X = matrix(i % 2 ? o_x1 : o_x0, xs, mp, np, f);
+    const Matrix Y = matrix(i % 2 ? o_x0 : o_x1, xs, mp, np, fine(i + 1));
+    const Matrix A = matrix(o_a, as, mp, mp, f);
+    const Matrix B = matrix(o_b, as, mp, mp, f);
+    with_tile(sym, [&](auto t) {
+      using C = decltype(t);
+      const int tiles = mp / C::BM;
+      auto launch = [&](auto kernel, int lds, const Matrix& P, int k,
+                        const Matrix& o) {
+        allow_lds(kernel, lds);
+        const int cut = cuts_of(k);
+        kernel<<<dim3(tiles * (tiles + 1) / 2 * cut, batch), C::THREADS, lds,
+                 stream>>>(P, k, (float)b, (float)c, o, tiles, cut, part,
+                           tickets);
         HIP_CHECK_KERNEL();
       };
-      auto second = [&](auto kernel) {
-        kernel<<<sym, C::THREADS, C::LDS_BYTES, stream>>>(
-            ptr(A), mp, alo, mp, (float)b, (float)c, mp, ptr(B), alo, f, f,
-            tiles);
-        HIP_CHECK_KERNEL();
-      };
-      auto third = [&](auto kernel) {
-        kernel<<<full, C::THREADS, C::LDS_BYTES, stream>>>(
-            ptr(B), alo, ptr(xa), xlo, (float)a, mp, np, ptr(xb),
+      if (f) {
+        launch(ns_sym_kernel<C, 2, false>, C::template lds<2>(), X, kn, A);
+        launch(ns_sym_kernel<C, 2, true>, C::template lds<2>(), A, km, B);
+      } else {
+        launch(ns_sym_kernel<C, 1, false>, C::template lds<1>(), X, kn, A);
+        launch(ns_sym_kernel<C, 1, true>, C::template lds<1>(), A, km, B);
+      }
+    });
+    with_tile(full, [&](auto t) {
+      using C = decltype(t);
+      auto launch = [&](auto kernel) {
+        constexpr int lds = C::template lds<2>();
+        allow_lds(kernel, lds);
+        const int nnt = np / C::BN;
+        kernel<<<dim3(mp / C::BM * nnt, batch), C::THREADS, lds, stream>>>(
+            B, km, X, (float)a, Y,
             i + 1 == steps ? out.data_ptr() : nullptr, type, (int)rows,
             (int)cols, flip, nnt);
         HIP_CHECK_KERNEL();
       };
       if (f) {
-        first(ns_sym_kernel<C, 3, false>);
-        second(ns_sym_kernel<C, 3, true>);
-        third(ns_next_kernel<C, 3>);
+        launch(ns_next_kernel<C, 2>);
       } else {
-        first(ns_sym_kernel<C, 1, false>);
-        second(ns_sym_kernel<C, 1, true>);
-        third(ns_next_kernel<C, 1>);
+        launch(ns_next_kernel<C, 1>);
       }
-      std::swap(xa, xb);
-    }
-  };
-  // 128-wide tiles once they fill the chip
-  const long wide = (long)((mp + 127) / 128) * ((np + 127) / 128) * batch;
-  if (wide >= 256) {
-    run(Wide{});
-  } else {
-    run(Small{});
+    });
   }
 }

@@ -22,21 +22,20 @@ class _LinearCEFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, labels, ignore_index, smoothing,
                 reduction):
-        loss, lse, total, tops = _ops.ext().linear_ce_fwd(
+        loss, saved = _ops.ext().linear_ce_fwd(
             x, weight, bias, labels, ignore_index, smoothing, reduction)
-        ctx.save_for_backward(x, weight, bias, labels, lse, total, tops)
+        ctx.save_for_backward(x, weight, bias, labels, saved)
         ctx.args = (ignore_index, smoothing, reduction)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, weight, bias, labels, lse, total, tops = ctx.saved_tensors
+        x, weight, bias, labels, saved = ctx.saved_tensors
         want = ctx.needs_input_grad
         dx, dw, db = _ops.ext().linear_ce_bwd(
-            dloss.float().contiguous(), x, weight, bias, labels, lse, total,
-            tops, *ctx.args, want[0], want[1],
-            bias is not None and want[2])
+            dloss.contiguous(), x, weight, bias, labels, saved, *ctx.args,
+            want[0], want[1], bias is not None and want[2])
         return dx, dw, db, None, None, None, None
 
 

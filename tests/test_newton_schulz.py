@@ -169,7 +169,7 @@ def test_refusals(dev):
     if dev == 'cuda':
         with pytest.raises(RuntimeError, match='bf16, fp16 or fp32'):
             f(g.double())
-        with pytest.raises(RuntimeError, match='16384'):
+        with pytest.raises(RuntimeError, match='32768'):
             f(torch.zeros(1, 40000, device=dev))
 
 
