@@ -174,7 +174,8 @@ std::vector<at::Tensor> linear_ce_bwd(
 
 // newton_schulz.hip
 void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
-                   double a, double b, double c, double eps, bool exact);
+                   double a, double b, double c, double eps, bool exact,
+                   int64_t turned);
 
 // rotary.hip
 std::vector<at::Tensor> rotary(const at::Tensor& q,

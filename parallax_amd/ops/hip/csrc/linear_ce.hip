@@ -47,7 +47,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // G of one piece of the vocabulary takes at most this much
 constexpr long kPieceBytes = 176L << 20;
 // and so do the split parts of an fp32 table's piece
-constexpr long kSplitBytes = 64L << 20;
+constexpr long kSplitBytes = 128L << 20;
 
 __host__ __device__ inline long up(long x, long m) {
   return (x + m - 1) / m * m;
@@ -156,7 +156,6 @@ struct Pack {
   int ntop;
   float* inv;
   float* bmax;
-  unsigned* zero;     // a counter to clear
   // backward: the rows, and sc = {S, 1/S} for 16-bit G
   Row* row;
   const float* dloss; // one or (each) of every row
@@ -198,7 +197,6 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
     scale = scale_to_half(block_reduce_max(t, scratch));
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    if (p.zero) *p.zero = 0;
     if (p.sc && !p.each) {
       // |softmax - target| <= 1, so S |G| stays below 2^14
       const float g = p.dloss[0] / (p.count ? p.count[0] : 1.f);
@@ -457,10 +455,6 @@ struct Join {
   float eps;
   float* loss;
   float* lse;
-  int reduction;     // 0: none, 1: mean, 2: sum
-  unsigned* ticket;
-  float* out;        // the scalar
-  float* count;      // rows that count
 };
 
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
@@ -471,12 +465,8 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 }
 
 // One wave a row: joins its partial sums, takes the label's logit as a dot
-// product, and the loss.  The last workgroup to finish adds the losses up,
-// in the rows' order.
+// product, and the loss.
 __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
-  __shared__ double sd[256];
-  __shared__ int sn[256];
-  __shared__ bool last;
   const int lane = threadIdx.x & 63;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r < p.n) {
@@ -516,24 +506,27 @@ __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
       p.loss[r] = live ? out : 0.f;
     }
   }
-  if (p.reduction == 0) return;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0)
-    last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
+}
+
+// Sum or mean of the rows that are not ignored, and their number, in the
+// rows' order.  (Left to the last workgroup of the join, its fences cost
+// 20 us: a kernel of its own takes 5.)
+__global__ __launch_bounds__(1024) void lce_total_kernel(
+    const float* __restrict__ loss, const int64_t* __restrict__ labels,
+    int64_t ignore, int n, bool mean, float* __restrict__ out,
+    float* __restrict__ count) {
+  __shared__ double sd[1024];
+  __shared__ int sn[1024];
   double a = 0.;
   int c = 0;
-  for (int i = threadIdx.x; i < p.n; i += 256) {
-    a += p.loss[i];
-    c += p.labels[i] != p.ignore;
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    a += loss[i];
+    c += labels[i] != ignore;
   }
   sd[threadIdx.x] = a;
   sn[threadIdx.x] = c;
   __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
+  for (int o = 512; o > 0; o >>= 1) {
     if (threadIdx.x < o) {
       sd[threadIdx.x] += sd[threadIdx.x + o];
       sn[threadIdx.x] += sn[threadIdx.x + o];
@@ -541,8 +534,8 @@ __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    p.out[0] = (float)(p.reduction == 1 ? sd[0] / sn[0] : sd[0]);
-    p.count[0] = (float)sn[0];
+    out[0] = (float)(mean ? sd[0] / sn[0] : sd[0]);
+    count[0] = (float)sn[0];
   }
 }
 
@@ -770,7 +763,8 @@ using Big = Tile<256, 256, 64, 64, 64, 2>;
 using Mid = Tile<128, 128, 64, 64, 64, 2>;
 // few rows: wide in the words
 using Flat = Tile<64, 256, 64, 32, 64, 2>;
-using Small = Tile<64, 64, 32, 32, 64, 2>;
+// few tiles: four stages deep, as a workgroup has a CU for itself
+using Small = Tile<64, 64, 32, 32, 64, 4>;
 
 int type_code(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -1033,7 +1027,6 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
     const auto o_winv = mem.take<float>(p.parts == 2 ? p.w_rows : 0);
     const auto o_part = mem.take<float>(p.n * blocks * (eps != 0.f ? 4 : 2));
     const auto o_loss = mem.take<float>(reduction == 0 ? 0 : p.n);
-    const auto o_ticket = mem.take<unsigned>(1);
     mem.allocate(x);
 
     Pack kx = pack_of(x, 0, p.n, p.np, p,
@@ -1042,7 +1035,6 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
     kx.labels = lab;
     kx.ignore = ignore;
     kx.inv = mem.at<float>(o_xinv);
-    kx.zero = mem.at<unsigned>(o_ticket);
     pack(kx, stream);
     for (long i = 0; i < pieces; ++i) {
       const long v0 = i * piece, vp = std::min(piece, p.v - v0);
@@ -1102,12 +1094,14 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
     j.eps = eps;
     j.loss = reduction == 0 ? out.data_ptr<float>() : mem.at<float>(o_loss);
     j.lse = lse;
-    j.reduction = (int)reduction;
-    j.ticket = mem.at<unsigned>(o_ticket);
-    j.out = out.data_ptr<float>();
-    j.count = lse + p.n;
     lce_join_kernel<<<(int)((p.n + 3) / 4), 256, 0, stream>>>(j);
     HIP_CHECK_KERNEL();
+    if (reduction != 0) {
+      lce_total_kernel<<<1, 1024, 0, stream>>>(
+          j.loss, lab, ignore, (int)p.n, reduction == 1,
+          out.data_ptr<float>(), lse + p.n);
+      HIP_CHECK_KERNEL();
+    }
   });
   return {out, saved};
 }

@@ -66,6 +66,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(
   __shared__ double red[256];
   const long base = (long)blockIdx.y * count;
   double s = 0.;
+#pragma unroll 4
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count;
        i += (long)gridDim.x * 256) {
     const double v = load_as(g, base + i, type);
@@ -122,26 +123,33 @@ struct Matrix {
   }
 };
 
+// The matrices of a batch are small x large, from `first_tall` on large x
+// small as they lie.
+struct Shape {
+  int small, large, first_tall;
+  __device__ __forceinline__ bool tall(int batch) const {
+    return batch >= first_tall;
+  }
+};
+
 // X0 in 64 x 64 tiles, transposed where the matrix is tall, zeros behind it.
 __global__ __launch_bounds__(256) void ns_start_kernel(
-    const void* __restrict__ g, int type, int rows, int cols, bool flip,
-    const double* __restrict__ part, int blocks, double eps, Matrix X,
-    unsigned* __restrict__ tickets, int ntickets) {
+    const void* __restrict__ g, int type, Shape shape,
+    const double* __restrict__ part, int blocks, double eps, Matrix X) {
   __shared__ float tile[64][65];
-  __shared__ double red[64];
-  if (threadIdx.x < 64) {
-    red[threadIdx.x] = threadIdx.x < blocks
-                           ? part[(long)blockIdx.z * blocks + threadIdx.x]
-                           : 0.;
-  }
-  if (blockIdx.x + blockIdx.y == 0) {
-    for (int i = threadIdx.x; i < ntickets; i += 256)
-      tickets[(long)blockIdx.z * ntickets + i] = 0;
-  }
+  __shared__ double red[256];
+  const bool flip = shape.tall(blockIdx.z);
+  const int rows = flip ? shape.large : shape.small;
+  const int cols = flip ? shape.small : shape.large;
+  red[threadIdx.x] = threadIdx.x < blocks
+                         ? part[(long)blockIdx.z * blocks + threadIdx.x]
+                         : 0.;
   __syncthreads();
-  double total = 0.;
-  for (int i = 0; i < blocks; ++i) total += red[i];
-  const double scale = kScale / (sqrt(total) + eps);
+  for (int o = 128; o > 0; o >>= 1) {
+    if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  const double scale = kScale / (sqrt(red[0]) + eps);
   X = X.of(blockIdx.z);
   const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
   const int r0 = flip ? n0 : m0, c0 = flip ? m0 : n0;
@@ -197,18 +205,20 @@ __device__ __forceinline__ void put_tile(char* lds, const Matrix& out, int m0,
 // One symmetric product [mp, mp]: S = sum_k P[i, k] P[j, k].
 //   SECOND = false: out = S                (P = X, S = A)
 //   SECOND = true:  out = b P + c S        (P = A, S = A A)
-// Where there are few tiles, k is cut into `cuts`: each workgroup leaves its
-// sums in `part`, and the last one of a tile adds them up, in order.
-template <class C, int PARTS, bool SECOND>
+// Where there are few tiles, k is cut (CUT = 1): each workgroup leaves its
+// sums in `part`, and a second kernel (CUT = 2) adds them up in order and
+// goes on.  (Left to the last workgroup of a tile, the fences that takes
+// cost more than the launch: 146 us for 12 x 512 x 2048, 50 this way.)
+template <class C, int PARTS, bool SECOND, int CUT>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
     Matrix P, int kp, float b, float c, Matrix out, int tiles, int cuts,
-    float* __restrict__ part, unsigned* __restrict__ tickets) {
+    float* __restrict__ part) {
   static_assert(C::BM == C::BN, "square tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ bool last;
   // tile pairs on and above the diagonal, row by row
   const int pairs = tiles * (tiles + 1) / 2;
-  const int cut = blockIdx.x / pairs, pair = blockIdx.x % pairs;
+  const int cut = CUT == 1 ? blockIdx.x / pairs : 0;
+  const int pair = CUT == 1 ? blockIdx.x % pairs : blockIdx.x;
   int t = pair, ti = 0;
   while (t >= tiles - ti) {
     t -= tiles - ti;
@@ -217,44 +227,35 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
   const int m0 = ti * C::BM, n0 = (ti + t) * C::BN;
   P = P.of(blockIdx.y);
   out = out.of(blockIdx.y);
-  const int each = (kp / 64 + cuts - 1) / cuts * 64;
-  const int k0 = cut * each, k1 = k0 + each < kp ? k0 + each : kp;
   f4 acc[C::FM][C::FN] = {};
-  if (k0 < k1) {
-    const Operand o = P.operand();
-    product<C, KROWS, KROWS, PARTS, false>(smem, o, m0, o, n0, k0, k1, acc);
-  }
-  if (cuts > 1) {
-    const long size = C::BM * C::BN;
-    f4* mine = reinterpret_cast<f4*>(
-        part + (((long)blockIdx.y * pairs + pair) * cuts) * size);
-    // in the order of the registers: 16 bytes of each thread next to one
-    // another
+  // a cut's sums lie in the order of the registers: 16 bytes of each thread
+  // next to one another
+  constexpr long SIZE = C::BM * C::BN / 4;
+  f4* sums = reinterpret_cast<f4*>(part) +
+             (((long)blockIdx.y * pairs + pair) * cuts) * SIZE + threadIdx.x;
+  if constexpr (CUT == 2) {
+    for (int q = 0; q < cuts; ++q)
 #pragma unroll
-    for (int i = 0; i < C::FM; ++i)
+      for (int i = 0; i < C::FM; ++i)
 #pragma unroll
-      for (int j = 0; j < C::FN; ++j)
-        mine[cut * (size / 4) + (i * C::FN + j) * C::THREADS + threadIdx.x] =
-            acc[i][j];
-    __threadfence();
-    __syncthreads();
-    unsigned* ticket = tickets + (long)blockIdx.y * pairs + pair;
-    if (threadIdx.x == 0)
-      last = atomicAdd(ticket, 1u) == (unsigned)cuts - 1;
-    __syncthreads();
-    if (!last) return;
-    if (threadIdx.x == 0) *ticket = 0;  // for the next product
-    __threadfence();
+        for (int j = 0; j < C::FN; ++j)
+          acc[i][j] += sums[q * SIZE + (i * C::FN + j) * C::THREADS];
+  } else {
+    const int each = CUT == 1 ? (kp / 64 + cuts - 1) / cuts * 64 : kp;
+    const int k0 = cut * each, k1 = k0 + each < kp ? k0 + each : kp;
+    if (k0 < k1) {
+      const Operand o = P.operand();
+      product<C, KROWS, KROWS, PARTS, false>(smem, o, m0, o, n0, k0, k1,
+                                             acc);
+    }
+    if constexpr (CUT == 1) {
 #pragma unroll
-    for (int i = 0; i < C::FM; ++i)
+      for (int i = 0; i < C::FM; ++i)
 #pragma unroll
-      for (int j = 0; j < C::FN; ++j) {
-        f4 v = {};
-        for (int q = 0; q < cuts; ++q)
-          v += mine[q * (size / 4) + (i * C::FN + j) * C::THREADS +
-                    threadIdx.x];
-        acc[i][j] = v;
-      }
+        for (int j = 0; j < C::FN; ++j)
+          sums[cut * SIZE + (i * C::FN + j) * C::THREADS] = acc[i][j];
+      return;
+    }
   }
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
@@ -320,8 +321,11 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
 template <class C, int PARTS>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_next_kernel(
     Matrix B, int kp, Matrix X, float a, Matrix out, void* __restrict__ last,
-    int type, int rows, int cols, bool flip, int nnt) {
+    int type, Shape shape, int nnt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  const bool flip = shape.tall(blockIdx.y);
+  const int rows = flip ? shape.large : shape.small;
+  const int cols = flip ? shape.small : shape.large;
   const int bid = die_contiguous(blockIdx.x, gridDim.x);
   const int m0 = bid / nnt * C::BM, n0 = bid % nnt * C::BN;
   B = B.of(blockIdx.y);
@@ -389,7 +393,9 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_next_kernel(
 
 using Big = Tile<256, 256, 64, 64, 64, 2>;
 using Mid = Tile<128, 128, 64, 64, 64, 2>;
-using Small = Tile<64, 64, 32, 32, 64, 2>;
+// few tiles: four stages deep, as a workgroup has a CU for itself
+using Deep = Tile<128, 128, 64, 64, 64, 4>;
+using Small = Tile<64, 64, 32, 32, 64, 4>;
 
 template <typename K>
 void allow_lds(K kernel, int bytes) {
@@ -409,13 +415,15 @@ void allow_lds(K kernel, int bytes) {
   done.insert(key);
 }
 
-// f(tile) for a tile size of 64, 128 or 256
+// f(tile) for a tile size of 64, 128 or 256, and so many workgroups
 template <typename F>
-void with_tile(int size, F f) {
+void with_tile(int size, long groups, F f) {
   if (size == 256) {
     f(Big{});
-  } else if (size == 128) {
+  } else if (size == 128 && groups > 256) {
     f(Mid{});
+  } else if (size == 128) {
+    f(Deep{});
   } else {
     f(Small{});
   }
@@ -424,9 +432,11 @@ void with_tile(int size, F f) {
 }  // namespace
 
 // g [batch, rows, cols] -> out of the same shape and type, which may be g.
+// The matrices from `turned` on lie as [cols, rows].
 // exact: two-part operands in every product, whatever the size.
 void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
-                   double a, double b, double c, double eps, bool exact) {
+                   double a, double b, double c, double eps, bool exact,
+                   int64_t turned) {
   TORCH_CHECK(g.is_cuda() && g.dim() == 3 && g.is_contiguous(),
               "newton_schulz: contiguous [batch, rows, cols] on the GPU "
               "expected");
@@ -444,6 +454,9 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
                   g.scalar_type());
   }
   const long batch = g.size(0), rows = g.size(1), cols = g.size(2);
+  TORCH_CHECK(turned >= 0 && turned <= batch &&
+                  (turned == batch || rows <= cols),
+              "newton_schulz: wide matrices first");
   TORCH_CHECK(steps >= 1 && steps <= 64, "newton_schulz: 1 to 64 steps");
   TORCH_CHECK(batch <= 65535, "newton_schulz: at most 65535 matrices");
   TORCH_CHECK(rows <= 32768 && cols <= 32768 && rows * cols <= (1L << 28),
@@ -452,8 +465,9 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
   if (g.numel() == 0) return;
   const c10::cuda::CUDAGuard guard(g.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  const bool flip = rows > cols;
   const long small = std::min(rows, cols), large = std::max(rows, cols);
+  const Shape shape{(int)small, (int)large,
+                    rows > cols ? 0 : (int)turned};
   const bool every = exact || small < 256;
   auto fine = [&](int64_t i) { return every || i >= steps - 3; };
 
@@ -480,7 +494,8 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
   const int km = (int)up(small, 64), kn = (int)up(large, 64);
   const long pairs = (long)(mp / sym) * (mp / sym + 1) / 2;
   const int cuts = std::max(cuts_of(kn), cuts_of(km));
-  const int blocks = (int)std::min<long>(64, (rows * cols + 2047) / 2048);
+  // ~16 values a thread
+  const int blocks = (int)std::min<long>(256, (rows * cols + 4095) / 4096);
 
   // one allocation: two X, A, B, the norm's partial sums, the cut sums
   const long xs = 2L * mp * np, as = 2L * mp * mp;
@@ -495,7 +510,6 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
   const size_t o_norm = take(batch * blocks * sizeof(double));
   const size_t o_part =
       take(cuts > 1 ? batch * pairs * cuts * sym * sym * 4 : 0);
-  const size_t o_ticket = take(batch * pairs * 4);
   auto mem = at::empty({(long)bytes}, g.options().dtype(at::kByte));
   char* base = static_cast<char*>(mem.data_ptr());
   auto matrix = [&](size_t at, long stride, int r, int c, bool in_pairs) {
@@ -504,14 +518,13 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
   };
   double* norm = reinterpret_cast<double*>(base + o_norm);
   float* part = reinterpret_cast<float*>(base + o_part);
-  unsigned* tickets = reinterpret_cast<unsigned*>(base + o_ticket);
 
   ns_norm_kernel<<<dim3(blocks, batch), 256, 0, stream>>>(
       g.data_ptr(), type, rows * cols, norm, blocks);
   HIP_CHECK_KERNEL();
   ns_start_kernel<<<dim3(np / 64, mp / 64, batch), 256, 0, stream>>>(
-      g.data_ptr(), type, (int)rows, (int)cols, flip, norm, blocks, eps,
-      matrix(o_x0, xs, mp, np, fine(0)), tickets, (int)pairs);
+      g.data_ptr(), type, shape, norm, blocks, eps,
+      matrix(o_x0, xs, mp, np, fine(0)));
   HIP_CHECK_KERNEL();
   for (int64_t i = 0; i < steps; ++i) {
     const bool f = fine(i);
@@ -519,27 +532,36 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
     const Matrix Y = matrix(i % 2 ? o_x0 : o_x1, xs, mp, np, fine(i + 1));
     const Matrix A = matrix(o_a, as, mp, mp, f);
     const Matrix B = matrix(o_b, as, mp, mp, f);
-    with_tile(sym, [&](auto t) {
-      using C = decltype(t);
-      const int tiles = mp / C::BM;
-      auto launch = [&](auto kernel, int lds, const Matrix& P, int k,
-                        const Matrix& o) {
-        allow_lds(kernel, lds);
-        const int cut = cuts_of(k);
-        kernel<<<dim3(tiles * (tiles + 1) / 2 * cut, batch), C::THREADS, lds,
-                 stream>>>(P, k, (float)b, (float)c, o, tiles, cut, part,
-                           tickets);
-        HIP_CHECK_KERNEL();
-      };
-      if (f) {
-        launch(ns_sym_kernel<C, 2, false>, C::template lds<2>(), X, kn, A);
-        launch(ns_sym_kernel<C, 2, true>, C::template lds<2>(), A, km, B);
-      } else {
-        launch(ns_sym_kernel<C, 1, false>, C::template lds<1>(), X, kn, A);
-        launch(ns_sym_kernel<C, 1, true>, C::template lds<1>(), A, km, B);
-      }
-    });
-    with_tile(full, [&](auto t) {
+    auto symmetric = [&](auto second, const Matrix& P, int k,
+                         const Matrix& o) {
+      constexpr bool SECOND = decltype(second)::value;
+      const int tiles = mp / sym, cut = cuts_of(k);
+      const long groups = pairs * batch * cut;
+      with_tile(sym, groups, [&](auto t) {
+        using C = decltype(t);
+        auto launch = [&](auto kernel, int lds, int n) {
+          allow_lds(kernel, lds);
+          kernel<<<dim3(pairs * n, batch), C::THREADS, lds, stream>>>(
+              P, k, (float)b, (float)c, o, tiles, cut, part);
+          HIP_CHECK_KERNEL();
+        };
+        constexpr int one = C::template lds<1>(), two = C::template lds<2>();
+        if (cut > 1 && f) {
+          launch(ns_sym_kernel<C, 2, SECOND, 1>, two, cut);
+          launch(ns_sym_kernel<C, 2, SECOND, 2>, two, 1);
+        } else if (cut > 1) {
+          launch(ns_sym_kernel<C, 1, SECOND, 1>, one, cut);
+          launch(ns_sym_kernel<C, 1, SECOND, 2>, one, 1);
+        } else if (f) {
+          launch(ns_sym_kernel<C, 2, SECOND, 0>, two, 1);
+        } else {
+          launch(ns_sym_kernel<C, 1, SECOND, 0>, one, 1);
+        }
+      });
+    };
+    symmetric(std::false_type{}, X, kn, A);
+    symmetric(std::true_type{}, A, km, B);
+    with_tile(full, full_tiles(full), [&](auto t) {
       using C = decltype(t);
       auto launch = [&](auto kernel) {
         constexpr int lds = C::template lds<2>();
@@ -547,8 +569,7 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
         const int nnt = np / C::BN;
         kernel<<<dim3(mp / C::BM * nnt, batch), C::THREADS, lds, stream>>>(
             B, km, X, (float)a, Y,
-            i + 1 == steps ? out.data_ptr() : nullptr, type, (int)rows,
-            (int)cols, flip, nnt);
+            i + 1 == steps ? out.data_ptr() : nullptr, type, shape, nnt);
         HIP_CHECK_KERNEL();
       };
       if (f) {

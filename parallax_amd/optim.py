@@ -557,37 +557,38 @@ class Muon(Adam):
                   for p in params]
         shapes = [_storage_matrix(p) for p in params]
         exact = params[0].dtype != torch.bfloat16
-        # tall and wide ones of one size: a stack for each
-        for shape in dict.fromkeys(shapes):
-            ii = [i for i, s in enumerate(shapes) if s == shape]
-            ps, gs, bs = ([t[i] for i in ii] for t in (params, grads, bufs))
-            ms = [masters[i] for i in ii] if has_m else []
-            sc = [scales[i] for i in ii]
-            if not _use_native(ps):
-                for k, (p, g, b) in enumerate(zip(ps, gs, bs)):
-                    g = g.to(b.dtype)
-                    b.mul_(mom).add_(g)
-                    v = g.add(b, alpha=mom) if group['nesterov'] else b
-                    o = v.reshape(1, p.shape[0], -1).clone()
-                    _into(o, o, group['ns_steps'], COEFFICIENTS, 1e-7, exact)
-                    w = ms[k] if ms else p
-                    w.mul_(decay).add_(o.view(p.shape).to(w.dtype),
-                                       alpha=-sc[k])
-                    if w is not p:
-                        p.copy_(w)
-                continue
-            e = _ops.ext()
-            gs = [g if _same_layout(p, g)
-                  else torch.empty_like(p, dtype=g.dtype).copy_(g)
-                  for p, g in zip(ps, gs)]
-            u = torch.empty((len(ii),) + shape, dtype=torch.float32,
-                            device=ps[0].device)
-            us = list(u.unbind(0))
-            for gg, bb, uu in _dtype_groups(gs, bs, us):
-                e.multi_tensor_muon_update(gg, bb, uu, mom,
-                                           group['nesterov'])
-            _into(u, u, group['ns_steps'], COEFFICIENTS, 1e-7, exact)
-            e.multi_tensor_muon_apply(ps, us, sc, decay, ms)
+        if not _use_native(params):
+            for i, (p, g, b) in enumerate(zip(params, grads, bufs)):
+                g = g.to(b.dtype)
+                b.mul_(mom).add_(g)
+                v = g.add(b, alpha=mom) if group['nesterov'] else b
+                o = v.reshape(1, p.shape[0], -1).clone()
+                _into(o, o, group['ns_steps'], COEFFICIENTS, 1e-7, exact)
+                w = masters[i] if has_m else p
+                w.mul_(decay).add_(o.view(p.shape).to(w.dtype),
+                                   alpha=-scales[i])
+                if w is not p:
+                    p.copy_(w)
+            return
+        # one stack: the wide ones, then those that lie the other way round
+        order = sorted(range(len(params)),
+                       key=lambda i: shapes[i][0] > shapes[i][1])
+        params, grads, bufs, scales, shapes = (
+            [t[i] for i in order]
+            for t in (params, grads, bufs, scales, shapes))
+        masters = [masters[i] for i in order] if has_m else []
+        turned = sum(r <= c for r, c in shapes)
+        e = _ops.ext()
+        grads = [g if _same_layout(p, g)
+                 else torch.empty_like(p, dtype=g.dtype).copy_(g)
+                 for p, g in zip(params, grads)]
+        u = torch.empty((len(params),) + tuple(sorted(shapes[0])),
+                        dtype=torch.float32, device=params[0].device)
+        us = list(u.unbind(0))
+        for gg, bb, uu in _dtype_groups(grads, bufs, us):
+            e.multi_tensor_muon_update(gg, bb, uu, mom, group['nesterov'])
+        _into(u, u, group['ns_steps'], COEFFICIENTS, 1e-7, exact, turned)
+        e.multi_tensor_muon_apply(params, us, scales, decay, masters)
 
     @torch.no_grad()
     def sparse_row_step(self, param, ids, grad_rows, group=None,
