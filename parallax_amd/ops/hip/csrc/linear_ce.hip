@@ -97,6 +97,9 @@ struct Bias {
                      ? kLog2e * load_as(p, (v + r) * stride, type) : 0.f;
     }
   }
+  __device__ __forceinline__ float one(int v, int words) const {
+    return p && v < words ? kLog2e * load_as(p, v * stride, type) : 0.f;
+  }
 };
 
 __device__ __forceinline__ ushort bf16_bits(float v) {
@@ -127,13 +130,12 @@ __device__ __forceinline__ float scale_to_half(float top) {
 
 // --- laying out an operand --------------------------------------------------
 
-// What the gradient needs of a row.  Rows that do not count: an infinite l
-// makes their exponentials 0, and g = 0.
-struct Row {
-  float l;   // log2 e lse
-  float g;   // what the row's G is multiplied by
-  int y;     // label
-  float xs;  // scale to undo
+// What the gradient needs of the rows.  Rows that do not count: an infinite
+// l makes their exponentials 0, and g = 0.
+struct Rows {
+  float* l;  // log2 e lse
+  float* g;  // what the row's G is multiplied by
+  int* y;    // label
 };
 
 struct Pack {
@@ -157,7 +159,7 @@ struct Pack {
   float* inv;
   float* bmax;
   // backward: the rows, and sc = {S, 1/S} for 16-bit G
-  Row* row;
+  Rows row;
   const float* dloss; // one or (each) of every row
   bool each;
   const float* count;
@@ -211,17 +213,16 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
     if (p.labels && live) {
       const int64_t y = p.labels[r];
       live = y != p.ignore;
-      if (p.row && lane == 0) {
-        Row row = {INFINITY, 0.f, 0, 1.f};
-        row.y = (int)(y < 0 ? 0 : (y >= p.V ? p.V - 1 : y));
-        if (live) {
-          row.g = p.dloss[p.each ? r : 0] / (p.count ? p.count[0] : 1.f);
-          row.l = p.lse[r] * kLog2e;
-        }
-        p.row[r] = row;
+      if (p.row.l && lane == 0) {
+        const float g = p.dloss[p.each ? r : 0] / (p.count ? p.count[0] : 1.f);
+        p.row.l[r] = live ? p.lse[r] * kLog2e : INFINITY;
+        p.row.g[r] = live ? g : 0.f;
+        p.row.y[r] = (int)(y < 0 ? 0 : (y >= p.V ? p.V - 1 : y));
       }
-    } else if (p.row && lane == 0) {
-      p.row[r] = Row{INFINITY, 0.f, 0, 1.f};
+    } else if (p.row.l && lane == 0) {
+      p.row.l[r] = INFINITY;
+      p.row.g[r] = 0.f;
+      p.row.y[r] = 0;
     }
     const char* src = static_cast<const char*>(p.src) + r * p.rs * size;
     if constexpr (PARTS == 1) {
@@ -541,75 +542,76 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(
 
 // --- backward ---------------------------------------------------------------
 
-// G of one piece, [rows padded to BM][ldg]; zeros outside the matrix.
-// DB: column sums of each row tile into dbp[row tile][..], or as they are
-// into db where there is one.
+// G of one piece, transposed: [words][ldg], zeros outside the matrix.  The
+// words are the tile's m: a lane holds four neighbouring rows of one word,
+// sums over the rows stay in it, and dw reads G k-contiguous.
+// DB: sums of each tile of rows into dbp[row tile][..], or as they are into
+// db where there is one.
 template <class C, int XL, int PARTS, bool BF, bool DB>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
-    Logits p, const Row* __restrict__ rows, const float* __restrict__ sc,
-    long V, long v0, float eps, ushort* __restrict__ G, int ldg,
-    float* __restrict__ dbp, long db_ld, void* __restrict__ db, int db_type,
-    int nmt, int nvt) {
+    Logits p, Rows rows, const float* __restrict__ sc, long V, long v0,
+    float eps, ushort* __restrict__ G, int ldg, float* __restrict__ dbp,
+    long db_ld, void* __restrict__ db, int db_type, int nvt, int nrt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int bid = die_contiguous(blockIdx.x, nmt * nvt);
-  const int mt = bid % nmt, vt = bid / nmt;
-  const int m0 = mt * C::BM, n0 = vt * C::BN;
+  const int bid = die_contiguous(blockIdx.x, nvt * nrt);
+  const int rt = bid % nrt, vt = bid / nrt;
+  const int m0 = vt * C::BM, n0 = rt * C::BN;
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
   f4 acc[C::FM][C::FN] = {};
-  product<C, XL, KROWS, PARTS, BF>(smem, p.x, m0, p.w, n0, 0, p.dp, acc);
-  const int c0 = n0 + wn + (lane >> 4) * 4;
+  product<C, KROWS, XL, PARTS, BF>(smem, p.w, m0, p.x, n0, 0, p.dp, acc);
   const float S = sc[0], uni = eps / (float)V;
-  const float xs = PARTS == 2 ? p.xinv[0] : 1.f;  // one for all rows
-  float add[C::FN][4], ws[C::FN][4];
-#pragma unroll
-  for (int j = 0; j < C::FN; ++j) p.bias.load(add[j], c0 + j * 16, p.vp);
-#pragma unroll
-  for (int j = 0; j < C::FN; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int v = c0 + j * 16 + r;
-      ws[j][r] = PARTS == 2 && v < p.vp ? p.winv[v] * kLog2e : kLog2e;
-    }
+  const int w0 = m0 + wm + (lane & 15);  // this lane's first word
+  float add[C::FM], ws[C::FM], sum[C::FM];
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
-    // one load of 16 bytes: there are rows up to a whole tile
-    const f4 row = reinterpret_cast<const f4*>(
-        rows)[m0 + wm + i * 16 + (lane & 15)];
-    const float l = row[0], gm = row[1];
-#pragma unroll
-    for (int j = 0; j < C::FN; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float z = PARTS == 2 ? acc[i][j][r] * xs : acc[i][j][r];
-        acc[i][j][r] =
-            (exp2_fast(fmaf(z, ws[j][r], add[j][r] - l)) - uni) * gm;
-      }
-    // the label's word: in few tiles, so not a comparison for each value
-    const long y = (long)__builtin_bit_cast(int, (float)row[2]) - v0 - n0 - wn;
-    const int hit = y >= 0 && y < C::WN ? (int)y - (lane >> 4) * 4 : -1;
-    if (__any(hit >= 0)) {
-#pragma unroll
-      for (int j = 0; j < C::FN; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (hit == j * 16 + r) acc[i][j][r] -= (1.f - eps) * gm;
-    }
+    const int v = w0 + i * 16;
+    add[i] = p.bias.one(v, p.vp);
+    ws[i] = kLog2e;
+    // one scale to undo for all rows
+    if (PARTS == 2) ws[i] *= (v < p.vp ? p.winv[v] : 0.f) * p.xinv[0];
+    sum[i] = 0.f;
   }
-  if (n0 + C::BN > p.vp) {  // words behind the last one
 #pragma unroll
-    for (int j = 0; j < C::FN; ++j)
+  for (int j = 0; j < C::FN; ++j) {
+    // there are rows up to a whole tile
+    const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+    const f4 l = *reinterpret_cast<const f4*>(rows.l + n);
+    const f4 g = *reinterpret_cast<const f4*>(rows.g + n);
+    const int4 y = *reinterpret_cast<const int4*>(rows.y + n);
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (c0 + j * 16 + r >= p.vp) {
+        acc[i][j][r] =
+            fmaf(exp2_fast(fmaf(acc[i][j][r], ws[i], add[i] - l[r])), g[r],
+                 -uni * g[r]);
+    // the label's word: in few tiles, so not a comparison for each value
+    const int at[4] = {y.x, y.y, y.z, y.w};
+    const int first = (int)v0 + m0 + wm;
+    bool hit = false;
 #pragma unroll
-          for (int i = 0; i < C::FM; ++i) acc[i][j][r] = 0.f;
-        }
+    for (int r = 0; r < 4; ++r)
+      hit |= (unsigned)(at[r] - first) < (unsigned)C::WM;
+    if (__any(hit)) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < C::FM; ++i)
+          if (at[r] - first == i * 16 + (lane & 15))
+            acc[i][j][r] -= (1.f - eps) * g[r];
+    }
   }
+#pragma unroll
+  for (int i = 0; i < C::FM; ++i)
+    if (w0 + i * 16 >= p.vp) {  // words behind the last one
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+    }
   if constexpr (PARTS == 2) {
-    store_pairs<C>(smem, G + ((long)m0 * ldg + n0) * 2, 2L * ldg,
+    store_pairs<C>(smem, G + (long)m0 * ldg + n0 * 2, ldg,
                    [&](int i, int j) { return acc[i][j] * S; });
   } else {
     store_tile<C>(smem, G + (long)m0 * ldg + n0, ldg, C::BM, C::BN,
@@ -623,28 +625,30 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     });
   }
   if (DB) {
-    float* red = reinterpret_cast<float*>(smem);  // [waves_m][BN]
+    float* red = reinterpret_cast<float*>(smem);  // [waves_n][BM]
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[i] += acc[i][j][r];
+      sum[i] += __shfl_xor(sum[i], 16, 64);
+      sum[i] += __shfl_xor(sum[i], 32, 64);
+    }
     __syncthreads();
+    if (lane < 16) {
 #pragma unroll
-    for (int j = 0; j < C::FN; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float c = 0.f;
-#pragma unroll
-        for (int i = 0; i < C::FM; ++i) c += acc[i][j][r];
-        c = sum16(c);
-        if ((lane & 15) == 0)
-          red[(wave / C::WAVES_N) * C::BN + wn + j * 16 + (lane >> 4) * 4 +
-              r] = c;
-      }
+      for (int i = 0; i < C::FM; ++i)
+        red[(wave % C::WAVES_N) * C::BM + wm + i * 16 + lane] = sum[i];
+    }
     __syncthreads();
-    for (int c = threadIdx.x; c < C::BN; c += C::THREADS) {
+    for (int c = threadIdx.x; c < C::BM; c += C::THREADS) {
       float s = red[c];
-      for (int w = 1; w < C::WAVES_M; ++w) s += red[w * C::BN + c];
-      if (nmt > 1) {
-        dbp[mt * db_ld + n0 + c] = s;
-      } else if (n0 + c < p.vp) {
-        store_as(db, n0 + c, db_type, s);
+      for (int w = 1; w < C::WAVES_N; ++w) s += red[w * C::BM + c];
+      if (nrt > 1) {
+        dbp[rt * db_ld + m0 + c] = s;
+      } else if (m0 + c < p.vp) {
+        store_as(db, m0 + c, db_type, s);
       }
     }
   }
@@ -660,7 +664,7 @@ __global__ __launch_bounds__(256) void lce_db_kernel(
   store_as(db, v, type, s);
 }
 
-// dw[v, :] = 1/S sum_n G[n, v] x[n, :]  (G and x both k-strided)
+// dw[v, :] = 1/S sum_n G[n, v] x[n, :]  (x k-strided)
 template <class C, int PARTS, bool BF>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
     Operand G, Operand x, int kn, const float* __restrict__ sc,
@@ -670,7 +674,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
   const int bid = die_contiguous(blockIdx.x, nmt * nnt);
   const int m0 = bid / nnt * C::BM, n0 = bid % nnt * C::BN;
   f4 acc[C::FM][C::FN] = {};
-  product<C, KCOLS, KCOLS, PARTS, BF>(smem, G, m0, x, n0, 0, kn, acc);
+  product<C, KROWS, KCOLS, PARTS, BF>(smem, G, m0, x, n0, 0, kn, acc);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
@@ -709,6 +713,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
 }
 
 // part[slice][n, :] (+)= sum over a slice of the piece's words G[n, v] w[v, :]
+// (both k-strided)
 template <class C, int PARTS, bool BF>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dx_kernel(
     Operand G, Operand w, int kv, int kslice, float* __restrict__ part,
@@ -719,25 +724,32 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dx_kernel(
   const int m0 = t / nnt * C::BM, n0 = t % nnt * C::BN;
   const int k0 = sl * kslice;
   const int k1 = k0 + kslice < kv ? k0 + kslice : kv;
-  f4 acc[C::FM][C::FN] = {};
-  if (k0 < k1)
-    product<C, KROWS, KCOLS, PARTS, BF>(smem, G, m0, w, n0, k0, k1, acc);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
-#pragma unroll
-  for (int i = 0; i < C::FM; ++i) {
+  auto at = [&](int i, int j) -> f4* {
     const int m = m0 + wm + i * 16 + (lane & 15);
-    if (m >= n_rows) continue;
+    const int c = n0 + wn + j * 16 + (lane >> 4) * 4;
+    if (m >= n_rows || c >= dp) return nullptr;
+    return reinterpret_cast<f4*>(part + ((long)sl * n_rows + m) * dp + c);
+  };
+  // go on from the sums of the pieces before
+  f4 acc[C::FM][C::FN] = {};
+  if (!first) {
 #pragma unroll
-    for (int j = 0; j < C::FN; ++j) {
-      const int c = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (c >= dp) continue;
-      f4* at = reinterpret_cast<f4*>(part + ((long)sl * n_rows + m) * dp + c);
-      *at = first ? acc[i][j] : *at + acc[i][j];
-    }
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j)
+        if (const f4* p = at(i, j)) acc[i][j] = *p;
   }
+  if (k0 < k1)
+    product<C, KCOLS, KCOLS, PARTS, BF>(smem, G, m0, w, n0, k0, k1, acc);
+#pragma unroll
+  for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j)
+      if (f4* p = at(i, j)) *p = acc[i][j];
 }
 
 __global__ __launch_bounds__(256) void lce_dx_sum_kernel(
@@ -763,6 +775,7 @@ using Big = Tile<256, 256, 64, 64, 64, 2>;
 using Mid = Tile<128, 128, 64, 64, 64, 2>;
 // few rows: wide in the words
 using Flat = Tile<64, 256, 64, 32, 64, 2>;
+using FlatT = Tile<256, 64, 64, 32, 64, 2>;
 // few tiles: four stages deep, as a workgroup has a CU for itself
 using Small = Tile<64, 64, 32, 32, 64, 4>;
 
@@ -952,16 +965,17 @@ void with_types(const Plan& p, F f) {
 // in two workgroups a CU, so that one's exponentials and stores run under the
 // other's products, with x in blocks.
 using Logit = Tile<256, 128, 64, 64, 32, 3>;
+using LogitT = Tile<128, 256, 64, 64, 32, 3>;  // words by rows
 
 template <class C>
 constexpr int x_layout() {
-  return std::is_same<C, Logit>::value ? KBLOCK : KROWS;
+  return C::BK == 32 ? KBLOCK : KROWS;
 }
 
-// two-part operands never meet that tile: its registers do not hold them
+// two-part operands never meet those tiles
 template <class C, int PARTS>
 constexpr bool reached() {
-  return !(std::is_same<C, Logit>::value && PARTS == 2);
+  return C::BK == 64 || PARTS == 1;
 }
 
 bool blocked(const Plan& p) {
@@ -969,14 +983,15 @@ bool blocked(const Plan& p) {
   return p.parts == 1 && p.n > 64 && up(p.n, 256) * 100 <= up(p.n, 128) * 115;
 }
 
+// f(tile of the forward, tile of the backward)
 template <typename F>
 void with_row_tile(const Plan& p, F f) {
   if (p.n <= 64) {
-    f(Flat{});
+    f(Flat{}, FlatT{});
   } else if (blocked(p)) {
-    f(Logit{});
+    f(Logit{}, LogitT{});
   } else {
-    f(Mid{});
+    f(Mid{}, Mid{});
   }
 }
 
@@ -1007,7 +1022,7 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
   float* lse = saved.data_ptr<float>();
   float* tops = lse + p.n + 1;
 
-  with_row_tile(p, [&](auto tile) {
+  with_row_tile(p, [&](auto tile, auto) {
     using C = decltype(tile);
     const int nmt = (int)((p.n + C::BM - 1) / C::BM);
     const long piece_tiles = (std::min(piece, p.v) + C::BN - 1) / C::BN;
@@ -1137,7 +1152,7 @@ std::vector<at::Tensor> linear_ce_bwd(
   // offsets inside a piece of w stay below 2^31
   const long w_ld = p.w_direct ? w.stride(0) : p.dp * p.parts;
   piece = std::max(256L, std::min(piece, (1L << 30) / w_ld / 256 * 256));
-  const int ldg = (int)piece;
+  const int ldg = (int)p.np * p.parts;
   // dx: few tiles and a long k, so k is cut until the chip is full
   const int dx_tile = p.n > 128 && p.dp >= 128 ? 128 : 64;
   const long dx_tiles = ((p.n + dx_tile - 1) / dx_tile) *
@@ -1149,15 +1164,15 @@ std::vector<at::Tensor> linear_ce_bwd(
   if (want_dw) dw = at::empty({p.v, p.d}, w.options());
   if (want_db) db = at::empty({p.v}, bias->options());
 
-  with_row_tile(p, [&](auto row_tile) {
+  with_row_tile(p, [&](auto, auto row_tile) {
     using R = decltype(row_tile);
-    const int nmt = (int)((p.n + R::BM - 1) / R::BM);
-    // column sums of all pieces are joined at the end where they are small
-    const bool db_late = up(p.v, 256) * nmt <= (16L << 20);
-    const long db_ld = db_late ? up(p.v, 256) : ldg;
+    const int nrt = (int)((p.n + R::BN - 1) / R::BN);
+    // sums over the rows are joined at the end where they are small
+    const bool db_late = up(p.v, 256) * nrt <= (16L << 20);
+    const long db_ld = db_late ? up(p.v, 256) : piece;
 
     Scratch mem;
-    const auto o_rows = mem.take<Row>(p.np);
+    const auto o_rows = mem.take<float>(3 * p.np);
     const auto o_sc = mem.take<float>(2);
     const auto o_x = mem.take<ushort>(p.np * p.dp * p.parts);
     const auto o_xblk = mem.take<ushort>(blk ? p.np * p.dp : 0);
@@ -1166,10 +1181,10 @@ std::vector<at::Tensor> linear_ce_bwd(
     const auto o_w = mem.take<ushort>(p.w_direct ? 0
                                                  : piece * p.dp * p.parts);
     const auto o_winv = mem.take<float>(two ? piece : 0);
-    const auto o_G = mem.take<ushort>(p.np * ldg * p.parts);
+    const auto o_G = mem.take<ushort>(piece * ldg);
     const auto o_part =
         mem.take<float>(want_dx ? slices * p.n * p.dp : 0);
-    const auto o_dbp = mem.take<float>(want_db && nmt > 1 ? nmt * db_ld : 0);
+    const auto o_dbp = mem.take<float>(want_db && nrt > 1 ? nrt * db_ld : 0);
     mem.allocate(x);
 
     Pack kx = pack_of(x, 0, p.n, p.np, p, mem.at<ushort>(o_x));
@@ -1186,7 +1201,8 @@ std::vector<at::Tensor> linear_ce_bwd(
       kx.ntop = pack_blocks(p.np);
     }
     if (blk) kx.blocks = mem.at<ushort>(o_xblk);
-    kx.row = mem.at<Row>(o_rows);
+    float* row = mem.at<float>(o_rows);
+    kx.row = Rows{row, row + p.np, reinterpret_cast<int*>(row + 2 * p.np)};
     kx.dloss = dloss.data_ptr<float>();
     kx.each = reduction == 0;
     kx.count = reduction == 1 ? lse + p.n : nullptr;
@@ -1231,7 +1247,7 @@ std::vector<at::Tensor> linear_ce_bwd(
         constexpr int PARTS = decltype(parts)::value;
         constexpr bool BF = decltype(bf)::value;
         if constexpr (reached<R, PARTS>()) {
-          const int nvt = (int)((vp + R::BN - 1) / R::BN);
+          const int nvt = (int)((vp + R::BM - 1) / R::BM);
           float* dbp = mem.at<float>(o_dbp) + (db_late ? v0 : 0);
           void* db_at = want_db ? static_cast<char*>(db.data_ptr()) +
                                       v0 * db.element_size()
@@ -1239,9 +1255,9 @@ std::vector<at::Tensor> linear_ce_bwd(
           auto launch = [&](auto kernel) {
             constexpr int lds = R::template lds<PARTS>();
             allow_lds(kernel, lds);
-            kernel<<<nmt * nvt, R::THREADS, lds, stream>>>(
-                q, mem.at<Row>(o_rows), sc, p.v, v0, eps, G, ldg, dbp, db_ld,
-                db_at, want_db ? type_code(db) : 0, nmt, nvt);
+            kernel<<<nvt * nrt, R::THREADS, lds, stream>>>(
+                q, kx.row, sc, p.v, v0, eps, G, ldg, dbp, db_ld, db_at,
+                want_db ? type_code(db) : 0, nvt, nrt);
             HIP_CHECK_KERNEL();
           };
           if (want_db) {
@@ -1250,15 +1266,16 @@ std::vector<at::Tensor> linear_ce_bwd(
             launch(lce_grad_kernel<R, x_layout<R>(), PARTS, BF, false>);
           }
           const bool done = v0 + piece >= p.v;
-          if (want_db && nmt > 1 && (!db_late || done)) {
+          if (want_db && nrt > 1 && (!db_late || done)) {
             const long words = db_late ? p.v : vp;
             lce_db_kernel<<<(int)((words + 255) / 256), 256, 0, stream>>>(
-                mem.at<float>(o_dbp), nmt, db_ld, words,
+                mem.at<float>(o_dbp), nrt, db_ld, words,
                 db_late ? db.data_ptr() : db_at, type_code(db));
             HIP_CHECK_KERNEL();
           }
         }
-        const Operand g_rows = operand(G, p.np, (long)ldg * PARTS, ldg);
+        // as rows of words for dw, as columns of rows for dx
+        const Operand g = operand(G, up(vp, 64), ldg, p.np);
         if (want_dw) {
           auto run = [&](auto tile) {
             using C = decltype(tile);
@@ -1268,7 +1285,7 @@ std::vector<at::Tensor> linear_ce_bwd(
             constexpr int lds = C::template lds<1>();
             allow_lds(kernel, lds);
             kernel<<<mt * nt, C::THREADS, lds, stream>>>(
-                g_rows, xr, (int)up(p.n, 64), sc, xinv,
+                g, xr, (int)up(p.n, 64), sc, xinv,
                 static_cast<char*>(dw.data_ptr()) +
                     v0 * p.d * dw.element_size(),
                 p.type, (int)vp, (int)p.d, mt, nt);
@@ -1294,7 +1311,7 @@ std::vector<at::Tensor> linear_ce_bwd(
             constexpr int lds = C::template lds<1>();
             allow_lds(kernel, lds);
             kernel<<<mt * nt * slices, C::THREADS, lds, stream>>>(
-                g_rows, q.w, kv, kslice, mem.at<float>(o_part), (int)p.n,
+                g, q.w, kv, kslice, mem.at<float>(o_part), (int)p.n,
                 (int)p.dp, v0 == 0, mt, nt, slices);
             HIP_CHECK_KERNEL();
           };

@@ -393,18 +393,4 @@ __device__ __forceinline__ int die_contiguous(int bid, int n) {
   return (die < r ? die * (q + 1) : r * (q + 1) + (die - r) * q) + pos;
 }
 
-// sum over the 16 lanes that hold the rows of a fragment
-__device__ __forceinline__ float sum16(float v) {
-  const auto add = [&](int moved) { v += __builtin_bit_cast(float, moved); };
-  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF,
-                                  0xF, true));   // lanes 1 0 3 2
-  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF,
-                                  0xF, true));   // lanes 2 3 0 1
-  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF,
-                                  0xF, true));   // mirrored in 8
-  add(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF,
-                                  0xF, true));   // mirrored in 16
-  return v;
-}
-
 }  // namespace mm
