@@ -773,6 +773,10 @@ __global__ __launch_bounds__(256) void lce_dx_sum_kernel(
 // byte that comes from memory, and four waves on a SIMD to wait for another.
 using Big = Tile<256, 256, 64, 64, 64, 2>;
 using Mid = Tile<128, 128, 64, 64, 64, 2>;
+// two parts: eight waves, as they leave the LDS more time
+using MidParts = Tile<128, 128, 64, 32, 64, 2>;
+template <int PARTS>
+using MidOf = std::conditional_t<PARTS == 2, MidParts, Mid>;
 // few rows: wide in the words
 using Flat = Tile<64, 256, 64, 32, 64, 2>;
 using FlatT = Tile<256, 64, 64, 32, 64, 2>;
@@ -975,7 +979,8 @@ constexpr int x_layout() {
 // two-part operands never meet those tiles
 template <class C, int PARTS>
 constexpr bool reached() {
-  return C::BK == 64 || PARTS == 1;
+  return !std::is_same<C, std::conditional_t<PARTS == 2, Mid, MidParts>>::value
+         && (C::BK == 64 || PARTS == 1);
 }
 
 bool blocked(const Plan& p) {
@@ -990,6 +995,8 @@ void with_row_tile(const Plan& p, F f) {
     f(Flat{}, FlatT{});
   } else if (blocked(p)) {
     f(Logit{}, LogitT{});
+  } else if (p.parts == 2) {
+    f(MidParts{}, MidParts{});
   } else {
     f(Mid{}, Mid{});
   }
@@ -1295,7 +1302,7 @@ std::vector<at::Tensor> linear_ce_bwd(
           if (cover >= 192 && p.dp % 256 == 0) {
             run(Big{});
           } else if (cover >= 48 && p.dp >= 128) {
-            run(Mid{});
+            run(MidOf<PARTS>{});
           } else {
             run(Small{});
           }

@@ -95,12 +95,14 @@ struct Tile {
 
 template <int BK>
 __device__ __forceinline__ int row_swizzle(int r) {
-  return BK == 32 ? ((-(r >> 2)) & 3) : (r & 7);
+  return BK == 32 ? ((-(r >> 2)) & 3) : BK == 64 ? (r & 7) : (r & 15);
 }
 
 template <int R>
 __device__ __forceinline__ int col_swizzle(int k) {
-  if constexpr (R == 64) {
+  if constexpr (R == 32) {
+    return (k >> 3) & 1;
+  } else if constexpr (R == 64) {
     return ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
   } else {
     return (k & 3) | (((k >> 3) & 1) << 2);
@@ -113,7 +115,7 @@ struct Stager {
   static constexpr int PER = R * BK * 2 / 16 / THREADS;
   static_assert(PER >= 1 && PER * THREADS * 16 == R * BK * 2,
                 "a stage has to be whole 16-byte pieces for every thread");
-  static_assert(PARTS == 1 || BK == 64, "pairs of 32");
+  static_assert(PARTS == 1 || BK >= 64, "pairs of 32");
   __amdgpu_buffer_rsrc_t rs;
   int off[PER];    // KROWS: byte offset; KCOLS: column byte offset
   int ld2;
@@ -166,7 +168,7 @@ struct Stager {
         v = off[i] + k0 * 2 * PARTS;
       } else {
         int k = (threadIdx.x + i * THREADS) / (R / 8);
-        k = (PARTS == 2 ? k & 31 : k) + k0;
+        k = (PARTS == 2 ? (k >> 6) * 32 + (k & 31) : k) + k0;
         if (k > rows - 1) k = rows - 1;
         v = off[i] + k * ld2;
       }
@@ -218,13 +220,13 @@ __device__ __forceinline__ void barrier() {
 
 // acc[i][j] of wave (wm, wn): element (m, n) with
 //   m = m0 + wm + i*16 + (lane & 15), n = n0 + wn + j*16 + (lane>>4)*4 + r.
-// k runs over [k0, k1), both multiples of BK, of 32 in pairs.
+// k runs over [k0, k1), both multiples of BK, of BK / 2 in pairs.
 template <class C, int AL, int BL, int PARTS, bool BF>
 __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
                                         const Operand& b, int n0, int k0,
                                         int k1, f4 (&acc)[C::FM][C::FN]) {
   constexpr int BK = C::BK, ST = C::ST, T = C::THREADS;
-  constexpr int STEP = PARTS == 2 ? 32 : BK;
+  constexpr int STEP = BK / PARTS;
   Stager<C::BM, AL, BK, T, PARTS> sa;
   Stager<C::BN, BL, BK, T, PARTS> sb;
   sa.init(a, m0);
@@ -278,14 +280,17 @@ __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
         f[j] = frag<C::BN, BL, BK>(pb, wn + j * 16, kk, lane);
     };
     if constexpr (PARTS == 2) {
-      s8 ah[C::FM], al[C::FM], bh[C::FN], bl[C::FN];
-      read_b(bh, 0);
-      read_a(al, 1);
-      multiply(al, bh);
-      read_a(ah, 0);
-      multiply(ah, bh);
-      read_b(bl, 1);
-      multiply(ah, bl);
+#pragma unroll
+      for (int kk = 0; kk < BK / 32; kk += 2) {
+        s8 ah[C::FM], al[C::FM], bh[C::FN], bl[C::FN];
+        read_b(bh, kk);
+        read_a(al, kk + 1);
+        multiply(al, bh);
+        read_a(ah, kk);
+        multiply(ah, bh);
+        read_b(bl, kk + 1);
+        multiply(ah, bl);
+      }
     } else {
 #pragma unroll
       for (int kk = 0; kk < BK / 32; ++kk) {

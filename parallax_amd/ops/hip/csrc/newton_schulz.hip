@@ -137,19 +137,19 @@ __global__ __launch_bounds__(256) void ns_start_kernel(
     const void* __restrict__ g, int type, Shape shape,
     const double* __restrict__ part, int blocks, double eps, Matrix X) {
   __shared__ float tile[64][65];
-  __shared__ double red[256];
+  __shared__ double red[4];
   const bool flip = shape.tall(blockIdx.z);
   const int rows = flip ? shape.large : shape.small;
   const int cols = flip ? shape.small : shape.large;
-  red[threadIdx.x] = threadIdx.x < blocks
-                         ? part[(long)blockIdx.z * blocks + threadIdx.x]
-                         : 0.;
+  double sum = threadIdx.x < blocks
+                   ? part[(long)blockIdx.z * blocks + threadIdx.x]
+                   : 0.;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
   __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-    __syncthreads();
-  }
-  const double scale = kScale / (sqrt(red[0]) + eps);
+  const double scale =
+      kScale / (sqrt(red[0] + red[1] + red[2] + red[3]) + eps);
   X = X.of(blockIdx.z);
   const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
   const int r0 = flip ? n0 : m0, c0 = flip ? m0 : n0;
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
         for (int j = 0; j < C::FN; ++j)
           acc[i][j] += sums[q * SIZE + (i * C::FN + j) * C::THREADS];
   } else {
-    const int each = CUT == 1 ? (kp / 64 + cuts - 1) / cuts * 64 : kp;
+    const int each = CUT == 1 ? (kp / 128 + cuts - 1) / cuts * 128 : kp;
     const int k0 = cut * each, k1 = k0 + each < kp ? k0 + each : kp;
     if (k0 < k1) {
       const Operand o = P.operand();
@@ -391,11 +391,15 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_next_kernel(
   }
 }
 
-using Big = Tile<256, 256, 64, 64, 64, 2>;
-using Mid = Tile<128, 128, 64, 64, 64, 2>;
-// few tiles: four stages deep, as a workgroup has a CU for itself
-using Deep = Tile<128, 128, 64, 64, 64, 4>;
-using Small = Tile<64, 64, 32, 32, 64, 4>;
+// Eight waves of 64 x 32, two workgroups on a CU.  2048 x 8192 x 1024 in two
+// parts: 1.28 PF of 16-bit products (four waves of 64 x 64: 1.18, a
+// 256 x 256 tile of sixteen: 1.25).
+using Mid = Tile<128, 128, 64, 32, 64, 2>;
+// Few tiles: what counts is the time of one, so many waves, 128 k a stage
+// and smaller tiles.  512 x 512 x 512 in two parts, launch included: 12 us
+// with Mid, 6.4 with Small, 4.7 with Tiny.
+using Small = Tile<64, 64, 32, 16, 128, 2>;
+using Tiny = Tile<32, 32, 16, 16, 128, 4>;
 
 template <typename K>
 void allow_lds(K kernel, int bytes) {
@@ -415,17 +419,15 @@ void allow_lds(K kernel, int bytes) {
   done.insert(key);
 }
 
-// f(tile) for a tile size of 64, 128 or 256, and so many workgroups
+// f(tile) for a tile size of 32, 64 or 128
 template <typename F>
-void with_tile(int size, long groups, F f) {
-  if (size == 256) {
-    f(Big{});
-  } else if (size == 128 && groups > 256) {
+void with_tile(int size, F f) {
+  if (size == 128) {
     f(Mid{});
-  } else if (size == 128) {
-    f(Deep{});
-  } else {
+  } else if (size == 64) {
     f(Small{});
+  } else {
+    f(Tiny{});
   }
 }
 
@@ -471,8 +473,9 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
   const bool every = exact || small < 256;
   auto fine = [&](int64_t i) { return every || i >= steps - 3; };
 
-  // The largest tile that still gives the chip's 256 CUs something to do;
-  // the symmetric products may cut k as well.
+  // The largest tile that still gives half of the chip's 256 CUs something
+  // to do (a symmetric product of 128 x 128 tiles all of them: 12 x 512 x
+  // 2048 takes XX us with 120 of those and XX with 432 smaller ones).
   auto full_tiles = [&](long t) {
     return (small + t - 1) / t * ((large + t - 1) / t) * batch;
   };
@@ -480,18 +483,17 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
     const long n = (small + t - 1) / t;
     return n * (n + 1) / 2 * batch;
   };
-  const int full = full_tiles(256) >= 200 ? 256
-                   : full_tiles(128) >= 128 ? 128 : 64;
-  const int sym = sym_tiles(256) >= 200 ? 256
-                  : sym_tiles(128) >= 30 ? 128 : 64;
+  const int full = full_tiles(128) >= 128 ? 128
+                   : full_tiles(64) >= 128 ? 64 : 32;
+  const int sym = sym_tiles(128) >= 256 ? 128
+                  : sym_tiles(64) >= 100 ? 64 : 32;
+  // and a long k of few tiles is cut
   auto cuts_of = [&](long k) {
-    const long slots = sym == 256 ? 256 : 512;
-    return (int)std::max(1L, std::min({slots / sym_tiles(sym), k / 512,
-                                       8L}));
+    return (int)std::max(1L, std::min({512 / sym_tiles(sym), k / 1024, 8L}));
   };
-  const int tile = std::max(full, sym);
-  const int mp = (int)up(small, tile), np = (int)up(large, tile);
-  const int km = (int)up(small, 64), kn = (int)up(large, 64);
+  // zeros up to whole tiles, and whole stages of 128 k
+  const int mp = (int)up(small, 128), np = (int)up(large, 128);
+  const int km = mp, kn = np;
   const long pairs = (long)(mp / sym) * (mp / sym + 1) / 2;
   const int cuts = std::max(cuts_of(kn), cuts_of(km));
   // ~16 values a thread
@@ -536,8 +538,7 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
                          const Matrix& o) {
       constexpr bool SECOND = decltype(second)::value;
       const int tiles = mp / sym, cut = cuts_of(k);
-      const long groups = pairs * batch * cut;
-      with_tile(sym, groups, [&](auto t) {
+      with_tile(sym, [&](auto t) {
         using C = decltype(t);
         auto launch = [&](auto kernel, int lds, int n) {
           allow_lds(kernel, lds);
@@ -561,7 +562,7 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
     };
     symmetric(std::false_type{}, X, kn, A);
     symmetric(std::true_type{}, A, km, B);
-    with_tile(full, full_tiles(full), [&](auto t) {
+    with_tile(full, [&](auto t) {
       using C = decltype(t);
       auto launch = [&](auto kernel) {
         constexpr int lds = C::template lds<2>();
