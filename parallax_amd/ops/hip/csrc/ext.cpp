@@ -174,8 +174,10 @@ std::vector<at::Tensor> linear_ce_bwd(
 
 // newton_schulz.hip
 void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
-                   double a, double b, double c, double eps, bool exact,
-                   int64_t turned);
+                   double a, double b, double c, double eps, bool exact);
+void newton_schulz_list(std::vector<at::Tensor> mats, int64_t steps,
+                        double a, double b, double c, double eps,
+                        bool exact);
 
 // rotary.hip
 std::vector<at::Tensor> rotary(const at::Tensor& q,
@@ -282,6 +284,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_ce_bwd", &linear_ce_bwd);
   m.def("newton_schulz", &newton_schulz,
         "Newton-Schulz orthogonalisation of a batch of matrices");
+  m.def("newton_schulz_list", &newton_schulz_list,
+        "the same for a list of matrices of one padded size, in place");
   m.def("multi_tensor_muon_update", &multi_tensor_muon_update);
   m.def("multi_tensor_muon_apply", &multi_tensor_muon_apply);
   m.def("rotary", &rotary, "rotary positions of queries and keys");

@@ -58,27 +58,76 @@ __device__ __forceinline__ void store_as(void* p, long i, int type, float v) {
   }
 }
 
+// The matrices of a batch, as they lie: of one shape behind one another, or
+// (`listed`) each with its own place and shape.  All fit the same padded
+// size, as zeros behind a matrix stay zeros.
+constexpr int kListed = 48;
+
+struct Given {
+  const void* in;
+  void* out;
+  int rows, cols;
+};
+
+struct Batch {
+  const void* in;
+  void* out;
+  long stride;       // in elements
+  int size;          // of an element in bytes
+  int rows, cols;
+  bool listed;
+  Given list[kListed];
+
+  __device__ __forceinline__ Given of(int b) const {
+    if (listed) return list[b];
+    return Given{static_cast<const char*>(in) + b * stride * size,
+                 static_cast<char*>(out) + b * stride * size, rows, cols};
+  }
+};
+
+// Four values from the 4 i-th of `p`, which lies at 16 bytes.
+__device__ __forceinline__ f4 load_four(const void* p, long i, int type) {
+  if (type == 2) return static_cast<const f4*>(p)[i];
+  const ushort4 u = static_cast<const ushort4*>(p)[i];
+  const ushort e[4] = {u.x, u.y, u.z, u.w};
+  f4 v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    v[r] = type == 1 ? half_bits(e[r]) : __uint_as_float((unsigned)e[r] << 16);
+  return v;
+}
+
 // Sums of squares in 64 bits (an fp32 square of 1e-20 or 1e20 is lost), one
 // partial per block.
 __global__ __launch_bounds__(256) void ns_norm_kernel(
-    const void* __restrict__ g, int type, long count,
-    double* __restrict__ part, int blocks) {
-  __shared__ double red[256];
-  const long base = (long)blockIdx.y * count;
+    Batch batch, int type, double* __restrict__ part) {
+  __shared__ double red[4];
+  const Given g = batch.of(blockIdx.y);
+  const long count = (long)g.rows * g.cols;
+  const long step = (long)gridDim.x * 256;
+  long i = (long)blockIdx.x * 256 + threadIdx.x;
   double s = 0.;
-#pragma unroll 4
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count;
-       i += (long)gridDim.x * 256) {
-    const double v = load_as(g, base + i, type);
+  if (reinterpret_cast<uintptr_t>(g.in) % 16 == 0) {
+    // four at a time, then what is left
+#pragma unroll 2
+    for (; i < count / 4; i += step) {
+      const f4 v = load_four(g.in, i, type);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s += (double)v[r] * v[r];
+    }
+    i = count / 4 * 4 + (long)blockIdx.x * 256 + threadIdx.x;
+  }
+  for (; i < count; i += step) {
+    const double v = load_as(g.in, i, type);
     s += v * v;
   }
-  red[threadIdx.x] = s;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) part[(long)blockIdx.y * blocks + blockIdx.x] = red[0];
+  if (threadIdx.x == 0)
+    part[(long)blockIdx.y * gridDim.x + blockIdx.x] =
+        red[0] + red[1] + red[2] + red[3];
 }
 
 // How X, A and B lie between the products: in pairs of parts for products of
@@ -123,53 +172,61 @@ struct Matrix {
   }
 };
 
-// The matrices of a batch are small x large, from `first_tall` on large x
-// small as they lie.
-struct Shape {
-  int small, large, first_tall;
-  __device__ __forceinline__ bool tall(int batch) const {
-    return batch >= first_tall;
-  }
-};
-
 // X0 in 64 x 64 tiles, transposed where the matrix is tall, zeros behind it.
 __global__ __launch_bounds__(256) void ns_start_kernel(
-    const void* __restrict__ g, int type, Shape shape,
-    const double* __restrict__ part, int blocks, double eps, Matrix X) {
+    Batch batch, int type, const double* __restrict__ part, int blocks,
+    double eps, Matrix X) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
-  const bool flip = shape.tall(blockIdx.z);
-  const int rows = flip ? shape.large : shape.small;
-  const int cols = flip ? shape.small : shape.large;
-  double sum = threadIdx.x < blocks
-                   ? part[(long)blockIdx.z * blocks + threadIdx.x]
-                   : 0.;
+  const Given g = batch.of(blockIdx.z);
+  const bool flip = g.rows > g.cols;
+  double sum = 0.;
+  for (int i = threadIdx.x; i < blocks; i += 256)
+    sum += part[(long)blockIdx.z * blocks + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  const double scale =
-      kScale / (sqrt(red[0] + red[1] + red[2] + red[3]) + eps);
   X = X.of(blockIdx.z);
   const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
   const int r0 = flip ? n0 : m0, c0 = flip ? m0 : n0;
-  const long base = (long)blockIdx.z * rows * cols;
-  for (int i = threadIdx.x; i < 4096; i += 256) {
-    const int r = r0 + (i >> 6), c = c0 + (i & 63);
-    float v = 0.f;
-    if (r < rows && c < cols)
-      v = (float)(load_as(g, base + (long)r * cols + c, type) * scale);
-    tile[i >> 6][i & 63] = v;
+  if (g.cols % 4 == 0 && reinterpret_cast<uintptr_t>(g.in) % 16 == 0) {
+#pragma unroll
+    for (int i = threadIdx.x; i < 1024; i += 256) {
+      const int r = r0 + (i >> 4), c = c0 + (i & 15) * 4;
+      const f4 v = r < g.rows && c < g.cols
+                       ? load_four(g.in, ((long)r * g.cols + c) / 4, type)
+                       : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tile[i >> 4][(i & 15) * 4 + e] = v[e];
+    }
+  } else {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < 4096; i += 256) {
+      const int r = r0 + (i >> 6), c = c0 + (i & 63);
+      tile[i >> 6][i & 63] =
+          r < g.rows && c < g.cols
+              ? load_as(g.in, (long)r * g.cols + c, type) : 0.f;
+    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 4096; i += 256) {
-    const int r = i >> 6, c = i & 63;
-    const float v = flip ? tile[c][r] : tile[r][c];
-    ushort h, l;
-    split(v, h, l);
-    const long at = X.at(m0 + r, n0 + c);
-    X.p[at] = h;
-    X.p[at + (X.pairs ? 32L : (long)X.rows * X.cols)] = l;
+  const double scale =
+      kScale / (sqrt(red[0] + red[1] + red[2] + red[3]) + eps);
+#pragma unroll
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const int r = i >> 3, c = (i & 7) * 8;
+    s8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      ushort hi, lo;
+      split((float)((flip ? tile[c + e][r] : tile[r][c + e]) * scale), hi,
+            lo);
+      h[e] = hi;
+      l[e] = lo;
+    }
+    ushort* at = X.p + X.at(m0 + r, n0 + c);
+    *reinterpret_cast<s8*>(at) = h;
+    *reinterpret_cast<s8*>(
+        at + (X.pairs ? 32L : (long)X.rows * X.cols)) = l;
   }
 }
 
@@ -317,35 +374,35 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
   }
 }
 
-// X' = a X + B X; the last one goes to the result.
+// X' = a X + B X; the last one goes to the result.  The sums start from
+// a X, so that it is read while the first stages are on their way.
 template <class C, int PARTS>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_next_kernel(
-    Matrix B, int kp, Matrix X, float a, Matrix out, void* __restrict__ last,
-    int type, Shape shape, int nnt) {
+    Matrix B, int kp, Matrix X, float a, Matrix out, bool last, Batch batch,
+    int type, int nnt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const bool flip = shape.tall(blockIdx.y);
-  const int rows = flip ? shape.large : shape.small;
-  const int cols = flip ? shape.small : shape.large;
   const int bid = die_contiguous(blockIdx.x, gridDim.x);
   const int m0 = bid / nnt * C::BM, n0 = bid % nnt * C::BN;
-  B = B.of(blockIdx.y);
-  X = X.of(blockIdx.y);
-  f4 acc[C::FM][C::FN] = {};
-  product<C, KROWS, KCOLS, PARTS, false>(smem, B.operand(), m0, X.operand(),
-                                         n0, 0, kp, acc);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
+  B = B.of(blockIdx.y);
+  X = X.of(blockIdx.y);
+  f4 acc[C::FM][C::FN];
 #pragma unroll
   for (int i = 0; i < C::FM; ++i)
 #pragma unroll
     for (int j = 0; j < C::FN; ++j)
-      acc[i][j] = a * X.four<true>(m0 + wm + i * 16 + (lane & 15),
-                                   n0 + wn + j * 16 + (lane >> 4) * 4) +
-                  acc[i][j] * (1.f / kScale);
-  const auto value = [&](int i, int j) { return acc[i][j]; };
-  if (last == nullptr) {
+      acc[i][j] = a * kScale *
+                  X.four<true>(m0 + wm + i * 16 + (lane & 15),
+                               n0 + wn + j * 16 + (lane >> 4) * 4);
+  product<C, KROWS, KCOLS, PARTS, false>(smem, B.operand(), m0, X.operand(),
+                                         n0, 0, kp, acc);
+  if (!last) {
+    const auto value = [&](int i, int j) {
+      return acc[i][j] * (1.f / kScale);
+    };
     out = out.of(blockIdx.y);
     if (out.pairs) {
       put_tile<C, 2, true>(smem, out, m0, n0, value);
@@ -354,38 +411,41 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_next_kernel(
     }
     return;
   }
-  const long base = (long)blockIdx.y * rows * cols;
-  if (type != 2 && !flip && cols % 8 == 0) {
-    store_tile<C>(smem, static_cast<ushort*>(last) + base + (long)m0 * cols +
-                            n0,
-                  cols, rows - m0, cols - n0, [&](int i, int j) {
+  const float back = 1.f / (kScale * kScale);
+  const Given g = batch.of(blockIdx.y);
+  const bool flip = g.rows > g.cols;
+  if (type != 2 && !flip && g.cols % 8 == 0 &&
+      reinterpret_cast<uintptr_t>(g.out) % 16 == 0) {
+    store_tile<C>(smem,
+                  static_cast<ushort*>(g.out) + (long)m0 * g.cols + n0,
+                  g.cols, g.rows - m0, g.cols - n0, [&](int i, int j) {
       ushort u[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        store_as(u, r, type, acc[i][j][r] * (1.f / kScale));
+      for (int r = 0; r < 4; ++r) store_as(u, r, type, acc[i][j][r] * back);
       return make_ushort4(u[0], u[1], u[2], u[3]);
     });
     return;
   }
+  const bool four = type == 2 && !flip && g.cols % 4 == 0 &&
+                    reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
     const int m = m0 + wm + i * 16 + (lane & 15);
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) {
       const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (type == 2 && !flip && cols % 4 == 0) {
-        if (m < rows && n < cols)
-          *reinterpret_cast<f4*>(static_cast<float*>(last) + base +
-                                 (long)m * cols + n) =
-              acc[i][j] * (1.f / kScale);
+      if (four) {
+        if (m < g.rows && n < g.cols)
+          *reinterpret_cast<f4*>(static_cast<float*>(g.out) +
+                                 (long)m * g.cols + n) = acc[i][j] * back;
         continue;
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = flip ? n + r : m, col = flip ? m : n + r;
-        if (row < rows && col < cols)
-          store_as(last, base + (long)row * cols + col, type,
-                   acc[i][j][r] * (1.f / kScale));
+        if (row < g.rows && col < g.cols)
+          store_as(g.out, (long)row * g.cols + col, type,
+                   acc[i][j][r] * back);
       }
     }
   }
@@ -431,57 +491,52 @@ void with_tile(int size, F f) {
   }
 }
 
-}  // namespace
-
-// g [batch, rows, cols] -> out of the same shape and type, which may be g.
-// The matrices from `turned` on lie as [cols, rows].
-// exact: two-part operands in every product, whatever the size.
-void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
-                   double a, double b, double c, double eps, bool exact,
-                   int64_t turned) {
-  TORCH_CHECK(g.is_cuda() && g.dim() == 3 && g.is_contiguous(),
-              "newton_schulz: contiguous [batch, rows, cols] on the GPU "
-              "expected");
-  TORCH_CHECK(out.is_contiguous() && out.sizes() == g.sizes() &&
-                  out.scalar_type() == g.scalar_type() &&
-                  out.device() == g.device(),
-              "newton_schulz: out has to be like g");
-  int type = 0;
-  switch (g.scalar_type()) {
-    case at::kBFloat16: type = 0; break;
-    case at::kHalf: type = 1; break;
-    case at::kFloat: type = 2; break;
+int type_code(at::ScalarType t) {
+  switch (t) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
     default:
       TORCH_CHECK(false, "newton_schulz: bf16, fp16 or fp32 expected, got ",
-                  g.scalar_type());
+                  t);
   }
-  const long batch = g.size(0), rows = g.size(1), cols = g.size(2);
-  TORCH_CHECK(turned >= 0 && turned <= batch &&
-                  (turned == batch || rows <= cols),
-              "newton_schulz: wide matrices first");
-  TORCH_CHECK(steps >= 1 && steps <= 64, "newton_schulz: 1 to 64 steps");
-  TORCH_CHECK(batch <= 65535, "newton_schulz: at most 65535 matrices");
+}
+
+void check_size(long rows, long cols) {
   TORCH_CHECK(rows <= 32768 && cols <= 32768 && rows * cols <= (1L << 28),
               "newton_schulz: matrices of up to 32768 rows and columns and "
               "2^28 values");
-  if (g.numel() == 0) return;
-  const c10::cuda::CUDAGuard guard(g.device());
+}
+
+struct Polynomial {
+  int64_t steps;
+  double a, b, c, eps;
+  bool exact;  // two-part operands in every product, whatever the size
+};
+
+// How many matrices go through the products together: 2^28 values, whose
+// working copies take up to 4 GB, are far more than fill the chip.  (At most
+// 16384: fewer than a grid's third dimension holds.)
+long at_once(long small, long large) {
+  return std::max(1L, (1L << 28) / (up(small, 128) * up(large, 128)));
+}
+
+// small x large: the largest of the batch's matrices, which has `count`;
+// least: the fewest rows (or columns of a tall one) of them
+void run(const Batch& batch, int type, long count, long small, long large,
+         long least, const Polynomial& p, const at::TensorOptions& options) {
   auto stream = at::cuda::getCurrentCUDAStream();
-  const long small = std::min(rows, cols), large = std::max(rows, cols);
-  const Shape shape{(int)small, (int)large,
-                    rows > cols ? 0 : (int)turned};
-  const bool every = exact || small < 256;
-  auto fine = [&](int64_t i) { return every || i >= steps - 3; };
+  const bool every = p.exact || least < 256;
+  auto fine = [&](int64_t i) { return every || i >= p.steps - 3; };
 
   // The largest tile that still gives half of the chip's 256 CUs something
-  // to do (a symmetric product of 128 x 128 tiles all of them: 12 x 512 x
-  // 2048 takes XX us with 120 of those and XX with 432 smaller ones).
+  // to do, for a symmetric product of 128 x 128 tiles all of them.
   auto full_tiles = [&](long t) {
-    return (small + t - 1) / t * ((large + t - 1) / t) * batch;
+    return (small + t - 1) / t * ((large + t - 1) / t) * count;
   };
   auto sym_tiles = [&](long t) {
     const long n = (small + t - 1) / t;
-    return n * (n + 1) / 2 * batch;
+    return n * (n + 1) / 2 * count;
   };
   const int full = full_tiles(128) >= 128 ? 128
                    : full_tiles(64) >= 128 ? 64 : 32;
@@ -493,11 +548,9 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
   };
   // zeros up to whole tiles, and whole stages of 128 k
   const int mp = (int)up(small, 128), np = (int)up(large, 128);
-  const int km = mp, kn = np;
   const long pairs = (long)(mp / sym) * (mp / sym + 1) / 2;
-  const int cuts = std::max(cuts_of(kn), cuts_of(km));
-  // ~16 values a thread
-  const int blocks = (int)std::min<long>(256, (rows * cols + 4095) / 4096);
+  const int cuts = std::max(cuts_of(np), cuts_of(mp));
+  const int blocks = (int)std::min<long>(1024, (small * large + 4095) / 4096);
 
   // one allocation: two X, A, B, the norm's partial sums, the cut sums
   const long xs = 2L * mp * np, as = 2L * mp * mp;
@@ -507,12 +560,12 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
     bytes += (n + 255) / 256 * 256;
     return at;
   };
-  const size_t o_x0 = take(batch * xs * 2), o_x1 = take(batch * xs * 2);
-  const size_t o_a = take(batch * as * 2), o_b = take(batch * as * 2);
-  const size_t o_norm = take(batch * blocks * sizeof(double));
+  const size_t o_x0 = take(count * xs * 2), o_x1 = take(count * xs * 2);
+  const size_t o_a = take(count * as * 2), o_b = take(count * as * 2);
+  const size_t o_norm = take(count * blocks * sizeof(double));
   const size_t o_part =
-      take(cuts > 1 ? batch * pairs * cuts * sym * sym * 4 : 0);
-  auto mem = at::empty({(long)bytes}, g.options().dtype(at::kByte));
+      take(cuts > 1 ? count * pairs * cuts * sym * sym * 4 : 0);
+  auto mem = at::empty({(long)bytes}, options.dtype(at::kByte));
   char* base = static_cast<char*>(mem.data_ptr());
   auto matrix = [&](size_t at, long stride, int r, int c, bool in_pairs) {
     return Matrix{reinterpret_cast<ushort*>(base + at), stride, r, c,
@@ -521,15 +574,13 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
   double* norm = reinterpret_cast<double*>(base + o_norm);
   float* part = reinterpret_cast<float*>(base + o_part);
 
-  ns_norm_kernel<<<dim3(blocks, batch), 256, 0, stream>>>(
-      g.data_ptr(), type, rows * cols, norm, blocks);
+  ns_norm_kernel<<<dim3(blocks, count), 256, 0, stream>>>(batch, type, norm);
   HIP_CHECK_KERNEL();
-  ns_start_kernel<<<dim3(np / 64, mp / 64, batch), 256, 0, stream>>>(
-      g.data_ptr(), type, shape, norm, blocks, eps,
-      matrix(o_x0, xs, mp, np, fine(0)));
+  ns_start_kernel<<<dim3(np / 64, mp / 64, count), 256, 0, stream>>>(
+      batch, type, norm, blocks, p.eps, matrix(o_x0, xs, mp, np, fine(0)));
   HIP_CHECK_KERNEL();
-  for (int64_t i = 0; i < steps; ++i) {
-    const bool f = fine(i);
+  for (int64_t i = 0; i < p.steps; ++i) {
+    const bool f = fine(i), last = i + 1 == p.steps;
     const Matrix X = matrix(i % 2 ? o_x1 : o_x0, xs, mp, np, f);
     const Matrix Y = matrix(i % 2 ? o_x0 : o_x1, xs, mp, np, fine(i + 1));
     const Matrix A = matrix(o_a, as, mp, mp, f);
@@ -542,8 +593,8 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
         using C = decltype(t);
         auto launch = [&](auto kernel, int lds, int n) {
           allow_lds(kernel, lds);
-          kernel<<<dim3(pairs * n, batch), C::THREADS, lds, stream>>>(
-              P, k, (float)b, (float)c, o, tiles, cut, part);
+          kernel<<<dim3(pairs * n, count), C::THREADS, lds, stream>>>(
+              P, k, (float)p.b, (float)p.c, o, tiles, cut, part);
           HIP_CHECK_KERNEL();
         };
         constexpr int one = C::template lds<1>(), two = C::template lds<2>();
@@ -560,17 +611,16 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
         }
       });
     };
-    symmetric(std::false_type{}, X, kn, A);
-    symmetric(std::true_type{}, A, km, B);
+    symmetric(std::false_type{}, X, np, A);
+    symmetric(std::true_type{}, A, mp, B);
     with_tile(full, [&](auto t) {
       using C = decltype(t);
       auto launch = [&](auto kernel) {
         constexpr int lds = C::template lds<2>();
         allow_lds(kernel, lds);
         const int nnt = np / C::BN;
-        kernel<<<dim3(mp / C::BM * nnt, batch), C::THREADS, lds, stream>>>(
-            B, km, X, (float)a, Y,
-            i + 1 == steps ? out.data_ptr() : nullptr, type, shape, nnt);
+        kernel<<<dim3(mp / C::BM * nnt, count), C::THREADS, lds, stream>>>(
+            B, mp, X, (float)p.a, Y, last, batch, type, nnt);
         HIP_CHECK_KERNEL();
       };
       if (f) {
@@ -579,5 +629,84 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
         launch(ns_next_kernel<C, 1>);
       }
     });
+  }
+}
+
+}  // namespace
+
+// g [batch, rows, cols] -> out of the same shape and type, which may be g.
+void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
+                   double a, double b, double c, double eps, bool exact) {
+  TORCH_CHECK(g.is_cuda() && g.dim() == 3 && g.is_contiguous(),
+              "newton_schulz: contiguous [batch, rows, cols] on the GPU "
+              "expected");
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == g.sizes() &&
+                  out.scalar_type() == g.scalar_type() &&
+                  out.device() == g.device(),
+              "newton_schulz: out has to be like g");
+  const long rows = g.size(1), cols = g.size(2);
+  TORCH_CHECK(steps >= 1 && steps <= 64, "newton_schulz: 1 to 64 steps");
+  check_size(rows, cols);
+  const int type = type_code(g.scalar_type());
+  if (g.numel() == 0) return;
+  const c10::cuda::CUDAGuard guard(g.device());
+  const long small = std::min(rows, cols), large = std::max(rows, cols);
+  const long most = at_once(small, large);
+  for (long i = 0; i < g.size(0); i += most) {
+    Batch batch = {};
+    const long offset = i * rows * cols * g.element_size();
+    batch.in = static_cast<const char*>(g.data_ptr()) + offset;
+    batch.out = static_cast<char*>(out.data_ptr()) + offset;
+    batch.stride = rows * cols;
+    batch.size = (int)g.element_size();
+    batch.rows = (int)rows;
+    batch.cols = (int)cols;
+    run(batch, type, std::min(most, g.size(0) - i), small, large, small,
+        Polynomial{steps, a, b, c, eps, exact}, g.options());
+  }
+}
+
+// Each matrix of a list in place.  They are of one type and device and fill
+// up to the same multiples of 128 rows and columns (of 128 columns and rows
+// the other way round).
+void newton_schulz_list(std::vector<at::Tensor> mats, int64_t steps,
+                        double a, double b, double c, double eps,
+                        bool exact) {
+  TORCH_CHECK(steps >= 1 && steps <= 64, "newton_schulz: 1 to 64 steps");
+  if (mats.empty()) return;
+  const at::Tensor& first = mats[0];
+  const int type = type_code(first.scalar_type());
+  TORCH_CHECK(first.is_cuda() && first.dim() == 2,
+              "newton_schulz: matrices on the GPU expected");
+  const c10::cuda::CUDAGuard guard(first.device());
+  const size_t most = std::min<long>(
+      kListed, at_once(std::min(first.size(0), first.size(1)),
+                       std::max(first.size(0), first.size(1))));
+  for (size_t i0 = 0; i0 < mats.size(); i0 += most) {
+    const size_t n = std::min(most, mats.size() - i0);
+    Batch batch = {};
+    batch.listed = true;
+    long small = 0, large = 0, least = 1L << 30;
+    for (size_t i = 0; i < n; ++i) {
+      const at::Tensor& m = mats[i0 + i];
+      TORCH_CHECK(m.dim() == 2 && m.is_contiguous() && m.numel() > 0 &&
+                      m.scalar_type() == first.scalar_type() &&
+                      m.device() == first.device(),
+                  "newton_schulz: contiguous matrices of one type and device "
+                  "expected");
+      check_size(m.size(0), m.size(1));
+      const long s = std::min(m.size(0), m.size(1));
+      const long l = std::max(m.size(0), m.size(1));
+      TORCH_CHECK(i == 0 || (up(s, 128) == up(small, 128) &&
+                             up(l, 128) == up(large, 128)),
+                  "newton_schulz: matrices of different padded sizes");
+      small = std::max(small, s);
+      large = std::max(large, l);
+      least = std::min(least, s);
+      batch.list[i] = Given{m.data_ptr(), m.data_ptr(), (int)m.size(0),
+                            (int)m.size(1)};
+    }
+    run(batch, type, (long)n, small, large, least,
+        Polynomial{steps, a, b, c, eps, exact}, first.options());
   }
 }

@@ -31,12 +31,10 @@ def _plain(g, steps, coefficients, eps):
     return (x.transpose(1, 2) if flip else x).to(g.dtype)
 
 
-def _into(g, out, steps, coefficients, eps, exact, turned=None):
-    """``g`` [batch, rows, cols] into ``out`` (which may be ``g``).  On the
-    GPU the matrices from ``turned`` on may lie as [cols, rows]."""
+def _into(g, out, steps, coefficients, eps, exact):
+    """``g`` [batch, rows, cols] into ``out`` (which may be ``g``)."""
     if _ops.use_native(g):
-        _ops.ext().newton_schulz(g, out, steps, *coefficients, eps, exact,
-                                 g.shape[0] if turned is None else turned)
+        _ops.ext().newton_schulz(g, out, steps, *coefficients, eps, exact)
     else:
         with torch.autocast(g.device.type, enabled=False):
             out.copy_(_plain(g, steps, coefficients, eps))

@@ -494,8 +494,8 @@ class Muon(Adam):
     for the matrices: parameters of two or more dimensions (a convolution
     is [out, in kh kw]) in groups with ``muon=True``.  Vectors, sparse rows
     and groups with ``muon=False`` (embeddings, heads) take Adam with
-    ``adam_lr`` and no weight decay.  Matrices of one size go through the
-    products as one batch.  fp32 parameters get products in 22 bits, bf16
+    ``adam_lr`` and no weight decay.  Matrices of about one size go
+    through the products as one batch.  fp32 parameters get products in 22 bits, bf16
     ones with fp32 masters what bf16's rounding can show."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True,
@@ -526,12 +526,15 @@ class Muon(Adam):
         if rest:
             self._adam_step([p for p, _ in rest], [g for _, g in rest],
                             group, group['adam_lr'], 0.0)
-        # one batch for each size, type and device
+        # one batch for each type, device and size: the products fill
+        # matrices up to multiples of 128 with zeros, either way round
         batches = {}
         for p, g in mats:
             if p.numel():
-                key = (tuple(sorted(_storage_matrix(p))), p.dtype, p.device)
-                batches.setdefault(key, []).append((p, g))
+                size = tuple(-(-n // 128)
+                             for n in sorted(_storage_matrix(p)))
+                batches.setdefault((size, p.dtype, p.device),
+                                   []).append((p, g))
         for batch in batches.values():
             self._muon_step([p for p, _ in batch], [g for _, g in batch],
                             group)
@@ -570,24 +573,20 @@ class Muon(Adam):
                 if w is not p:
                     p.copy_(w)
             return
-        # one stack: the wide ones, then those that lie the other way round
-        order = sorted(range(len(params)),
-                       key=lambda i: shapes[i][0] > shapes[i][1])
-        params, grads, bufs, scales, shapes = (
-            [t[i] for i in order]
-            for t in (params, grads, bufs, scales, shapes))
-        masters = [masters[i] for i in order] if has_m else []
-        turned = sum(r <= c for r, c in shapes)
         e = _ops.ext()
         grads = [g if _same_layout(p, g)
                  else torch.empty_like(p, dtype=g.dtype).copy_(g)
                  for p, g in zip(params, grads)]
-        u = torch.empty((len(params),) + tuple(sorted(shapes[0])),
-                        dtype=torch.float32, device=params[0].device)
-        us = list(u.unbind(0))
+        # the updates, each at 16 bytes
+        sizes = [-(-p.numel() // 4) * 4 for p in params]
+        flat = torch.empty(sum(sizes), dtype=torch.float32,
+                           device=params[0].device)
+        us = [u[:p.numel()].view(s) for u, p, s in zip(
+            flat.split(sizes), params, shapes)]
         for gg, bb, uu in _dtype_groups(grads, bufs, us):
             e.multi_tensor_muon_update(gg, bb, uu, mom, group['nesterov'])
-        _into(u, u, group['ns_steps'], COEFFICIENTS, 1e-7, exact, turned)
+        e.newton_schulz_list(us, group['ns_steps'], *COEFFICIENTS, 1e-7,
+                             exact)
         e.multi_tensor_muon_apply(params, us, scales, decay, masters)
 
     @torch.no_grad()

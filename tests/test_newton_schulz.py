@@ -97,6 +97,19 @@ def test_wide_tiles(dtype):
             assert _off(got[i], want[i]) < _bound(dtype, *shape[1:])
 
 
+@GPU
+def test_more_than_go_through_together():
+    g = torch.randn(70, 2048, 2048, dtype=torch.bfloat16, device='cuda')
+    got = ops.newton_schulz(g)
+    for i in (0, 69):
+        off = _off(got[i], _exact(g[i]))
+        assert off < _bound(torch.bfloat16, 2048, 2048), off
+    g = torch.randn(70000, 2, 3, device='cuda')
+    got = ops.newton_schulz(g)
+    for i in (0, 20000, 69999):
+        assert _off(got[i], _exact(g[i])) < _bound(torch.float32, 2, 3)
+
+
 @pytest.mark.parametrize('dev', DEVICES)
 def test_batches_are_separate(dev):
     g = torch.stack([_matrix(40, 70, k, i) * 10.0 ** (3 * i - 3)
@@ -244,6 +257,54 @@ def test_muon_fp32(dev, nesterov, wd):
         assert float(off) < o + 6 * 2.0 ** -24 * float(w.norm()), p.shape
         buf = opt.state[p]['momentum_buffer'].cpu().double()
         assert torch.allclose(buf.reshape(w.shape), b, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_muon_many_of_about_one_size(dev, dtype):
+    """Wide, tall, odd ones and vectors as matrices, more than go together;
+    each as if it were the only one."""
+    g = torch.Generator().manual_seed(6)
+    shapes = [(5 + i, 60 - i) for i in range(55)] + [(1, 128), (128, 128),
+                                                     (3, 129), (129, 3)]
+    ws = [torch.randn(s, generator=g).to(dtype) for s in shapes]
+    gs = [torch.randn(s, generator=g).to(dtype) for s in shapes]
+    ps = [torch.nn.Parameter(w.clone().to(dev)) for w in ws]
+    for p, gr in zip(ps, gs):
+        p.grad = gr.to(dev)
+    opt = optim.Muon(ps)
+    opt.step()
+    for p, w, gr in zip(ps, ws, gs):
+        w, b = w.double(), torch.zeros(w.shape, dtype=torch.float64)
+        _muon_exact(w, b, gr.double())
+        got = opt.state[p]['master'] if dtype == torch.bfloat16 else p
+        step = 0.02 * max(1.0, w.shape[0] / w.shape[1]) ** 0.5 \
+            * 1.25 * min(w.shape) ** 0.5
+        off = float((got.detach().cpu().double() - w).norm())
+        assert off < step * _bound(torch.float32, *w.shape) \
+            + 2 * 2.0 ** -24 * float(w.norm()), p.shape
+
+
+def test_list_refusals():
+    f = ops.ext().newton_schulz_list
+    with pytest.raises(RuntimeError, match='GPU'):
+        f([torch.zeros(4, 4)], 5, A, B, C, 1e-7, True)
+    with pytest.raises(RuntimeError, match='steps'):
+        f([torch.zeros(4, 4)], 0, A, B, C, 1e-7, True)
+    f([], 5, A, B, C, 1e-7, True)
+
+
+@GPU
+def test_list_refusals_on_the_gpu():
+    f = ops.ext().newton_schulz_list
+    z = torch.zeros(8, 8, device='cuda')
+    for other in (torch.zeros(8, 200, device='cuda'),
+                  torch.zeros(200, 8, device='cuda')):
+        with pytest.raises(RuntimeError, match='padded'):
+            f([z, other], 5, A, B, C, 1e-7, True)
+    for other in (z[:, :4], z.bfloat16(), z.cpu(), z[:0], z[0]):
+        with pytest.raises(RuntimeError, match='one type'):
+            f([z, other], 5, A, B, C, 1e-7, True)
 
 
 @pytest.mark.parametrize('dev', DEVICES)
