@@ -159,18 +159,16 @@ std::vector<at::Tensor> sampled_ce_bwd(const at::Tensor& true_logits,
                                        const at::Tensor& lse,
                                        const at::Tensor& dloss);
 
-// linear_ce.hip
-std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
-                                      const at::Tensor& w,
-                                      const c10::optional<at::Tensor>& bias,
-                                      const at::Tensor& labels,
-                                      int64_t ignore, double smoothing,
-                                      int64_t reduction);
-std::vector<at::Tensor> linear_ce_bwd(
-    const at::Tensor& dloss, const at::Tensor& x, const at::Tensor& w,
-    const c10::optional<at::Tensor>& bias, const at::Tensor& labels,
-    const at::Tensor& saved, int64_t ignore, double smoothing,
-    int64_t reduction, bool want_dx, bool want_dw, bool want_db);
+// functions.cpp, of linear_ce.hip and rotary.hip
+at::Tensor linear_ce(const at::Tensor& x, const at::Tensor& w,
+                     const c10::optional<at::Tensor>& bias,
+                     const at::Tensor& labels, int64_t ignore,
+                     double smoothing, int64_t reduction);
+std::vector<at::Tensor> rotary_positions(
+    const at::Tensor& q, const c10::optional<at::Tensor>& k,
+    const at::Tensor& cos, const at::Tensor& sin,
+    const c10::optional<at::Tensor>& positions, int64_t offset,
+    bool interleaved);
 
 // newton_schulz.hip
 void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
@@ -178,13 +176,6 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
 void newton_schulz_list(std::vector<at::Tensor> mats, int64_t steps,
                         double a, double b, double c, double eps,
                         bool exact);
-
-// rotary.hip
-std::vector<at::Tensor> rotary(const at::Tensor& q,
-                               const c10::optional<at::Tensor>& k,
-                               const at::Tensor& cos, const at::Tensor& sin,
-                               const c10::optional<at::Tensor>& positions,
-                               int64_t offset, bool interleaved, bool back);
 
 // lstm_cell.hip
 std::vector<at::Tensor> lstm_gates_fwd(const at::Tensor& gates,
@@ -279,16 +270,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("softmax_ce_bwd", &softmax_ce_bwd);
   m.def("sampled_ce_fwd", &sampled_ce_fwd);
   m.def("sampled_ce_bwd", &sampled_ce_bwd);
-  m.def("linear_ce_fwd", &linear_ce_fwd,
-        "softmax CE of a projection onto a vocabulary, logits not kept");
-  m.def("linear_ce_bwd", &linear_ce_bwd);
+  m.def("linear_ce", &linear_ce,
+        "softmax cross entropy of x @ w.t() + bias, differentiable");
   m.def("newton_schulz", &newton_schulz,
         "Newton-Schulz orthogonalisation of a batch of matrices");
   m.def("newton_schulz_list", &newton_schulz_list,
         "the same for a list of matrices of one padded size, in place");
   m.def("multi_tensor_muon_update", &multi_tensor_muon_update);
   m.def("multi_tensor_muon_apply", &multi_tensor_muon_apply);
-  m.def("rotary", &rotary, "rotary positions of queries and keys");
+  m.def("rotary", &rotary_positions,
+        "rotary positions of queries and keys, differentiable");
   m.def("lstm_gates_fwd", &lstm_gates_fwd);
   m.def("lstm_gates_bwd", &lstm_gates_bwd);
   m.def("lstm_gates_fwd_out", &lstm_gates_fwd_out);

@@ -163,6 +163,10 @@ std::vector<at::Tensor> rotary(const at::Tensor& q,
   TORCH_CHECK(q.is_cuda() && q.dim() == 4 && q.stride(3) == 1,
               "rotary: [B, T, H, D] with a dense last dimension on the GPU "
               "expected");
+  const auto type = q.scalar_type();
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf ||
+                  type == at::kFloat,
+              "rotary: bf16, fp16 or fp32 expected, got ", type);
   const long B = q.size(0), T = q.size(1), D = q.size(3);
   if (k.has_value()) {
     TORCH_CHECK(k->dim() == 4 && k->size(0) == B && k->size(1) == T &&
@@ -244,25 +248,32 @@ std::vector<at::Tensor> rotary(const at::Tensor& q,
     const bool cut = interleaved ? R % v == 0 : R % (2 * v) == 0;
     return cut && D % v == 0 && fits(sq, v, size) && fits(sk, v, size);
   };
-  AT_DISPATCH_FLOATING_TYPES_AND2(
-      at::kBFloat16, at::kHalf, q.scalar_type(), "rotary", [&] {
-        constexpr int W = 16 / sizeof(scalar_t);
-        using Full = std::integral_constant<int, W>;
-        using Two = std::integral_constant<int, 2>;
-        using One = std::integral_constant<int, 1>;
-        constexpr std::true_type yes{};
-        constexpr std::false_type no{};
-        if (interleaved) {
-          if (ok(W)) {
-            launch(scalar_t{}, Full{}, Full{}, yes, yes);
-          } else {
-            launch(scalar_t{}, Two{}, One{}, yes, no);
-          }
-        } else if (ok(W)) {
-          launch(scalar_t{}, Full{}, Full{}, no, yes);
-        } else {
-          launch(scalar_t{}, One{}, One{}, no, no);
-        }
-      });
+  auto run = [&](auto tag) {
+    using E = decltype(tag);
+    constexpr int W = 16 / sizeof(E);
+    using Full = std::integral_constant<int, W>;
+    using Two = std::integral_constant<int, 2>;
+    using One = std::integral_constant<int, 1>;
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    if (interleaved) {
+      if (ok(W)) {
+        launch(E{}, Full{}, Full{}, yes, yes);
+      } else {
+        launch(E{}, Two{}, One{}, yes, no);
+      }
+    } else if (ok(W)) {
+      launch(E{}, Full{}, Full{}, no, yes);
+    } else {
+      launch(E{}, One{}, One{}, no, no);
+    }
+  };
+  if (type == at::kBFloat16) {
+    run(c10::BFloat16{});
+  } else if (type == at::kHalf) {
+    run(c10::Half{});
+  } else {
+    run(float{});
+  }
   return res;
 }

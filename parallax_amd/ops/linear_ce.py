@@ -18,27 +18,6 @@ from parallax_amd import ops as _ops
 _REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
 
 
-class _LinearCEFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, labels, ignore_index, smoothing,
-                reduction):
-        loss, saved = _ops.ext().linear_ce_fwd(
-            x, weight, bias, labels, ignore_index, smoothing, reduction)
-        ctx.save_for_backward(x, weight, bias, labels, saved)
-        ctx.args = (ignore_index, smoothing, reduction)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss):
-        x, weight, bias, labels, saved = ctx.saved_tensors
-        want = ctx.needs_input_grad
-        dx, dw, db = _ops.ext().linear_ce_bwd(
-            dloss.contiguous(), x, weight, bias, labels, saved, *ctx.args,
-            want[0], want[1], bias is not None and want[2])
-        return dx, dw, db, None, None, None, None
-
-
 def _check(inputs, weight, bias, labels, label_smoothing, reduction):
     if reduction not in _REDUCTIONS:
         raise ValueError("linear_cross_entropy: reduction is 'mean', 'sum' "
@@ -105,16 +84,16 @@ def linear_cross_entropy(inputs, weight, bias, labels, reduction='mean',
     if weight.dtype != x.dtype:
         weight = weight.to(x.dtype)
     if x.shape[0] == 0:  # no rows: what a sum over nothing is
-        z = (x.float().sum() + weight.float().sum() * 0) * 0
+        z = x.float().sum() + weight[:0].float().sum()
         if bias is not None:
-            z = z + bias.float().sum() * 0
+            z = z + bias[:0].float().sum()
         if reduction == 'none':
-            return x.float().sum(-1).reshape(labels.shape)
+            return (x.float().sum(-1) + z).reshape(labels.shape)
         return z / 0 if reduction == 'mean' else z
     if _ops.use_native(x):
-        losses = _LinearCEFn.apply(x, weight, bias, y.contiguous(),
-                                   ignore_index, float(label_smoothing),
-                                   _REDUCTIONS[reduction])
+        losses = _ops.ext().linear_ce(x, weight, bias, y.contiguous(),
+                                      ignore_index, label_smoothing,
+                                      _REDUCTIONS[reduction])
     else:
         with torch.autocast(x.device.type, enabled=False):
             losses = _plain(x, weight, bias, y, ignore_index,

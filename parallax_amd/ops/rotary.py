@@ -32,30 +32,6 @@ def _turn(x, cos, sin, interleaved):
     return torch.cat((y.to(x.dtype), x[..., r:]), -1)
 
 
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, offset, interleaved):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(cos, sin, positions)
-        ctx.args = (offset, interleaved)
-        out = _ops.ext().rotary(q, k, cos, sin, positions, offset,
-                                interleaved, False)
-        return (out[0], out[1]) if k is not None else (out[0], None)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        cos, sin, positions = ctx.saved_tensors
-        live = [_last_dense(g) for g in (gq, gk) if g is not None]
-        if not live:
-            return (None,) * 7
-        out = _ops.ext().rotary(live[0], live[1] if len(live) > 1 else None,
-                                cos, sin, positions, *ctx.args, True)
-        dq = out.pop(0) if gq is not None else None
-        dk = out.pop(0) if gk is not None else None
-        return dq, dk, None, None, None, None, None
-
-
 def _last_dense(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
@@ -111,9 +87,9 @@ def apply_rotary(q, k, cos, sin, positions=None, offset=0,
         cos, sin = cos.float().contiguous(), sin.float().contiguous()
         q = _last_dense(q)
         k = _last_dense(k) if k is not None else None
-        a, b = _RotaryFn.apply(q, k, cos, sin, positions, offset,
-                               interleaved)
-        return a if k is None else (a, b)
+        out = _ops.ext().rotary(q, k, cos, sin, positions, offset,
+                                interleaved)
+        return out[0] if k is None else tuple(out)
     if positions is None:
         c, s = (t[offset:offset + q.shape[1]][None, :, None]
                 for t in (cos, sin))

@@ -459,3 +459,43 @@ def test_refusals(dev):
             f(x.double(), w, b, y)
         with pytest.raises(RuntimeError, match='GPU|device'):
             f(x, w.cpu(), b, y)
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('asked', [(0,), (1,), (2,), (0, 2), (1, 2)])
+def test_only_the_asked_gradients(dev, asked):
+    x, w, b, y = _inputs(70, 300, 64, torch.float32, dev, seed=21)
+    every = [t.clone().requires_grad_() for t in (x, w, b)]
+    ops.linear_cross_entropy(*every, y).backward()
+    some = [t.clone().requires_grad_(i in asked)
+            for i, t in enumerate((x, w, b))]
+    ops.linear_cross_entropy(*some, y).backward()
+    for i, (s, t) in enumerate(zip(some, every)):
+        if i in asked:
+            assert torch.equal(s.grad, t.grad)
+        else:
+            assert s.grad is None
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+def test_no_rows_give_no_gradient(dev):
+    x, w, b, y = _inputs(5, 40, 64, torch.float32, dev, seed=22)
+    w[3] = float('nan')
+    for reduction in ('mean', 'sum', 'none'):
+        leaf = [t.clone().requires_grad_() for t in (x[:0], w, b)]
+        ops.linear_cross_entropy(*leaf, y[:0], reduction=reduction).sum() \
+            .backward()
+        assert not leaf[1].grad.any() and not leaf[2].grad.any()
+
+
+@GPU
+def test_second_derivatives_are_refused():
+    x, w, b, y = _inputs(9, 40, 64, torch.float32, 'cuda', seed=23)
+    leaf = [t.clone().requires_grad_() for t in (x, w, b)]
+    loss = ops.linear_cross_entropy(*leaf, y)
+    first = torch.autograd.grad(loss, leaf, create_graph=True)
+    plain = torch.autograd.grad(ops.linear_cross_entropy(*leaf, y), leaf)
+    for p, q in zip(first, plain):
+        assert torch.equal(p, q)
+        with pytest.raises(RuntimeError, match='again'):
+            torch.autograd.grad(p.sum(), leaf, retain_graph=True)

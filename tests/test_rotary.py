@@ -322,3 +322,17 @@ def test_refusals(dev):
         ops.rotary_tables(8, 0)
     with pytest.raises(ValueError, match='rotary_dim'):
         ops.ParallaxRotary(16, 8, rotary_dim=32)
+
+
+@GPU
+def test_refused_on_the_gpu():
+    cos, sin = ops.rotary_tables(16, 8, device='cuda')
+    q, k = _pair(2, 4, 3, 2, 16, torch.float32, 'cuda')
+    with pytest.raises(RuntimeError, match='bf16, fp16 or fp32'):
+        ops.apply_rotary(q.double(), k.double(), cos, sin)
+    q.requires_grad_()
+    a, _ = ops.apply_rotary(q, k, cos, sin)
+    up = torch.ones_like(a, requires_grad=True)
+    dq, = torch.autograd.grad(a, q, up, create_graph=True)
+    with pytest.raises(RuntimeError, match='again'):
+        torch.autograd.grad(dq.sum(), up)
