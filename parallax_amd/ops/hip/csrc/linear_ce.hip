@@ -17,11 +17,11 @@
 // fp32.  No atomics: every result is independent of the order of blocks.
 //
 // Types.  bf16 and fp16 inputs are multiplied as they are; G is rounded to
-// the same type once (2^-9 or 2^-12 of each value, as the final rounding of
-// the gradients is).  fp32 inputs are split into two fp16 parts (22 bits)
-// after a scaling by a power of two, and so is G: three products in the
-// place of one.  fp16 G is scaled by a power of two that brings the largest
-// |g| near the top of fp16's range, and the results are scaled back.
+// the same type once, relative to the largest |g|, and the results are
+// scaled back (2^-9 or 2^-12 of each value, as the final rounding of the
+// gradients is).  fp32 inputs are split into two fp16 parts (22 bits) after
+// a scaling by a power of two, and so is G: three products in the place of
+// one.
 //
 // Rows whose label is ignored are read as zeros, so what lies in them (a
 // padded batch's garbage, NaN) reaches no gradient.
@@ -128,6 +128,17 @@ __device__ __forceinline__ float scale_to_half(float top) {
   return ldexpf(1.f, e);
 }
 
+// S for G: bf16 and fp16 rows of the largest |g| get -1 or -2^13 at a label
+// without probability, where G = -(1 - e) g.  These values are many and, as
+// g is often that of all rows, equal: rounded, they would all be off by the
+// same, up to 2^-8 (2^-11) of dx and dw.
+__device__ __forceinline__ float scale_of_g(float top, float e, int type) {
+  if (e <= 0.5f) top *= 1.f - e;
+  if (type == 2 || !(top > 1e-30f) || !(top < 1e30f))
+    return type == 0 ? 1.f : scale_to_half(top);
+  return (type == 0 ? 1.f : 8192.f) / top;
+}
+
 // --- laying out an operand --------------------------------------------------
 
 // What the gradient needs of the rows.  Rows that do not count: an infinite
@@ -165,6 +176,7 @@ struct Pack {
   const float* count;
   const float* lse;
   long V;
+  float eps;
   float* sc;
 };
 
@@ -200,9 +212,9 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     if (p.sc && !p.each) {
-      // |softmax - target| <= 1, so S |G| stays below 2^14
+      // |softmax - target| <= 1, so S |G| stays below 2^15
       const float g = p.dloss[0] / (p.count ? p.count[0] : 1.f);
-      const float s = p.type != 0 ? scale_to_half(fabsf(g)) : 1.f;
+      const float s = scale_of_g(fabsf(g), p.eps, p.type);
       p.sc[0] = s;
       p.sc[1] = 1.f / s;
     }
@@ -288,14 +300,14 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
 // sc = {S, 1/S} where every row has a gradient of its own
 __global__ __launch_bounds__(1024) void lce_scale_kernel(
     const float* __restrict__ dloss, const int64_t* __restrict__ labels,
-    int64_t ignore, int n, bool half, float* __restrict__ sc) {
+    int64_t ignore, int n, float eps, int type, float* __restrict__ sc) {
   __shared__ float red[16];
   float most = 0.f;
   for (int i = threadIdx.x; i < n; i += 1024)
     if (labels[i] != ignore) most = fmaxf(most, fabsf(dloss[i]));
   most = block_reduce_max(most, red);
   if (threadIdx.x == 0) {
-    const float s = half ? scale_to_half(most) : 1.f;
+    const float s = scale_of_g(most, eps, type);
     sc[0] = s;
     sc[1] = 1.f / s;
   }
@@ -465,14 +477,20 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = top;
 }
 
-// One wave a row: joins its partial sums, takes the label's logit as a dot
-// product, and the loss.
+// One wave a row joins its partial sums, takes the label's logit as a dot
+// product, and the loss.  WAVES: that many take a row's sums (6,200 of each
+// of 320 rows: 22 us with four, 61 with one).
+template <int WAVES>
 __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
+  __shared__ float red[4][3];
   const int lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int wave = threadIdx.x >> 6;
+  const int r = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
   if (r < p.n) {
     float m = -INFINITY, s = 0.f, t = 0.f;
-    for (int b = lane; b < p.nblocks; b += 64) {
+#pragma unroll 4
+    for (int b = WAVES == 1 ? lane : threadIdx.x; b < p.nblocks;
+         b += 64 * WAVES) {
       const long at = (long)r * p.nblocks + b;
       if (p.eps != 0.f) {
         const f4 v = reinterpret_cast<const f4*>(p.part)[at];
@@ -487,7 +505,7 @@ __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
     const bool live = y0 != p.ignore;
     const long y = y0 < 0 ? 0 : (y0 >= p.V ? p.V - 1 : y0);
     float a = 0.f;
-    if (live) {
+    if (live && (WAVES == 1 || wave == 0)) {
       for (int c = lane; c < p.d; c += 64)
         a += load_as(p.x.p, r * p.x.rs + c * p.x.cs, p.x.type) *
              load_as(p.w.p, y * p.w.rs + c * p.w.cs, p.w.type);
@@ -497,6 +515,19 @@ __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
       join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
       t += __shfl_xor(t, o, 64);
       a += __shfl_xor(a, o, 64);
+    }
+    if (WAVES > 1) {
+      if (lane == 0) {
+        red[wave][0] = m;
+        red[wave][1] = s;
+        red[wave][2] = t;
+      }
+      __syncthreads();
+      if (wave > 0) return;
+      for (int q = 1; q < WAVES; ++q) {
+        join(m, s, red[q][0], red[q][1]);
+        t += red[q][2];
+      }
     }
     if (lane == 0) {
       if (live && p.bias.p) a += load_as(p.bias.p, y * p.bias.rs, p.bias.type);
@@ -579,7 +610,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     // there are rows up to a whole tile
     const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
     const f4 l = *reinterpret_cast<const f4*>(rows.l + n);
-    const f4 g = *reinterpret_cast<const f4*>(rows.g + n);
+    const f4 g = S * *reinterpret_cast<const f4*>(rows.g + n);
     const int4 y = *reinterpret_cast<const int4*>(rows.y + n);
 #pragma unroll
     for (int i = 0; i < C::FM; ++i)
@@ -612,7 +643,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     }
   if constexpr (PARTS == 2) {
     store_pairs<C>(smem, G + (long)m0 * ldg + n0 * 2, ldg,
-                   [&](int i, int j) { return acc[i][j] * S; });
+                   [&](int i, int j) { return acc[i][j]; });
   } else {
     store_tile<C>(smem, G + (long)m0 * ldg + n0, ldg, C::BM, C::BN,
                   [&](int i, int j) {
@@ -620,8 +651,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
       if (BF)
         return make_ushort4(bf16_bits(v[0]), bf16_bits(v[1]),
                             bf16_bits(v[2]), bf16_bits(v[3]));
-      return make_ushort4(fp16_bits(v[0] * S), fp16_bits(v[1] * S),
-                          fp16_bits(v[2] * S), fp16_bits(v[3] * S));
+      return make_ushort4(fp16_bits(v[0]), fp16_bits(v[1]), fp16_bits(v[2]),
+                          fp16_bits(v[3]));
     });
   }
   if (DB) {
@@ -645,6 +676,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     for (int c = threadIdx.x; c < C::BM; c += C::THREADS) {
       float s = red[c];
       for (int w = 1; w < C::WAVES_N; ++w) s += red[w * C::BM + c];
+      s *= sc[1];
       if (nrt > 1) {
         dbp[rt * db_ld + m0 + c] = s;
       } else if (m0 + c < p.vp) {
@@ -773,8 +805,9 @@ __global__ __launch_bounds__(256) void lce_dx_sum_kernel(
 // byte that comes from memory, and four waves on a SIMD to wait for another.
 using Big = Tile<256, 256, 64, 64, 64, 2>;
 using Mid = Tile<128, 128, 64, 64, 64, 2>;
-// two parts: eight waves, as they leave the LDS more time
-using MidParts = Tile<128, 128, 64, 32, 64, 2>;
+// two parts: eight waves, as they leave the LDS more time (both operands
+// k-strided, 20480 x 512 x 2560: 148 us, 160 with four waves of 64 x 64)
+using MidParts = Tile<128, 128, 32, 64, 64, 2>;
 template <int PARTS>
 using MidOf = std::conditional_t<PARTS == 2, MidParts, Mid>;
 // few rows: wide in the words
@@ -1116,7 +1149,11 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
     j.eps = eps;
     j.loss = reduction == 0 ? out.data_ptr<float>() : mem.at<float>(o_loss);
     j.lse = lse;
-    lce_join_kernel<<<(int)((p.n + 3) / 4), 256, 0, stream>>>(j);
+    if (blocks > 1024) {
+      lce_join_kernel<4><<<(int)p.n, 256, 0, stream>>>(j);
+    } else {
+      lce_join_kernel<1><<<(int)((p.n + 3) / 4), 256, 0, stream>>>(j);
+    }
     HIP_CHECK_KERNEL();
     if (reduction != 0) {
       lce_total_kernel<<<1, 1024, 0, stream>>>(
@@ -1215,11 +1252,12 @@ std::vector<at::Tensor> linear_ce_bwd(
     kx.count = reduction == 1 ? lse + p.n : nullptr;
     kx.lse = lse;
     kx.V = p.v;
+    kx.eps = eps;
     kx.sc = mem.at<float>(o_sc);
     pack(kx, stream);
     if (kx.each) {
       lce_scale_kernel<<<1, 1024, 0, stream>>>(
-          kx.dloss, lab, ignore, (int)p.n, p.type != 0, kx.sc);
+          kx.dloss, lab, ignore, (int)p.n, eps, p.type, kx.sc);
       HIP_CHECK_KERNEL();
     }
     auto* G = mem.at<ushort>(o_G);
@@ -1323,7 +1361,7 @@ std::vector<at::Tensor> linear_ce_bwd(
             HIP_CHECK_KERNEL();
           };
           if (dx_tile == 128) {
-            run(Mid{});
+            run(MidOf<PARTS>{});
           } else {
             run(Small{});
           }

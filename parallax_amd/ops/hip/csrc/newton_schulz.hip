@@ -2,7 +2,7 @@
 // step), batched:
 //
 //   X0 = G / (|G|_F + eps)             [m, n], m <= n (else transposed)
-//   A = X X^T,  B = b A + c A A,  X <- a X + B X      `steps` times
+//   A = X X^T,  B = b A + c A A,  X <- (a + B) X      `steps` times
 //
 // Each singular value s of X0 goes to p(p(..p(s))), p(s) = a s + b s^3 +
 // c s^5.  Three products an iteration: X X^T and A A are symmetric, so only
@@ -11,7 +11,7 @@
 // transposing LDS read.
 //
 // Precision.  Everything between the products lives in fp16 scaled by 2^12
-// (|X| <= 1.2, |A| <= 1.5, |B| <= 3: 2^12 keeps 2^-26 of the largest value
+// (|X| <= 1.2, |A| <= 1.5, |a + B| <= 4: 2^12 keeps 2^-26 of the largest value
 // out of fp16's subnormals).  X is always a high and a low part (22 bits);
 // the operands of a product are one part (11 bits) or both, and the sums
 // are fp32.  A relative error of a singular value grows by up to 10, 18, 11,
@@ -261,15 +261,17 @@ __device__ __forceinline__ void put_tile(char* lds, const Matrix& out, int m0,
 
 // One symmetric product [mp, mp]: S = sum_k P[i, k] P[j, k].
 //   SECOND = false: out = S                (P = X, S = A)
-//   SECOND = true:  out = b P + c S        (P = A, S = A A)
+//   SECOND = true:  out = b P + c S        (P = A, S = A A), in two parts
+//                   also + a on the diagonal, as that takes aX from the next
+//                   product: 22 bits of a are as many as X' keeps
 // Where there are few tiles, k is cut (CUT = 1): each workgroup leaves its
 // sums in `part`, and a second kernel (CUT = 2) adds them up in order and
 // goes on.  (Left to the last workgroup of a tile, the fences that takes
 // cost more than the launch: 146 us for 12 x 512 x 2048, 50 this way.)
 template <class C, int PARTS, bool SECOND, int CUT>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
-    Matrix P, int kp, float b, float c, Matrix out, int tiles, int cuts,
-    float* __restrict__ part) {
+    Matrix P, int kp, float a, float b, float c, Matrix out, int tiles,
+    int cuts, float* __restrict__ part) {
   static_assert(C::BM == C::BN, "square tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // tile pairs on and above the diagonal, row by row
@@ -323,10 +325,16 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) {
       f4 v = acc[i][j] * (1.f / kScale);
-      if (SECOND)
-        v = b * P.four<PARTS == 2>(m0 + wm + i * 16 + (lane & 15),
-                                   n0 + wn + j * 16 + (lane >> 4) * 4) +
-            c * v;
+      if (SECOND) {
+        const int m = m0 + wm + i * 16 + (lane & 15);
+        const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+        v = b * P.four<PARTS == 2>(m, n) + c * v;
+        if (PARTS == 2) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (m == n + r) v[r] += a * kScale;
+        }
+      }
       acc[i][j] = v;
     }
   put_tile<C, PARTS, false>(smem, out, m0, n0,
@@ -374,8 +382,9 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
   }
 }
 
-// X' = a X + B X; the last one goes to the result.  The sums start from
-// a X, so that it is read while the first stages are on their way.
+// X' = a X + B X (two parts: B holds the a); the last one goes to the result.
+// The sums start from a X, so that it is read while the first stages are on
+// their way.
 template <class C, int PARTS>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_next_kernel(
     Matrix B, int kp, Matrix X, float a, Matrix out, bool last, Batch batch,
@@ -389,14 +398,16 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_next_kernel(
   const int wn = (wave % C::WAVES_N) * C::WN;
   B = B.of(blockIdx.y);
   X = X.of(blockIdx.y);
-  f4 acc[C::FM][C::FN];
+  f4 acc[C::FM][C::FN] = {};
+  if (PARTS == 1) {
 #pragma unroll
-  for (int i = 0; i < C::FM; ++i)
+    for (int i = 0; i < C::FM; ++i)
 #pragma unroll
-    for (int j = 0; j < C::FN; ++j)
-      acc[i][j] = a * kScale *
-                  X.four<true>(m0 + wm + i * 16 + (lane & 15),
-                               n0 + wn + j * 16 + (lane >> 4) * 4);
+      for (int j = 0; j < C::FN; ++j)
+        acc[i][j] = a * kScale *
+                    X.four<true>(m0 + wm + i * 16 + (lane & 15),
+                                 n0 + wn + j * 16 + (lane >> 4) * 4);
+  }
   product<C, KROWS, KCOLS, PARTS, false>(smem, B.operand(), m0, X.operand(),
                                          n0, 0, kp, acc);
   if (!last) {
@@ -594,7 +605,7 @@ void run(const Batch& batch, int type, long count, long small, long large,
         auto launch = [&](auto kernel, int lds, int n) {
           allow_lds(kernel, lds);
           kernel<<<dim3(pairs * n, count), C::THREADS, lds, stream>>>(
-              P, k, (float)p.b, (float)p.c, o, tiles, cut, part);
+              P, k, (float)p.a, (float)p.b, (float)p.c, o, tiles, cut, part);
           HIP_CHECK_KERNEL();
         };
         constexpr int one = C::template lds<1>(), two = C::template lds<2>();

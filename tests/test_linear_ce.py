@@ -499,3 +499,34 @@ def test_second_derivatives_are_refused():
         assert torch.equal(p, q)
         with pytest.raises(RuntimeError, match='again'):
             torch.autograd.grad(p.sum(), leaf, retain_graph=True)
+
+
+@GPU
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('eps', [0.0, 0.1])
+def test_equal_rows_are_not_rounded_alike(dtype, eps):
+    """A mean over 45 or 53 rows gives every row 1/45 or 1/53, and a label
+    without probability -(1 - eps) of that: rounded to 8 or 11 bits, all
+    labels' parts of the gradients would be off by the same.  Relative to
+    that value they are 1 and round to themselves: G is off by D = what
+    rounding G / up / (1 - eps) changes, dx by D w and dw by D^T x, and each
+    by its own rounding, so in norm by at most the sum of both.  The other
+    bounds above, of 2^-24, are below a hundredth of it."""
+    for n in (45, 53):
+        x, w, b, y = _inputs(n, 3000, 256, dtype, 'cuda', seed=24)
+        leaf = [t.clone().requires_grad_() for t in (x, w, b)]
+        ops.linear_cross_entropy(*leaf, y, label_smoothing=eps).backward()
+        up = torch.full((n,), 1.0 / n, dtype=torch.float64)
+        _, dx, dw, _ = _exact(x, w, b, y, up, eps)
+        x, w, b, y = (t.cpu() for t in (x, w, b, y))
+        x, w, b = x.double(), w.double(), b.double()
+        G = torch.softmax(x @ w.t() + b, 1) - eps / 3000
+        G[torch.arange(n), y] -= 1 - eps
+        G = G / (1 - eps) * (1.0 if dtype == torch.bfloat16 else 8192.0)
+        D = (G.to(dtype).double() - G) * ((1 - eps) / n)
+        if dtype == torch.float16:
+            D = D / 8192.0
+        for t, (want, _), part in zip(leaf, (dx, dw), (D @ w, D.t() @ x)):
+            own = (want.to(dtype).double() - want).norm()
+            off = (t.grad.cpu().double() - want).norm()
+            assert float(off) < 1.01 * float(own + part.norm())
