@@ -973,8 +973,8 @@ void check(const at::Tensor& x, const at::Tensor& w,
   TORCH_CHECK(x.size(0) >= 1 && x.size(0) <= (1 << 20),
               "linear_ce: 1 to 2^20 rows expected");
   TORCH_CHECK(w.size(0) < (1L << 31) - 1024, "linear_ce: too many words");
-  TORCH_CHECK(up(x.size(0), 256) * up(x.size(1), 64) <= (1L << 29),
-              "linear_ce: x has more than 2^29 values: take fewer rows at a "
+  TORCH_CHECK(up(x.size(0), 256) * up(x.size(1), 64) < (1L << 29),
+              "linear_ce: x has 2^29 values or more: take fewer rows at a "
               "time");
   TORCH_CHECK(labels.scalar_type() == at::kLong && labels.dim() == 1 &&
                   labels.size(0) == x.size(0) && labels.is_contiguous(),
@@ -1193,9 +1193,9 @@ std::vector<at::Tensor> linear_ce_bwd(
                                  : piece / 256 * 256;
   piece = std::max(256L, std::min(piece, up(p.v, 256)));
   if (!p.w_direct) piece = std::min(piece, p.w_rows);
-  // offsets inside a piece of w stay below 2^31
+  // a piece of w ends before its byte 2^31, the largest offset there is
   const long w_ld = p.w_direct ? w.stride(0) : p.dp * p.parts;
-  piece = std::max(256L, std::min(piece, (1L << 30) / w_ld / 256 * 256));
+  piece = std::max(256L, std::min(piece, ((1L << 30) - 1) / w_ld / 256 * 256));
   const int ldg = (int)p.np * p.parts;
   // dx: few tiles and a long k, so k is cut until the chip is full
   const int dx_tile = p.n > 128 && p.dp >= 128 ? 128 : 64;

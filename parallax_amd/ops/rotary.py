@@ -78,8 +78,11 @@ def apply_rotary(q, k, cos, sin, positions=None, offset=0,
     sin [places, R/2] fp32, R <= D: the rest of a head passes through.
     Pairs are (i, i + R/2), or (2i, 2i+1) where ``interleaved``.  Token t of
     a sequence stands at ``positions[b, t]`` (integers [T] or [B, T],
-    clamped to the tables) or at ``offset + t``."""
+    clamped to the tables) or at ``offset + t``.  No gradient flows to the
+    tables."""
     _check(q, k, cos, sin, positions, offset)
+    if cos.requires_grad or sin.requires_grad:
+        cos, sin = cos.detach(), sin.detach()
     if positions is not None:
         positions = positions.long()
         positions = positions[None] if positions.dim() == 1 else positions

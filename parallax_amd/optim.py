@@ -495,8 +495,8 @@ class Muon(Adam):
     is [out, in kh kw]) in groups with ``muon=True``.  Vectors, sparse rows
     and groups with ``muon=False`` (embeddings, heads) take Adam with
     ``adam_lr`` and no weight decay.  Matrices of about one size go
-    through the products as one batch.  fp32 parameters get products in 22 bits, bf16
-    ones with fp32 masters what bf16's rounding can show."""
+    through the products as one batch.  fp32 parameters get products in 22
+    bits, bf16 ones with fp32 masters what bf16's rounding can show."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True,
                  weight_decay=0.0, ns_steps=5, muon=True, adam_lr=3e-4,

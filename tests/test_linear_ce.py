@@ -530,3 +530,41 @@ def test_equal_rows_are_not_rounded_alike(dtype, eps):
             own = (want.to(dtype).double() - want).norm()
             off = (t.grad.cpu().double() - want).norm()
             assert float(off) < 1.01 * float(own + part.norm())
+
+
+@GPU
+def test_piece_at_the_largest_offset():
+    """A table of 2^31 bytes and more: the last values before that."""
+    last = (1 << 31) // 8192 - 1
+    v, d = last + 300, 4096
+    g = torch.Generator(device='cuda').manual_seed(25)
+    w = torch.empty(v, d, dtype=torch.bfloat16, device='cuda')
+    w.normal_(0, 1 / 64, generator=g)
+    x = torch.randn(3, d, generator=g, device='cuda').bfloat16()
+    xl = x.clone().requires_grad_()
+    y = torch.full((3,), last, device='cuda')
+    ops.linear_cross_entropy(xl, w, None, y, reduction='sum').backward()
+    # E[w exp(x w)] / E[exp(x w)] = x / 64^2 for words of deviation 1 / 64;
+    # about it the mean over V words with logits of deviation 1 has one of
+    # sqrt(e / V) / 64, which the second term is 4.8 times; bf16 rounds by
+    # 2^-8 of the result
+    tol = 2.0 ** -8 * w[last].float().abs() + 8 * v ** -0.5 / 64
+    off = (xl.grad.float() + w[last].float() - x.float() / 4096).abs()
+    assert bool((off <= tol).all()), float((off - tol).max())
+    assert float(w[last, -8:].abs().max()) > 4 * float(tol.max())
+
+
+@GPU
+def test_refused_sizes():
+    f = ops.linear_cross_entropy
+    big = torch.zeros(1, 1, device='cuda').expand(1 << 20, 512)
+    y = torch.zeros(1, dtype=torch.long, device='cuda').expand(1 << 20)
+    w = torch.zeros(4, 512, device='cuda')
+    with pytest.raises(RuntimeError, match='fewer rows'):
+        f(big, w, None, y)
+    with pytest.raises(RuntimeError, match='2.20 rows'):
+        f(big[:, :1].expand(1 << 20, 1).repeat(2, 1), w[:, :1], None,
+          y.repeat(2))
+    with pytest.raises(RuntimeError, match='32768'):
+        f(torch.zeros(2, 40000, device='cuda'),
+          torch.zeros(3, 40000, device='cuda'), None, y[:2])

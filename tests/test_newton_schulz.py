@@ -435,3 +435,38 @@ def test_muon_in_a_graph():
         torch.cuda.synchronize()
         oq.step()
         assert torch.equal(p, q)
+
+
+@GPU
+def test_muon_fp16():
+    g = torch.Generator().manual_seed(7)
+    w0 = torch.randn(30, 50, generator=g).half()
+    gr = torch.randn(30, 50, generator=g).half()
+    p = torch.nn.Parameter(w0.cuda())
+    p.grad = gr.cuda()
+    opt = optim.Muon([p])
+    opt.step()
+    w, b = w0.double(), torch.zeros(30, 50, dtype=torch.float64)
+    _muon_exact(w, b, gr.double())
+    off = (opt.state[p]['master'].cpu().double() - w).norm()
+    assert float(off) < 0.02 * 1.25 * 30 ** 0.5 \
+        * _bound(torch.float32, 30, 50) + 2 * 2.0 ** -24 * float(w.norm())
+    assert torch.equal(p.detach(), opt.state[p]['master'].half())
+
+
+@GPU
+def test_two_streams_at_once():
+    """Calls that run side by side share nothing."""
+    g = [_matrix(300, 500, seed=i).cuda() for i in range(2)]
+    want = [ops.newton_schulz(t) for t in g]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        for s, t in zip(streams, g):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(ops.newton_schulz(t))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 2])

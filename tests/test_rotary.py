@@ -324,6 +324,16 @@ def test_refusals(dev):
         ops.ParallaxRotary(16, 8, rotary_dim=32)
 
 
+@pytest.mark.parametrize('dev', DEVICES)
+def test_tables_get_no_gradient(dev):
+    cos, sin = ops.rotary_tables(16, 8, device=dev)
+    q, k = _pair(2, 4, 3, 2, 16, torch.float32, dev)
+    want = ops.apply_rotary(q, k, cos, sin)
+    got = ops.apply_rotary(q, k, cos.requires_grad_(), sin.requires_grad_())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b) and not a.requires_grad
+
+
 @GPU
 def test_refused_on_the_gpu():
     cos, sin = ops.rotary_tables(16, 8, device='cuda')
