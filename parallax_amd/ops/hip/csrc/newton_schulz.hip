@@ -540,27 +540,37 @@ void run(const Batch& batch, int type, long count, long small, long large,
   const bool every = p.exact || least < 256;
   auto fine = [&](int64_t i) { return every || i >= p.steps - 3; };
 
+  // zeros up to whole tiles, and whole stages of 128 k
+  const int mp = (int)up(small, 128), np = (int)up(large, 128);
   // The largest tile that still gives half of the chip's 256 CUs something
-  // to do, for a symmetric product of 128 x 128 tiles all of them.
+  // to do.
   auto full_tiles = [&](long t) {
     return (small + t - 1) / t * ((large + t - 1) / t) * count;
   };
-  auto sym_tiles = [&](long t) {
-    const long n = (small + t - 1) / t;
-    return n * (n + 1) / 2 * count;
-  };
   const int full = full_tiles(128) >= 128 ? 128
                    : full_tiles(64) >= 128 ? 64 : 32;
-  const int sym = sym_tiles(128) >= 256 ? 128
-                  : sym_tiles(64) >= 100 ? 64 : 32;
-  // and a long k of few tiles is cut
-  auto cuts_of = [&](long k) {
-    return (int)std::max(1L, std::min({512 / sym_tiles(sym), k / 1024, 8L}));
+  // The same for a symmetric product over k, where few tiles' k is cut for
+  // more of them.  12 x 512 over 2048, two parts: 120 tiles of 128 cut in two
+  // 33 + 9 us, in four 36 + 12, 432 of 64 uncut 53.  Over 512, not worth a
+  // cut: 120 of 128 23 us, 432 of 64 19.  Fewer of 128 lose as well, as the
+  // sums are added up by a workgroup a tile: 1024 over 8192, 36 cut in seven
+  // 39 + 10 us, 136 of 64 cut in three 43 + 6; 1024 over 4096 five steps 393
+  // and 373 us.
+  struct Cut {
+    int tile, cuts;
+    long pairs;  // tiles of one matrix
   };
-  // zeros up to whole tiles, and whole stages of 128 k
-  const int mp = (int)up(small, 128), np = (int)up(large, 128);
-  const long pairs = (long)(mp / sym) * (mp / sym + 1) / 2;
-  const int cuts = std::max(cuts_of(np), cuts_of(mp));
+  auto cut_of = [&](long k) {
+    auto cut = [&](long tile, long all, long least) {
+      const long pairs = mp / tile * (mp / tile + 1) / 2;
+      const long cuts = std::min(all / (pairs * count), k / least);
+      return Cut{(int)tile, (int)std::max(1L, cuts), pairs};
+    };
+    const Cut big = cut(128, 256, 512), mid = cut(64, 512, 1024);
+    if (big.pairs * count >= (big.cuts > 1 ? 100 : 256)) return big;
+    return mid.pairs * count >= 100 ? mid : cut(32, 256, 1024);
+  };
+  const Cut wide = cut_of(np), square = cut_of(mp);
   const int blocks = (int)std::min<long>(1024, (small * large + 4095) / 4096);
 
   // one allocation: two X, A, B, the norm's partial sums, the cut sums
@@ -574,8 +584,11 @@ void run(const Batch& batch, int type, long count, long small, long large,
   const size_t o_x0 = take(count * xs * 2), o_x1 = take(count * xs * 2);
   const size_t o_a = take(count * as * 2), o_b = take(count * as * 2);
   const size_t o_norm = take(count * blocks * sizeof(double));
-  const size_t o_part =
-      take(cuts > 1 ? count * pairs * cuts * sym * sym * 4 : 0);
+  auto part_of = [&](const Cut& c) {
+    return c.cuts > 1 ? c.pairs * c.cuts * c.tile * c.tile * 4 : 0L;
+  };
+  const size_t o_part = take(count * std::max(part_of(wide),
+                                              part_of(square)));
   auto mem = at::empty({(long)bytes}, options.dtype(at::kByte));
   char* base = static_cast<char*>(mem.data_ptr());
   auto matrix = [&](size_t at, long stride, int r, int c, bool in_pairs) {
@@ -599,12 +612,13 @@ void run(const Batch& batch, int type, long count, long small, long large,
     auto symmetric = [&](auto second, const Matrix& P, int k,
                          const Matrix& o) {
       constexpr bool SECOND = decltype(second)::value;
-      const int tiles = mp / sym, cut = cuts_of(k);
-      with_tile(sym, [&](auto t) {
+      const Cut& way = SECOND ? square : wide;
+      const int tiles = mp / way.tile, cut = way.cuts;
+      with_tile(way.tile, [&](auto t) {
         using C = decltype(t);
         auto launch = [&](auto kernel, int lds, int n) {
           allow_lds(kernel, lds);
-          kernel<<<dim3(pairs * n, count), C::THREADS, lds, stream>>>(
+          kernel<<<dim3(way.pairs * n, count), C::THREADS, lds, stream>>>(
               P, k, (float)p.a, (float)p.b, (float)p.c, o, tiles, cut, part);
           HIP_CHECK_KERNEL();
         };
