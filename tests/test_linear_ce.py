@@ -568,3 +568,10 @@ def test_refused_sizes():
     with pytest.raises(RuntimeError, match='32768'):
         f(torch.zeros(2, 40000, device='cuda'),
           torch.zeros(3, 40000, device='cuda'), None, y[:2])
+
+
+@GPU
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n', [128, 130, 192, 193, 256, 320, 321, 440, 449])
+def test_every_tile_of_rows(dtype, n):
+    _check(*_inputs(n, 600, 128, dtype, 'cuda', seed=26))
