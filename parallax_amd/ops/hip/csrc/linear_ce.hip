@@ -383,7 +383,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
         const int v = n0 + wn + j * 16 + (lane >> 4) * 4 + r;
         ws[j][r] = PARTS == 2 && v < p.vp ? p.winv[v] * kLog2e : kLog2e;
       }
-    if (n0 + C::BN > p.vp) {  // words behind the last one
+    const bool whole = n0 + C::BN <= p.vp;
+    if (!whole) {  // words behind the last one
 #pragma unroll
       for (int j = 0; j < C::FN; ++j)
 #pragma unroll
@@ -413,13 +414,20 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           s += exp2_fast(acc[i][j][r] - off);
-          if (SMOOTH) {
-            const int v = n0 + wn + j * 16 + (lane >> 4) * 4 + r;
-            if (v < p.vp) tot[i] += acc[i][j][r];
-          }
+          if (SMOOTH && whole) tot[i] += acc[i][j][r];
         }
       mx[i] = top;
       se[i] = s;
+    }
+    if (SMOOTH && !whole) {
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n0 + wn + j * 16 + (lane >> 4) * 4 + r < p.vp)
+              tot[i] += acc[i][j][r];
     }
   }
   // join the four lane groups, then the waves of a row of waves
@@ -514,6 +522,7 @@ __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
     const long y = y0 < 0 ? 0 : (y0 >= p.V ? p.V - 1 : y0);
     float a = 0.f;
     if (live && (WAVES == 1 || wave == 0)) {
+#pragma unroll 4
       for (int c = lane; c < p.d; c += 64)
         a += load_as(p.x.p, r * p.x.rs + c * p.x.cs, p.x.type) *
              load_as(p.w.p, y * p.w.rs + c * p.w.cs, p.w.type);
@@ -555,23 +564,30 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(
     const float* __restrict__ loss, const int64_t* __restrict__ labels,
     int64_t ignore, int n, bool mean, float* __restrict__ out,
     float* __restrict__ count) {
-  __shared__ double sd[1024];
-  __shared__ int sn[1024];
+  __shared__ double sd[16];
+  __shared__ int sn[16];
   double a = 0.;
   int c = 0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += 1024) {
     a += loss[i];
     c += labels[i] != ignore;
   }
-  sd[threadIdx.x] = a;
-  sn[threadIdx.x] = c;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o, 64);
+    c += __shfl_xor(c, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sd[threadIdx.x >> 6] = a;
+    sn[threadIdx.x >> 6] = c;
+  }
   __syncthreads();
-  for (int o = 512; o > 0; o >>= 1) {
-    if (threadIdx.x < o) {
-      sd[threadIdx.x] += sd[threadIdx.x + o];
-      sn[threadIdx.x] += sn[threadIdx.x + o];
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) {
+      sd[0] += sd[w];
+      sn[0] += sn[w];
     }
-    __syncthreads();
   }
   if (threadIdx.x == 0) {
     out[0] = (float)(mean ? sd[0] / sn[0] : sd[0]);
