@@ -1075,7 +1075,7 @@ void with_row_tile(const Plan& p, F f) {
 }  // namespace
 
 // {loss (scalar or [N]), what the backward needs: lse [N], the count, and
-// (fp32) the largest |w| of blocks}
+// (fp32) the largest |w| and |x| of blocks}
 std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
                                       const at::Tensor& w,
                                       const c10::optional<at::Tensor>& bias,
@@ -1095,7 +1095,8 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
   const int wblocks = pack_blocks(p.w_rows);
   const long ntop = p.parts == 2 ? pieces * wblocks : 0;
   auto out = reduction == 0 ? at::empty({p.n}, f32) : at::empty({}, f32);
-  auto saved = at::empty({p.n + 1 + ntop}, f32);
+  const long xtop = p.parts == 2 ? pack_blocks(p.np) : 0;
+  auto saved = at::empty({p.n + 1 + ntop + xtop}, f32);
   float* lse = saved.data_ptr<float>();
   float* tops = lse + p.n + 1;
 
@@ -1127,6 +1128,7 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
     kx.labels = lab;
     kx.ignore = ignore;
     kx.inv = mem.at<float>(o_xinv);
+    if (p.parts == 2) kx.bmax = tops + ntop;
     pack(kx, stream);
     for (long i = 0; i < pieces; ++i) {
       const long v0 = i * piece, vp = std::min(piece, p.v - v0);
@@ -1221,7 +1223,8 @@ std::vector<at::Tensor> linear_ce_bwd(
   const bool two = p.parts == 2, blk = blocked(p);
   const float* lse = saved.data_ptr<float>();
   const float* tops = lse + p.n + 1;
-  const int ntop = (int)(saved.numel() - p.n - 1);
+  const int xtop = two ? pack_blocks(p.np) : 0;
+  const int ntop = (int)(saved.numel() - p.n - 1) - xtop;
 
   // words for which the tiles of dw fill the chip's 256 CUs once
   const long wave_of_words = 256 * 256 / ((p.dp + 255) / 256);
@@ -1258,7 +1261,6 @@ std::vector<at::Tensor> linear_ce_bwd(
     const auto o_x = mem.take<ushort>(p.np * p.dp * p.parts);
     const auto o_xblk = mem.take<ushort>(blk ? p.np * p.dp : 0);
     const auto o_xinv = mem.take<float>(two ? p.np : 0);
-    const auto o_xtop = mem.take<float>(two ? pack_blocks(p.np) : 0);
     const auto o_w = mem.take<ushort>(p.w_direct ? 0
                                                  : piece * p.dp * p.parts);
     const auto o_winv = mem.take<float>(two ? piece : 0);
@@ -1272,14 +1274,9 @@ std::vector<at::Tensor> linear_ce_bwd(
     kx.labels = lab;
     kx.ignore = ignore;
     kx.inv = mem.at<float>(o_xinv);
-    if (two) {
-      // one scale for all rows, as the rows are summed over: the first call
-      // only finds the largest value
-      kx.bmax = mem.at<float>(o_xtop);
-      pack(kx, stream);
-      kx.bmax = nullptr;
-      kx.top = mem.at<float>(o_xtop);
-      kx.ntop = pack_blocks(p.np);
+    if (two) {  // one scale for all rows, as the rows are summed over
+      kx.top = tops + ntop;
+      kx.ntop = xtop;
     }
     if (blk) kx.blocks = mem.at<ushort>(o_xblk);
     float* row = mem.at<float>(o_rows);
