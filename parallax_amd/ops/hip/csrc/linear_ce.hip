@@ -200,12 +200,17 @@ __device__ __forceinline__ void load8(const Pack& p, const char* src, long c,
   }
 }
 
-// One wave a row, eight values a lane at a time.  Bound by memory: 61,000 fp32
-// rows of 512 into pairs 57 us, 4.4 TB/s read and written.
+// A wave takes one row, or several of fewer than 512 values, eight values a
+// lane at a time.  Bound by memory: 61,000 fp32 rows of 512 into pairs 57 us,
+// 4.4 TB/s read and written.
 template <int PARTS>
 __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
   __shared__ float scratch[PX_BLOCK / WAVE];
-  const int lane = threadIdx.x & 63;
+  // lanes of a row, rows of a wave, this lane's place in its row
+  const int lanes = p.dp > 256 ? 64 : p.dp > 128 ? 32 : p.dp > 64 ? 16 : 8;
+  const int rows = 64 / lanes;
+  const int lane = threadIdx.x & (lanes - 1);
+  const int sub = (threadIdx.x & 63) / lanes;
   const int size = PARTS == 2 ? 4 : 2;
   float scale = 1.f, most = 0.f;
   if (PARTS == 2 && p.top != nullptr) {
@@ -223,8 +228,8 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
       p.sc[1] = 1.f / s;
     }
   }
-  for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < p.rows_out;
-       r += (long)gridDim.x * 4) {
+  for (long r = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows + sub;
+       r < p.rows_out; r += (long)gridDim.x * 4 * rows) {
     bool live = r < p.rows;
     if (p.labels && live) {
       const int64_t y = p.labels[r];
@@ -242,7 +247,7 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
     }
     const char* src = static_cast<const char*>(p.src) + r * p.rs * size;
     if constexpr (PARTS == 1) {
-      for (int c = lane * 8; c < p.dp; c += 512) {
+      for (int c = lane * 8; c < p.dp; c += lanes * 8) {
         s8 u = {};
         if (live && p.eight && c < p.d) {
           u = *reinterpret_cast<const s8*>(src + c * 2);
@@ -262,7 +267,7 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
       if (p.top == nullptr) {
         float t = 0.f;
         if (live) {
-          for (int c = lane * 8; c < p.d; c += 512) {
+          for (int c = lane * 8; c < p.d; c += lanes * 8) {
             float v[8];
             load8(p, src, c, v);
 #pragma unroll
@@ -272,13 +277,13 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
             }
           }
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
+        for (int o = lanes / 2; o > 0; o >>= 1)
+          t = fmaxf(t, __shfl_xor(t, o, 64));
         most = fmaxf(most, t);
         scale = scale_to_half(t);
       }
       if (lane == 0) p.inv[r] = 1.f / scale;
-      for (int c = lane * 8; c < p.dp; c += 512) {
+      for (int c = lane * 8; c < p.dp; c += lanes * 8) {
         float v[8] = {};
         if (live && c < p.d) load8(p, src, c, v);
         s8 h, l;
@@ -522,10 +527,20 @@ __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
     const long y = y0 < 0 ? 0 : (y0 >= p.V ? p.V - 1 : y0);
     float a = 0.f;
     if (live && (WAVES == 1 || wave == 0)) {
-#pragma unroll 4
-      for (int c = lane; c < p.d; c += 64)
-        a += load_as(p.x.p, r * p.x.rs + c * p.x.cs, p.x.type) *
-             load_as(p.w.p, y * p.w.rs + c * p.w.cs, p.w.type);
+      auto dot = [&](auto type) {  // known, so that loads need not wait
+        constexpr int T = decltype(type)::value;
+#pragma unroll 8
+        for (int c = lane; c < p.d; c += 64)
+          a += load_as(p.x.p, r * p.x.rs + c * p.x.cs, T) *
+               load_as(p.w.p, y * p.w.rs + c * p.w.cs, T);
+      };
+      if (p.x.type == 2) {
+        dot(std::integral_constant<int, 2>{});
+      } else if (p.x.type == 1) {
+        dot(std::integral_constant<int, 1>{});
+      } else {
+        dot(std::integral_constant<int, 0>{});
+      }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -813,20 +828,42 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dx_kernel(
       if (f4* p = at(i, j)) *p = acc[i][j];
 }
 
-// dx = 1/S of the slices' sums.  Bound by memory: 32 slices of 999 x 256, 33
-// MB, 11 us.
-__global__ __launch_bounds__(256) void lce_dx_sum_kernel(
+// dx = 1/S of the slices' sums.  GROUPS waves of a workgroup take every
+// GROUPS-th slice each, in order: many slices of few values would be one long
+// chain of loads (185 of 4 x 64: 45 us by one thread each, 4.4 us so).
+// Otherwise bound by memory: 32 of 999 x 256, 33 MB, 8 us.
+template <int GROUPS>
+__global__ __launch_bounds__(GROUPS == 1 ? 256 : 64 * GROUPS)
+void lce_dx_sum_kernel(
     const float* __restrict__ part, int slices, long n, int d, int dp,
     const float* __restrict__ sc, const float* __restrict__ winv,
     void* __restrict__ dx, int type) {
   const float back = sc[1] * (winv ? winv[0] : 1.f);
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n * d;
-       i += (long)gridDim.x * 256) {
+  __shared__ float red[GROUPS][64];
+  constexpr int AT_ONCE = GROUPS == 1 ? 256 : 64;
+  const int group = GROUPS == 1 ? 0 : threadIdx.x >> 6;
+  const int first = GROUPS == 1 ? threadIdx.x : threadIdx.x & 63;
+  for (long i0 = (long)blockIdx.x * AT_ONCE; i0 < n * d;
+       i0 += (long)gridDim.x * AT_ONCE) {
+    const long i = i0 + first;
+    const bool there = i < n * d;
     const long r = i / d;
     const long at = r * dp + (i - r * d);
     float s = 0.f;
-    for (int q = 0; q < slices; ++q) s += part[q * n * dp + at];
-    store_as(dx, i, type, s * back);
+    if (there) {
+#pragma unroll 4
+      for (int q = group; q < slices; q += GROUPS) s += part[q * n * dp + at];
+    }
+    if (GROUPS > 1) {
+      red[group][first] = s;
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g) s += red[g][first];
+      }
+      __syncthreads();
+    }
+    if (there && group == 0) store_as(dx, i, type, s * back);
   }
 }
 
@@ -1403,10 +1440,17 @@ std::vector<at::Tensor> linear_ce_bwd(
       });
     }
     if (want_dx) {
-      lce_dx_sum_kernel<<<px_grid(p.n * p.d), 256, 0, stream>>>(
-          mem.at<float>(o_part), slices, p.n, (int)p.d, (int)p.dp, sc, winv,
-          dx.data_ptr(), p.type);
-      HIP_CHECK_KERNEL();
+      auto launch = [&](auto kernel, int threads, int at_once) {
+        kernel<<<px_grid(p.n * p.d, at_once), threads, 0, stream>>>(
+            mem.at<float>(o_part), slices, p.n, (int)p.d, (int)p.dp, sc,
+            winv, dx.data_ptr(), p.type);
+        HIP_CHECK_KERNEL();
+      };
+      if (slices >= 32) {
+        launch(lce_dx_sum_kernel<8>, 512, 64);
+      } else {
+        launch(lce_dx_sum_kernel<1>, 256, 256);
+      }
     }
   });
   return {dx, dw, db};
