@@ -1089,9 +1089,16 @@ constexpr bool reached() {
 // and 158, 385 and 408
 bool flat(const Plan& p) { return up(p.n, 64) * 8 <= up(p.n, 128) * 7; }
 
+// Fewer 128 x 128 tiles than half of the CUs: 64 x 64.  512 x 1000 x 512
+// forward 23 us, 26 with the larger, in fp32 27 and 36; 1228 x 860 x 896 in
+// fp32 with gradients 110 and 126.
+bool few(const Plan& p) {
+  return !flat(p) && (up(p.n, 128) / 128) * (up(p.v, 128) / 128) < 128;
+}
+
 bool blocked(const Plan& p) {
   // not where 256-row tiles would be empty by more than they gain
-  return p.parts == 1 && !flat(p) &&
+  return p.parts == 1 && !flat(p) && !few(p) &&
          up(p.n, 256) * 100 <= up(p.n, 128) * 115;
 }
 
@@ -1100,6 +1107,8 @@ template <typename F>
 void with_row_tile(const Plan& p, F f) {
   if (flat(p)) {
     f(Flat{}, FlatT{});
+  } else if (few(p)) {
+    f(Small{}, Small{});
   } else if (blocked(p)) {
     f(Logit{}, LogitT{});
   } else if (p.parts == 2) {

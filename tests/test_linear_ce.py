@@ -575,3 +575,14 @@ def test_refused_sizes():
 @pytest.mark.parametrize('n', [128, 130, 192, 193, 256, 320, 321, 440, 449])
 def test_every_tile_of_rows(dtype, n):
     _check(*_inputs(n, 600, 128, dtype, 'cuda', seed=26))
+
+
+@GPU
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n', [193, 256, 320, 350, 385, 512])
+@pytest.mark.parametrize('eps', [0.0, 0.1])
+def test_larger_tiles(dtype, n, eps):
+    """Enough words that the large tiles of rows run, whole and cut."""
+    x, w, b, y = _inputs(n, 8310, 64, dtype, 'cuda', seed=27)
+    y[3:9] = -100
+    _check(x, w, b, y, eps)
