@@ -344,7 +344,7 @@ struct Logits {
 // tiles of words.  2,560 x 793,470 x 512 bf16: 2.17 ms, 0.96 PF; what the
 // product alone does not reach is the exponentials, a quarter of the rate of
 // other instructions, under which only the other workgroup's products run.
-// fp32, 320 rows: 82 us for 61,000 words, 0.73 PF of 16-bit products.
+// fp32, 320 rows: 76 us for 61,000 words, 0.79 PF of 16-bit products.
 template <class C, int XL, int PARTS, bool BF, bool SMOOTH>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
     Logits p, float* __restrict__ part, int vb0, int nblocks, int nmt,
@@ -500,7 +500,8 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 
 // One wave a row joins its partial sums, takes the label's logit as a dot
 // product, and the loss.  WAVES: that many take a row's sums (6,200 of each
-// of 320 rows: 22 us with four, 61 with one).
+// of 320 rows: 22 us with four, 61 with one; 12 since the label's product
+// does not ask for its type at each load).
 template <int WAVES>
 __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
   __shared__ float red[4][3];
