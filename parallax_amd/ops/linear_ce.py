@@ -30,6 +30,10 @@ def _check(inputs, weight, bias, labels, label_smoothing, reduction):
         raise ValueError('linear_cross_entropy: inputs [..., D] and weight '
                          '[V, D] expected, got %s and %s'
                          % (tuple(inputs.shape), tuple(weight.shape)))
+    if not weight.numel():
+        raise ValueError('linear_cross_entropy: at least one word of one '
+                         'value expected, got a weight of %s'
+                         % (tuple(weight.shape),))
     if labels.shape != inputs.shape[:-1]:
         raise ValueError('linear_cross_entropy: labels %s expected, got %s'
                          % (tuple(inputs.shape[:-1]), tuple(labels.shape)))

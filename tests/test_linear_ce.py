@@ -586,3 +586,12 @@ def test_larger_tiles(dtype, n, eps):
     x, w, b, y = _inputs(n, 8310, 64, dtype, 'cuda', seed=27)
     y[3:9] = -100
     _check(x, w, b, y, eps)
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+def test_no_words_are_refused(dev):
+    x, w, b, y = _inputs(5, 7, 4, torch.float32, dev, seed=28)
+    with pytest.raises(ValueError, match='one word'):
+        ops.linear_cross_entropy(x, w[:0], b[:0], y)
+    with pytest.raises(ValueError, match='one word'):
+        ops.linear_cross_entropy(x[:, :0], w[:, :0], b, y)
