@@ -26,6 +26,14 @@ def build(verbose=True):
         [s for s in glob.glob(os.path.join(CSRC, '*.hip'))
          if not s.endswith('_hip.hip')])  # torch-hipify build artifacts
     assert sources, 'no kernel sources found under %s' % CSRC
+    # the compiler's record of included headers does not reach the build of
+    # the kernels: objects older than a header are made anew
+    headers = [os.path.getmtime(h)
+               for h in glob.glob(os.path.join(CSRC, '*.h'))
+               if not h.endswith('_hip.h')]
+    for obj in glob.glob(os.path.join(LIB_DIR, '*.cuda.o')):
+        if os.path.getmtime(obj) < max(headers):
+            os.remove(obj)
     mod = cpp_extension.load(
         name=EXT_NAME,
         sources=sources,
