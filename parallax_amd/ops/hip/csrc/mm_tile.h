@@ -243,12 +243,40 @@ __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
     sb.load(at + C::BM * BK * 2, k0 + t * STEP);
     lbuf = lbuf + 1 == ST ? 0 : lbuf + 1;
   };
-  auto multiply = [&](const s8 (&fa)[C::FM], const s8 (&fb)[C::FN]) {
+  auto multiply = [&](const s8 (&fa)[C::FM], const s8 (&fb)[C::FN],
+                      f4 (&sum)[C::FM][C::FN]) {
 #pragma unroll
     for (int i = 0; i < C::FM; ++i)
 #pragma unroll
       for (int j = 0; j < C::FN; ++j)
-        acc[i][j] = mma<BF>(fb[j], fa[i], acc[i][j]);
+        sum[i][j] = mma<BF>(fb[j], fa[i], sum[i][j]);
+  };
+  // Small tiles have registers to add up what is 2^-12 of the rest apart:
+  // the large sums are then rounded a third as often.  With one fragment a
+  // wave, which waits for loads anyway, each stage's sum goes to the total
+  // by a two-sum, whose error is added up as well.
+  constexpr bool APART = PARTS == 2 && C::FM * C::FN <= 4;
+  constexpr bool EXACT = PARTS == 2 && C::FM * C::FN == 1;
+  f4 low[APART ? C::FM : 1][APART ? C::FN : 1] = {};
+  auto multiply_low = [&](const s8 (&fa)[C::FM], const s8 (&fb)[C::FN]) {
+    if constexpr (APART) {
+      multiply(fa, fb, low);
+    } else {
+      multiply(fa, fb, acc);
+    }
+  };
+  auto stage_of_pairs = [&](auto read_a, auto read_b) {
+#pragma unroll
+    for (int kk = 0; kk < BK / 32; kk += 2) {
+      s8 ah[C::FM], al[C::FM], bh[C::FN], bl[C::FN];
+      read_b(bh, kk);
+      read_a(al, kk + 1);
+      multiply_low(al, bh);
+      read_a(ah, kk);
+      multiply(ah, bh, acc);
+      read_b(bl, kk + 1);
+      multiply_low(ah, bl);
+    }
   };
 
 #pragma unroll
@@ -277,27 +305,30 @@ __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
       for (int j = 0; j < C::FN; ++j)
         f[j] = frag<C::BN, BL, BK>(pb, wn + j * 16, kk, lane);
     };
-    if constexpr (PARTS == 2) {
-#pragma unroll
-      for (int kk = 0; kk < BK / 32; kk += 2) {
-        s8 ah[C::FM], al[C::FM], bh[C::FN], bl[C::FN];
-        read_b(bh, kk);
-        read_a(al, kk + 1);
-        multiply(al, bh);
-        read_a(ah, kk);
-        multiply(ah, bh);
-        read_b(bl, kk + 1);
-        multiply(ah, bl);
-      }
+    if constexpr (EXACT) {
+      const f4 t = acc[0][0];
+      acc[0][0] = f4{0.f, 0.f, 0.f, 0.f};
+      stage_of_pairs(read_a, read_b);
+      const f4 v = acc[0][0], sum = t + v, v1 = sum - t;
+      low[0][0] += (t - (sum - v1)) + (v - v1);
+      acc[0][0] = sum;
+    } else if constexpr (PARTS == 2) {
+      stage_of_pairs(read_a, read_b);
     } else {
 #pragma unroll
       for (int kk = 0; kk < BK / 32; ++kk) {
         s8 fa[C::FM], fb[C::FN];
         read_b(fb, kk);
         read_a(fa, kk);
-        multiply(fa, fb);
+        multiply(fa, fb, acc);
       }
     }
+  }
+  if constexpr (APART) {
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) acc[i][j] += low[i][j];
   }
   barrier();  // the caller may use the LDS
 }

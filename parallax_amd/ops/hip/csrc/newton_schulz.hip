@@ -330,11 +330,14 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
       if (SECOND) {
         const int m = m0 + wm + i * 16 + (lane & 15);
         const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-        v = b * P.four<PARTS == 2>(m, n) + c * v;
-        if (PARTS == 2) {
+        const f4 old = P.four<PARTS == 2>(m, n);
+        if (PARTS == 2) {  // rounded once: the terms are larger than the sum
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (m == n + r) v[r] += a * kScale;
+            v[r] = (float)((double)b * old[r] + (double)c * v[r] +
+                           (m == n + r ? (double)a * kScale : 0.));
+        } else {
+          v = b * old + c * v;
         }
       }
       acc[i][j] = v;
