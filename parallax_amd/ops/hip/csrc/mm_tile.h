@@ -71,6 +71,7 @@ template <int BM_, int BN_, int WM_, int WN_, int BK_, int ST_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int BK = BK_, ST = ST_;
+  static constexpr bool TWO_SUM = false;
   static constexpr int WAVES_M = BM / WM, WAVES_N = BN / WN;
   static constexpr int THREADS = 64 * WAVES_M * WAVES_N;
   static constexpr int FM = WM / 16, FN = WN / 16;
@@ -252,11 +253,10 @@ __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
         sum[i][j] = mma<BF>(fb[j], fa[i], sum[i][j]);
   };
   // Small tiles have registers to add up what is 2^-12 of the rest apart:
-  // the large sums are then rounded a third as often.  With one fragment a
-  // wave, which waits for loads anyway, each stage's sum goes to the total
-  // by a two-sum, whose error is added up as well.
+  // the large sums are then rounded a third as often.  TWO_SUM: each stage's
+  // sum goes to the total by a two-sum, whose error is added up as well.
   constexpr bool APART = PARTS == 2 && C::FM * C::FN <= 4;
-  constexpr bool EXACT = PARTS == 2 && C::FM * C::FN == 1;
+  constexpr bool EXACT = PARTS == 2 && C::TWO_SUM;
   f4 low[APART ? C::FM : 1][APART ? C::FN : 1] = {};
   auto multiply_low = [&](const s8 (&fa)[C::FM], const s8 (&fb)[C::FN]) {
     if constexpr (APART) {

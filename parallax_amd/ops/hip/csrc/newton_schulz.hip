@@ -478,6 +478,12 @@ using Mid = Tile<128, 128, 64, 32, 64, 2>;
 // with Mid, 6.4 with Small, 4.7 with Tiny.
 using Small = Tile<64, 64, 32, 16, 128, 2>;
 using Tiny = Tile<32, 32, 16, 16, 128, 4>;
+// fp32 results of few rows: with a two-sum a stage they are as near to 64
+// bits as fp32 products (11 x 8 x 687: 1.1e-6, 1.4e-6 without), for 4% of
+// the time
+struct TinyExact : Tiny {
+  static constexpr bool TWO_SUM = true;
+};
 
 template <typename K>
 void allow_lds(K kernel, int bytes) {
@@ -499,11 +505,13 @@ void allow_lds(K kernel, int bytes) {
 
 // f(tile) for a tile size of 32, 64 or 128
 template <typename F>
-void with_tile(int size, F f) {
+void with_tile(int size, bool exact, F f) {
   if (size == 128) {
     f(Mid{});
   } else if (size == 64) {
     f(Small{});
+  } else if (exact) {
+    f(TinyExact{});
   } else {
     f(Tiny{});
   }
@@ -621,7 +629,7 @@ void run(const Batch& batch, int type, long count, long small, long large,
       constexpr bool SECOND = decltype(second)::value;
       const Cut& way = SECOND ? square : wide;
       const int tiles = mp / way.tile, cut = way.cuts;
-      with_tile(way.tile, [&](auto t) {
+      with_tile(way.tile, p.exact, [&](auto t) {
         using C = decltype(t);
         auto launch = [&](auto kernel, int lds, int n) {
           allow_lds(kernel, lds);
@@ -645,7 +653,7 @@ void run(const Batch& batch, int type, long count, long small, long large,
     };
     symmetric(std::false_type{}, X, np, A);
     symmetric(std::true_type{}, A, mp, B);
-    with_tile(full, [&](auto t) {
+    with_tile(full, p.exact, [&](auto t) {
       using C = decltype(t);
       auto launch = [&](auto kernel) {
         constexpr int lds = C::template lds<2>();
