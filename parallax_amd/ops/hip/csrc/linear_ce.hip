@@ -1273,8 +1273,9 @@ std::vector<at::Tensor> linear_ce_bwd(
   const int xtop = two ? pack_blocks(p.np) : 0;
   const int ntop = (int)(saved.numel() - p.n - 1) - xtop;
 
-  // words for which the tiles of dw fill the chip's 256 CUs once
-  const long wave_of_words = 256 * 256 / ((p.dp + 255) / 256);
+  // words for which the tiles of dw fill the chip's 256 CUs once; a piece is
+  // whole tiles of 256, as G and the words laid out are written by such
+  const long wave_of_words = 256 * 256 / ((p.dp + 255) / 256) / 256 * 256;
   long piece = kPieceBytes / (p.np * 2 * p.parts);
   piece = piece >= wave_of_words ? piece / wave_of_words * wave_of_words
                                  : piece / 256 * 256;
@@ -1283,6 +1284,7 @@ std::vector<at::Tensor> linear_ce_bwd(
   // a piece of w ends before its byte 2^31, the largest offset there is
   const long w_ld = p.w_direct ? w.stride(0) : p.dp * p.parts;
   piece = std::max(256L, std::min(piece, ((1L << 30) - 1) / w_ld / 256 * 256));
+  TORCH_CHECK(piece % 256 == 0, "linear_ce_bwd: pieces of whole tiles");
   const int ldg = (int)p.np * p.parts;
   // dx: few tiles and a long k, so k is cut until the chip is full
   const int dx_tile = p.n > 128 && p.dp >= 128 ? 128 : 64;

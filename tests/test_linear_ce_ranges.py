@@ -1,0 +1,85 @@
+"""linear_cross_entropy over sizes and values that a small case does not
+reach, against its definition in 64 bits on the same device.
+
+Bounds.  With u half a step of the results' type, ug one of G's and
+e = 2^-24: a logit is off by dz = (D + 32) e (|x| |w|^T + |b|), so the
+logarithm of a probability by dz, the largest dz of its row (for lse) and the
+rounding of exp2's argument, 3 e |z - lse| + 4 e; lse adds V e for the sum of
+V positive terms.  G is off by that times p and by ug |G|, the products by
+the sums of that and by (K + 32) e of the magnitudes of their K terms, and
+the results are rounded by u.
+"""
+
+import pytest
+import torch
+
+from parallax_amd import ops
+
+E = 2.0 ** -24
+GPU = pytest.mark.gpu
+DEVICES = ['cpu', pytest.param('cuda', marks=GPU)]
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11,
+     torch.float32: 2.0 ** -24}
+
+
+def _exact(x, w, b, y, up):
+    """{name: (value, bound)} of dx, dw and db for the rows' upstream
+    gradients ``up``."""
+    u = U[x.dtype]
+    ug = u if x.dtype != torch.float32 else 2.0 ** -22
+    x, w, up = x.detach().double(), w.detach().double(), up.double()
+    n, d = x.shape
+    v = w.shape[0]
+    z = x @ w.t()
+    dz = x.abs() @ w.abs().t()
+    if b is not None:
+        z += b.detach().double()
+        dz += b.detach().double().abs()
+    dz *= (d + 32) * E
+    z -= torch.logsumexp(z, 1, keepdim=True)
+    rel = dz + (3 * z.abs() + 4) * E
+    rel += dz.amax(1, keepdim=True) + v * E
+    p = z.exp()
+    g = up[:, None]
+    G = p * g
+    dG = g.abs() * p * (rel + 4 * E)
+    rows = torch.arange(n, device=x.device)
+    G[rows, y] -= up
+    dG[rows, y] += 4 * E * up.abs()
+    dG += ug * G.abs()
+
+    def out(val, mag, err, k):
+        return val, err + (k + 32) * E * mag + u * val.abs() + 1e-30
+
+    A = G.abs()
+    return dict(dx=out(G @ w, A @ w.abs(), dG @ w.abs(), v),
+                dw=out(G.t() @ x, A.t() @ x.abs(), dG.t() @ x.abs(), n),
+                db=out(G.sum(0), A.sum(0), dG.sum(0), n))
+
+
+def _inside(got, want, what):
+    val, tol = want
+    off = (got.double() - val).abs()
+    assert bool((off <= tol).all()), (what, float((off / tol).max()))
+
+
+@GPU
+@pytest.mark.parametrize('asked', [(0, 1, 2), (0,), (1,)])
+@pytest.mark.parametrize('n,v,d', [(4000, 22600, 640), (4000, 21800, 640)])
+def test_widths_that_do_not_divide_a_piece(n, v, d, asked):
+    """Rows of 640 values are three tiles of 256, of which 256 CUs hold
+    21,845 words' worth, no multiple of a tile: the pieces of the vocabulary
+    have to be, whether there are several or one."""
+    g = torch.Generator(device='cuda').manual_seed(0)
+    x = torch.randn(n, d, generator=g, device='cuda').bfloat16()
+    w = (torch.randn(v, d, generator=g, device='cuda') * d ** -0.5) \
+        .bfloat16()
+    b = torch.randn(v, generator=g, device='cuda').bfloat16()
+    y = torch.randint(0, v, (n,), generator=g, device='cuda')
+    leaf = [t.clone().requires_grad_(i in asked)
+            for i, t in enumerate((x, w, b))]
+    ops.linear_cross_entropy(*leaf, y, reduction='sum').backward()
+    want = _exact(x, w, b, y, torch.ones(n, device='cuda'))
+    for i, name in enumerate(('dx', 'dw', 'db')):
+        if i in asked:
+            _inside(leaf[i].grad, want[name], name)
