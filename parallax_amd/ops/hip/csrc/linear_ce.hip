@@ -22,9 +22,15 @@
 // Types.  bf16 and fp16 inputs are multiplied as they are; G is rounded to
 // the same type once, relative to the largest |g|, and the results are
 // scaled back (at most 2^-8 or 2^-11 of each value, as the final rounding of
-// the gradients is).  fp32 inputs are split into two fp16 parts (22 bits) after
-// a scaling by a power of two, and so is G: three products in the place of
-// one.
+// the gradients is).  fp32 inputs are split into two fp16 parts after a
+// scaling by a power of two, and so is G: three products in the place of one.
+// Two parts hold 22 bits of values down to 2^-17 of the largest that shares
+// their scale, and 2^-39 of that of smaller ones, so scales have to follow
+// the values: x has one a row, and G is made in fp32 and split twice, for dw
+// with one a word (the words of a large vocabulary differ by 1e12 and more in
+// probability, and each has a gradient of its own) and for dx with one a row.
+// w has one a row in the forward and a single one in the backward: dx is
+// exact to 2^-38 of the row's |g| max |w| where its values are below that.
 //
 // Rows whose label is ignored are read as zeros, so what lies in them (a
 // padded batch's garbage, NaN) reaches no gradient.
@@ -124,11 +130,11 @@ __device__ __forceinline__ void store_as(void* p, long i, int type, float v) {
 // 2^k that brings `top` into [2^13, 2^14); 1 where there is nothing to scale
 __device__ __forceinline__ float scale_to_half(float top) {
   if (!(top > 0.f) || !(top < INFINITY)) return 1.f;
-  int e;
-  frexpf(top, &e);  // top in [2^(e-1), 2^e)
-  e = 14 - e;
-  e = e < -120 ? -120 : (e > 120 ? 120 : e);
-  return ldexpf(1.f, e);
+  // top in [2^(e - 127), 2^(e - 126)), or below 2^-126 where e = 0
+  const int e = __float_as_uint(top) >> 23;
+  int k = 13 - (e - 127);
+  k = k < -120 ? -120 : (k > 120 ? 120 : k);
+  return __uint_as_float((unsigned)(k + 127) << 23);
 }
 
 // S for G: bf16 and fp16 rows of the largest |g| get -1 or -2^13 at a label
@@ -613,7 +619,8 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(
 
 // --- backward ---------------------------------------------------------------
 
-// G of one piece, transposed: [words][ldg], zeros outside the matrix.  The
+// G of one piece, transposed: [words][ldg], zeros outside the matrix, in the
+// inputs' 16 bits or (PARTS = 2) in fp32 for lce_split_kernel.  The
 // words are the tile's m: a lane holds four neighbouring rows of one word,
 // sums over the rows stay in it, and dw reads G k-contiguous.
 // DB: sums of each tile of rows into dbp[row tile][..], or as they are into
@@ -622,7 +629,7 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(
 template <class C, int XL, int PARTS, bool BF, bool DB>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     Logits p, Rows rows, const float* __restrict__ sc, long V, long v0,
-    float eps, ushort* __restrict__ G, int ldg, float* __restrict__ dbp,
+    float eps, void* __restrict__ G, int ldg, float* __restrict__ dbp,
     long db_ld, void* __restrict__ db, int db_type, int nvt, int nrt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int bid = die_contiguous(blockIdx.x, nvt * nrt);
@@ -642,8 +649,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     const int v = w0 + i * 16;
     add[i] = p.bias.one(v, p.vp);
     ws[i] = kLog2e;
-    // one scale to undo for all rows
-    if (PARTS == 2) ws[i] *= (v < p.vp ? p.winv[v] : 0.f) * p.xinv[0];
+    if (PARTS == 2) ws[i] *= v < p.vp ? p.winv[v] : 0.f;
     sum[i] = 0.f;
   }
 #pragma unroll
@@ -653,13 +659,16 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     const f4 l = *reinterpret_cast<const f4*>(rows.l + n);
     const f4 g = S * *reinterpret_cast<const f4*>(rows.g + n);
     const int4 y = *reinterpret_cast<const int4*>(rows.y + n);
+    f4 xs = {1.f, 1.f, 1.f, 1.f};
+    if (PARTS == 2) xs = *reinterpret_cast<const f4*>(p.xinv + n);
 #pragma unroll
     for (int i = 0; i < C::FM; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        acc[i][j][r] =
-            fmaf(exp2_fast(fmaf(acc[i][j][r], ws[i], add[i] - l[r])), g[r],
-                 -uni * g[r]);
+      for (int r = 0; r < 4; ++r) {
+        const float z = PARTS == 2 ? acc[i][j][r] * xs[r] : acc[i][j][r];
+        acc[i][j][r] = fmaf(exp2_fast(fmaf(z, ws[i], add[i] - l[r])), g[r],
+                            -uni * g[r]);
+      }
     // the label's word: in few tiles, so not a comparison for each value
     const int at[4] = {y.x, y.y, y.z, y.w};
     const int first = (int)v0 + m0 + wm;
@@ -683,11 +692,11 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
       for (int j = 0; j < C::FN; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
     }
   if constexpr (PARTS == 2) {
-    store_pairs<C>(smem, G + (long)m0 * ldg + n0 * 2, ldg,
-                   [&](int i, int j) { return acc[i][j]; });
+    store_floats<C>(smem, static_cast<float*>(G) + (long)m0 * ldg + n0, ldg,
+                    [&](int i, int j) { return acc[i][j]; });
   } else {
-    store_tile<C>(smem, G + (long)m0 * ldg + n0, ldg, C::BM, C::BN,
-                  [&](int i, int j) {
+    store_tile<C>(smem, static_cast<ushort*>(G) + (long)m0 * ldg + n0, ldg,
+                  C::BM, C::BN, [&](int i, int j) {
       const f4 v = acc[i][j];
       if (BF)
         return make_ushort4(bf16_bits(v[0]), bf16_bits(v[1]),
@@ -727,6 +736,72 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
   }
 }
 
+// fp32 G in pairs of parts: for dx (Gx) scaled by a power of two for each row,
+// for dw in its place by one for each word, whose reciprocal goes to tinv.
+// The rows of x have scales of their own, 1 / xinv, which dw sums over: they
+// are undone here.  A wave (WIDE: a workgroup) takes a word; in its place, a
+// wave has read what it writes over, 1 KiB, before.  cols: of the np, those
+// that G has been made for.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void lce_split_kernel(
+    float* __restrict__ G, int np, int cols, int words,
+    const float* __restrict__ g,
+    const float* __restrict__ sc, const float* __restrict__ xinv,
+    ushort* __restrict__ Gx, float* __restrict__ tinv) {
+  __shared__ float scratch[PX_BLOCK / WAVE];
+  constexpr int STEP = WIDE ? 1024 : 256;
+  const int v = WIDE ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int first = (WIDE ? threadIdx.x : threadIdx.x & 63) * 4;
+  if (v >= words) return;  // WIDE: never
+  float* row = G + (long)v * np;
+  float scale = 1.f;
+  if (tinv) {
+    float top = 0.f;
+#pragma unroll 4
+    for (int n = first; n < cols; n += STEP) {
+      const f4 a = *reinterpret_cast<const f4*>(row + n);
+      const f4 b = *reinterpret_cast<const f4*>(xinv + n);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(a[r] * b[r]));
+    }
+    if (WIDE) {
+      top = block_reduce_max(top, scratch);
+    } else {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1)
+        top = fmaxf(top, __shfl_xor(top, o, 64));
+    }
+    scale = scale_to_half(top);
+    if (first == 0) tinv[v] = 1.f / scale;
+  }
+  const float S = sc[0];
+#pragma unroll 2
+  for (int n = first; n < cols; n += STEP) {
+    const f4 a = *reinterpret_cast<const f4*>(row + n);
+    const long at = (long)v * np * 2 + (n >> 5) * 64 + (n & 31);
+    ushort h[4], l[4];
+    if (Gx) {
+      const f4 gn = *reinterpret_cast<const f4*>(g + n);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        split(a[r] * scale_to_half(fabsf(S * gn[r])), h[r], l[r]);
+      *reinterpret_cast<ushort4*>(Gx + at) =
+          make_ushort4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<ushort4*>(Gx + at + 32) =
+          make_ushort4(l[0], l[1], l[2], l[3]);
+    }
+    if (tinv) {
+      const f4 b = *reinterpret_cast<const f4*>(xinv + n);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) split(a[r] * b[r] * scale, h[r], l[r]);
+      ushort* to = reinterpret_cast<ushort*>(G) + at;
+      *reinterpret_cast<ushort4*>(to) = make_ushort4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<ushort4*>(to + 32) =
+          make_ushort4(l[0], l[1], l[2], l[3]);
+    }
+  }
+}
+
 // db from the sums of the tiles of rows, in their order (10 of 793,470 words:
 // 13 us, 2.4 TB/s).
 __global__ __launch_bounds__(256) void lce_db_kernel(
@@ -740,11 +815,12 @@ __global__ __launch_bounds__(256) void lce_db_kernel(
 }
 
 // dw[v, :] = 1/S sum_n G[n, v] x[n, :]  (x k-strided).  32,768 x 512 over
-// 2,560 rows bf16: 85 us, 1.01 PF.
+// 2,560 rows bf16: 85 us, 1.01 PF.  tinv: what is left to undo of a word's
+// scale (PARTS = 2).
 template <class C, int PARTS, bool BF>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
     Operand G, Operand x, int kn, const float* __restrict__ sc,
-    const float* __restrict__ xinv, void* __restrict__ dw, int type, int vp,
+    const float* __restrict__ tinv, void* __restrict__ dw, int type, int vp,
     int d, int nmt, int nnt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int bid = die_contiguous(blockIdx.x, nmt * nnt);
@@ -755,7 +831,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
-  const float back = sc[1] * (PARTS == 2 ? xinv[0] : 1.f);
+  const float back = sc[1];
   if (type != 2 && (d & 7) == 0) {
     store_tile<C>(smem, static_cast<ushort*>(dw) + (long)m0 * d + n0, d,
                   vp - m0, d - n0, [&](int i, int j) {
@@ -772,17 +848,18 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
   for (int i = 0; i < C::FM; ++i) {
     const int v = m0 + wm + i * 16 + (lane & 15);
     if (v >= vp) continue;
+    const float word = PARTS == 2 ? tinv[v] : 1.f;
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) {
       const int c = n0 + wn + j * 16 + (lane >> 4) * 4;
       const long at = (long)v * d + c;
+      const f4 val = acc[i][j] * word * back;
       if (type == 2 && c + 4 <= d && (d & 3) == 0) {
-        *reinterpret_cast<f4*>(static_cast<float*>(dw) + at) =
-            acc[i][j] * back;
+        *reinterpret_cast<f4*>(static_cast<float*>(dw) + at) = val;
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (c + r < d) store_as(dw, at + r, type, acc[i][j][r] * back);
+          if (c + r < d) store_as(dw, at + r, type, val[r]);
       }
     }
   }
@@ -829,7 +906,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dx_kernel(
       if (f4* p = at(i, j)) *p = acc[i][j];
 }
 
-// dx = 1/S of the slices' sums.  GROUPS waves of a workgroup take every
+// dx = 1/S of the slices' sums, and (fp32: winv) what the scales of w and of
+// the row of G leave to undo.  GROUPS waves of a workgroup take every
 // GROUPS-th slice each, in order: many slices of few values would be one long
 // chain of loads (185 of 4 x 64: 45 us by one thread each, 4.4 us so).
 // Otherwise bound by memory: 32 of 999 x 256, 33 MB, 8 us.
@@ -838,8 +916,7 @@ __global__ __launch_bounds__(GROUPS == 1 ? 256 : 64 * GROUPS)
 void lce_dx_sum_kernel(
     const float* __restrict__ part, int slices, long n, int d, int dp,
     const float* __restrict__ sc, const float* __restrict__ winv,
-    void* __restrict__ dx, int type) {
-  const float back = sc[1] * (winv ? winv[0] : 1.f);
+    const float* __restrict__ g, void* __restrict__ dx, int type) {
   __shared__ float red[GROUPS][64];
   constexpr int AT_ONCE = GROUPS == 1 ? 256 : 64;
   const int group = GROUPS == 1 ? 0 : threadIdx.x >> 6;
@@ -864,7 +941,10 @@ void lce_dx_sum_kernel(
       }
       __syncthreads();
     }
-    if (there && group == 0) store_as(dx, i, type, s * back);
+    if (there && group == 0) {
+      if (winv) s = s / scale_to_half(fabsf(sc[0] * g[r])) * winv[0];
+      store_as(dx, i, type, s * sc[1]);
+    }
   }
 }
 
@@ -1122,7 +1202,7 @@ void with_row_tile(const Plan& p, F f) {
 }  // namespace
 
 // {loss (scalar or [N]), what the backward needs: lse [N], the count, and
-// (fp32) the largest |w| and |x| of blocks}
+// (fp32) the largest |w| of blocks}
 std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
                                       const at::Tensor& w,
                                       const c10::optional<at::Tensor>& bias,
@@ -1142,8 +1222,7 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
   const int wblocks = pack_blocks(p.w_rows);
   const long ntop = p.parts == 2 ? pieces * wblocks : 0;
   auto out = reduction == 0 ? at::empty({p.n}, f32) : at::empty({}, f32);
-  const long xtop = p.parts == 2 ? pack_blocks(p.np) : 0;
-  auto saved = at::empty({p.n + 1 + ntop + xtop}, f32);
+  auto saved = at::empty({p.n + 1 + ntop}, f32);
   float* lse = saved.data_ptr<float>();
   float* tops = lse + p.n + 1;
 
@@ -1175,7 +1254,6 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
     kx.labels = lab;
     kx.ignore = ignore;
     kx.inv = mem.at<float>(o_xinv);
-    if (p.parts == 2) kx.bmax = tops + ntop;
     pack(kx, stream);
     for (long i = 0; i < pieces; ++i) {
       const long v0 = i * piece, vp = std::min(piece, p.v - v0);
@@ -1270,13 +1348,13 @@ std::vector<at::Tensor> linear_ce_bwd(
   const bool two = p.parts == 2, blk = blocked(p);
   const float* lse = saved.data_ptr<float>();
   const float* tops = lse + p.n + 1;
-  const int xtop = two ? pack_blocks(p.np) : 0;
-  const int ntop = (int)(saved.numel() - p.n - 1) - xtop;
+  const int ntop = (int)(saved.numel() - p.n - 1);
 
   // words for which the tiles of dw fill the chip's 256 CUs once; a piece is
   // whole tiles of 256, as G and the words laid out are written by such
   const long wave_of_words = 256 * 256 / ((p.dp + 255) / 256) / 256 * 256;
-  long piece = kPieceBytes / (p.np * 2 * p.parts);
+  // fp32: G of dw and that of dx
+  long piece = kPieceBytes / (p.np * (two ? 8 : 2));
   piece = piece >= wave_of_words ? piece / wave_of_words * wave_of_words
                                  : piece / 256 * 256;
   piece = std::max(256L, std::min(piece, up(p.v, 256)));
@@ -1314,6 +1392,8 @@ std::vector<at::Tensor> linear_ce_bwd(
                                                  : piece * p.dp * p.parts);
     const auto o_winv = mem.take<float>(two ? piece : 0);
     const auto o_G = mem.take<ushort>(piece * ldg);
+    const auto o_Gx = mem.take<ushort>(two && want_dx ? piece * ldg : 0);
+    const auto o_tinv = mem.take<float>(two ? piece : 0);
     const auto o_part =
         mem.take<float>(want_dx ? slices * p.n * p.dp : 0);
     const auto o_dbp = mem.take<float>(want_db && nrt > 1 ? nrt * db_ld : 0);
@@ -1323,10 +1403,6 @@ std::vector<at::Tensor> linear_ce_bwd(
     kx.labels = lab;
     kx.ignore = ignore;
     kx.inv = mem.at<float>(o_xinv);
-    if (two) {  // one scale for all rows, as the rows are summed over
-      kx.top = tops + ntop;
-      kx.ntop = xtop;
-    }
     if (blk) kx.blocks = mem.at<ushort>(o_xblk);
     float* row = mem.at<float>(o_rows);
     kx.row = Rows{row, row + p.np, reinterpret_cast<int*>(row + 2 * p.np)};
@@ -1344,6 +1420,8 @@ std::vector<at::Tensor> linear_ce_bwd(
       HIP_CHECK_KERNEL();
     }
     auto* G = mem.at<ushort>(o_G);
+    auto* Gx = two ? mem.at<ushort>(o_Gx) : G;
+    float* tinv = two && want_dw ? mem.at<float>(o_tinv) : nullptr;
     const float* sc = kx.sc;
     const float* xinv = two ? kx.inv : nullptr;
     const float* winv = two ? mem.at<float>(o_winv) : nullptr;
@@ -1384,7 +1462,8 @@ std::vector<at::Tensor> linear_ce_bwd(
             constexpr int lds = R::template lds<PARTS>();
             allow_lds(kernel, lds);
             kernel<<<nvt * nrt, R::THREADS, lds, stream>>>(
-                q, kx.row, sc, p.v, v0, eps, G, ldg, dbp, db_ld, db_at,
+                q, kx.row, sc, p.v, v0, eps, G, ldg / PARTS, dbp, db_ld,
+                db_at,
                 want_db ? type_code(db) : 0, nvt, nrt);
             HIP_CHECK_KERNEL();
           };
@@ -1402,8 +1481,23 @@ std::vector<at::Tensor> linear_ce_bwd(
             HIP_CHECK_KERNEL();
           }
         }
+        if (two && (want_dx || want_dw)) {
+          const int words = (int)up(vp, 64);  // as many as are read
+          auto launch = [&](auto kernel, int blocks) {
+            kernel<<<blocks, 256, 0, stream>>>(
+                reinterpret_cast<float*>(G), (int)p.np, nrt * R::BN, words,
+                kx.row.g, sc, xinv, want_dx ? Gx : nullptr, tinv);
+            HIP_CHECK_KERNEL();
+          };
+          if (p.np > 4096) {
+            launch(lce_split_kernel<true>, words);
+          } else {
+            launch(lce_split_kernel<false>, words / 4);
+          }
+        }
         // as rows of words for dw, as columns of rows for dx
         const Operand g = operand(G, up(vp, 64), ldg, p.np);
+        const Operand gx = operand(Gx, up(vp, 64), ldg, p.np);
         if (want_dw) {
           auto run = [&](auto tile) {
             using C = decltype(tile);
@@ -1413,7 +1507,7 @@ std::vector<at::Tensor> linear_ce_bwd(
             constexpr int lds = C::template lds<1>();
             allow_lds(kernel, lds);
             kernel<<<mt * nt, C::THREADS, lds, stream>>>(
-                g, xr, (int)up(p.n, 64), sc, xinv,
+                g, xr, (int)up(p.n, 64), sc, tinv,
                 static_cast<char*>(dw.data_ptr()) +
                     v0 * p.d * dw.element_size(),
                 p.type, (int)vp, (int)p.d, mt, nt);
@@ -1439,7 +1533,7 @@ std::vector<at::Tensor> linear_ce_bwd(
             constexpr int lds = C::template lds<1>();
             allow_lds(kernel, lds);
             kernel<<<mt * nt * slices, C::THREADS, lds, stream>>>(
-                g, q.w, kv, kslice, mem.at<float>(o_part), (int)p.n,
+                gx, q.w, kv, kslice, mem.at<float>(o_part), (int)p.n,
                 (int)p.dp, v0 == 0, mt, nt, slices);
             HIP_CHECK_KERNEL();
           };
@@ -1455,7 +1549,7 @@ std::vector<at::Tensor> linear_ce_bwd(
       auto launch = [&](auto kernel, int threads, int at_once) {
         kernel<<<px_grid(p.n * p.d, at_once), threads, 0, stream>>>(
             mem.at<float>(o_part), slices, p.n, (int)p.d, (int)p.dp, sc,
-            winv, dx.data_ptr(), p.type);
+            winv, kx.row.g, dx.data_ptr(), p.type);
         HIP_CHECK_KERNEL();
       };
       if (slices >= 32) {

@@ -421,6 +421,37 @@ __device__ __forceinline__ void store_pairs(char* lds, ushort* out, long ld,
   }
 }
 
+// The same for values in fp32.
+template <class C, typename F>
+__device__ __forceinline__ void store_floats(char* lds, float* out, long ld,
+                                             F value) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int wm = (wave / C::WAVES_N) * C::WM;
+  const int wn = (wave % C::WAVES_N) * C::WN;
+  constexpr int HALF = C::BM / C::PAIR_GOES, PER_ROW = C::BN / 4;
+#pragma unroll
+  for (int go = 0; go < C::PAIR_GOES; ++go) {
+    if (go) __syncthreads();
+    if (wm / HALF == go) {
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j)
+          *reinterpret_cast<f4*>(
+              lds + (wm % HALF + i * 16 + (lane & 15)) * C::PAIR_ROW +
+              (wn + j * 16 + (lane >> 4) * 4) * 4) = value(i, j);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int c = threadIdx.x; c < HALF * PER_ROW; c += C::THREADS) {
+      const int r = c / PER_ROW, q = (c % PER_ROW) * 4;
+      *reinterpret_cast<f4*>(out + (go * HALF + r) * ld + q) =
+          *reinterpret_cast<const f4*>(lds + r * C::PAIR_ROW + q * 4);
+    }
+  }
+}
+
 // Spreads a flat block id over the 8 dies so that each die works on one
 // contiguous range of tiles: neighbours then share operands in its L2.
 __device__ __forceinline__ int die_contiguous(int bid, int n) {

@@ -83,3 +83,59 @@ def test_widths_that_do_not_divide_a_piece(n, v, d, asked):
     for i, name in enumerate(('dx', 'dw', 'db')):
         if i in asked:
             _inside(leaf[i].grad, want[name], name)
+
+
+def _spread(dev, n=300, v=3000, d=96, seed=1):
+    """Words whose probabilities go from 1e-1 to 1e-16."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, d, generator=g)
+    w = torch.randn(v, d, generator=g) * d ** -0.5
+    b = -30.0 * torch.rand(v, generator=g)
+    y = torch.randint(0, v, (n,), generator=g)
+    b[y] = b[y] / 4
+    return [t.to(dev) for t in (x, w, b, y)]
+
+
+def _gradients_inside(x, w, b, y, up):
+    leaf = [t.clone().requires_grad_() for t in (x, w, b)]
+    ops.linear_cross_entropy(*leaf, y, reduction='none').backward(up)
+    want = _exact(x, w, b, y, up)
+    for t, name in zip(leaf, ('dx', 'dw', 'db')):
+        _inside(t.grad, want[name], name)
+    return want
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('n', [5, 300, 5000])
+def test_fp32_words_of_tiny_probability(dev, n):
+    """Each word's gradient is as exact as fp32 values are, however rare the
+    word: _exact's bounds are relative to the word's own terms."""
+    x, w, b, y = _spread(dev, n=n)
+    up = torch.ones(n, device=dev)
+    dw = _gradients_inside(x, w, b, y, up)['dw'][0]
+    size = dw.norm(dim=1)
+    assert float(size.min()) < 1e-11 * float(size.max())
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+def test_fp32_rows_of_tiny_gradient(dev):
+    """Rows whose upstream gradients differ by 1e15."""
+    x, w, b, y = _spread(dev, seed=2)
+    up = 10.0 ** torch.linspace(-12, 3, 300, device=dev)
+    _gradients_inside(x, w, b, y, up)
+    up[::3] = 0.0
+    _gradients_inside(x, w, b, y, -up)
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+def test_fp32_rows_of_tiny_inputs(dev):
+    """A word that only rows of tiny inputs make likely has a gradient as
+    exact as the others'."""
+    x, w, b, y = _spread(dev, seed=3)
+    x[:150] *= 1e-7
+    y[:150] = torch.arange(150, device=dev) + 2000
+    y[150:] %= 2000
+    b[2000:2150] = -30.0
+    dw = _gradients_inside(x, w, b, y, torch.ones(300, device=dev))['dw'][0]
+    size = dw.norm(dim=1)
+    assert float(size[2000:2150].max()) < 1e-5 * float(size[:2000].max())
