@@ -50,11 +50,13 @@ def _check(inputs, weight, bias, labels, label_smoothing, reduction):
 
 
 def _plain(x, weight, bias, labels, ignore_index, smoothing, reduction):
-    logits = x.float() @ weight.float().t()
+    live = labels != ignore_index
+    # a product with what ignored rows hold would carry it into the gradients
+    x = torch.where(live[:, None], x.float(), 0.0)
+    logits = x @ weight.float().t()
     if bias is not None:
         logits = logits + bias.float()
     # labels outside the vocabulary go to its nearest end, as on the GPU
-    live = labels != ignore_index
     y = torch.where(live, labels.clamp(0, weight.shape[0] - 1), 0)
     lse = torch.logsumexp(logits, 1)
     losses = lse - (1 - smoothing) * logits.gather(1, y[:, None])[:, 0]

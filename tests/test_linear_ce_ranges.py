@@ -139,3 +139,29 @@ def test_fp32_rows_of_tiny_inputs(dev):
     dw = _gradients_inside(x, w, b, y, torch.ones(300, device=dev))['dw'][0]
     size = dw.norm(dim=1)
     assert float(size[2000:2150].max()) < 1e-5 * float(size[:2000].max())
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+@pytest.mark.parametrize('ignore', [-100, 7])
+def test_what_ignored_rows_hold_is_not_read(dev, reduction, ignore):
+    """NaN and infinities in the rows of a padded batch, whatever the label
+    that marks them."""
+    x, w, b, y = _spread(dev, n=40, v=200, d=24, seed=4)
+    y[y == 7] = 8
+    y[::3] = ignore
+    bad = x.clone()
+    bad[::3] = float('nan')
+    bad[3] = float('inf')
+    bad[6, 5] = -float('inf')
+    outs = []
+    for t in (x, bad):
+        leaf = [s.clone().requires_grad_() for s in (t, w, b)]
+        loss = ops.linear_cross_entropy(*leaf, y, reduction=reduction,
+                                        ignore_index=ignore,
+                                        label_smoothing=0.1)
+        loss.sum().backward()
+        outs.append([loss.detach()] + [s.grad for s in leaf])
+    for p, q in zip(*outs):
+        assert torch.isfinite(p).all() and torch.equal(p, q)
+    assert not outs[1][1][::3].any() and outs[1][1][1::3].any()
