@@ -494,7 +494,10 @@ class Muon(Adam):
     for the matrices: parameters of two or more dimensions (a convolution
     is [out, in kh kw]) in groups with ``muon=True``.  Vectors, sparse rows
     and groups with ``muon=False`` (embeddings, heads) take Adam with
-    ``adam_lr`` and no weight decay.  Matrices of about one size go
+    ``adam_lr`` and no weight decay.  A schedule that sets a group's ``lr``
+    reaches them too: Adam's rate is ``adam_lr`` times what ``lr`` is of
+    ``base_lr``, its value when the group was made (``adam_lr`` as it is
+    where that was 0).  Matrices of about one size go
     through the products as one batch.  fp32 parameters get products in 22
     bits, bf16 ones with fp32 masters what bf16's rounding can show."""
 
@@ -516,6 +519,22 @@ class Muon(Adam):
             for group in self.param_groups:
                 group.setdefault(k, v)
 
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        group.setdefault('base_lr', group['lr'])
+
+    def load_state_dict(self, state_dict):
+        base = [group['base_lr'] for group in self.param_groups]
+        super().load_state_dict(state_dict)
+        for group, lr in zip(self.param_groups, base):
+            group.setdefault('base_lr', lr)
+
+    @staticmethod
+    def _adam_lr(group):
+        base = group['base_lr']
+        return group['adam_lr'] * (group['lr'] / base if base else 1.0)
+
     def _dense_step(self, params, grads, group):
         mats, rest = [], []
         for p, g in zip(params, grads):
@@ -525,7 +544,7 @@ class Muon(Adam):
                 rest.append((p, g))
         if rest:
             self._adam_step([p for p, _ in rest], [g for _, g in rest],
-                            group, group['adam_lr'], 0.0)
+                            group, self._adam_lr(group), 0.0)
         # one batch for each type, device and size: the products fill
         # matrices up to multiples of 128 with zeros, either way round
         batches = {}
@@ -594,4 +613,4 @@ class Muon(Adam):
                         nvalid=None):
         group = group or self.group_of(param)
         super().sparse_row_step(param, ids, grad_rows,
-                                dict(group, lr=group['adam_lr']), nvalid)
+                                dict(group, lr=self._adam_lr(group)), nvalid)
