@@ -18,11 +18,14 @@
 // 8 and 5 over the steps behind the first to fifth, so one-part products
 // cost more than their 2^-12.  Emulated in 64 bits over gaussian, low-rank,
 // badly scaled and orthogonal matrices, relative to the result's norm: one
-// part in the first two steps 2e-4..6e-4 from 256 rows up, where the errors
+// part in the first two steps 3e-6..8e-4 from 256 rows up, where the errors
 // of many singular values average, and up to 1e-2 for a few rows; one part
-// in three steps up to 2e-3; two parts everywhere 1e-7..6e-7.  A bf16 result
-// is rounded by 1.5e-3 anyway, so bf16 takes one part in the first two
-// steps of matrices of 256 rows or more, and all else two parts.
+// in three steps up to 2e-3; two parts everywhere 3e-8..1.5e-6.  A bf16
+// result is rounded by 1.5e-3 anyway, so bf16 takes one part in the first two
+// steps of matrices of 256 rows or more, and all else two parts.  With two
+// parts, what is left is the fp32 sums' rounding, as in any fp32 product:
+// 2e-7..2.1e-6 for gaussian and badly scaled matrices, up to 9.4e-6 near low
+// rank, where plain fp32 products give 8.3e-6.
 
 #include <torch/extension.h>
 #include <ATen/ATen.h>
