@@ -42,6 +42,7 @@ namespace {
 using namespace mm;
 
 constexpr float kScale = 4096.f;  // of X, A and B in fp16
+constexpr long kFewRows = 256;    // below: two parts in every step
 
 inline long up(long x, long m) { return (x + m - 1) / m * m; }
 
@@ -555,7 +556,7 @@ long at_once(long small, long large) {
 void run(const Batch& batch, int type, long count, long small, long large,
          long least, const Polynomial& p, const at::TensorOptions& options) {
   auto stream = at::cuda::getCurrentCUDAStream();
-  const bool every = p.exact || least < 256;
+  const bool every = p.exact || least < kFewRows;
   auto fine = [&](int64_t i) { return every || i >= p.steps - 3; };
 
   // zeros up to whole tiles, and whole stages of 128 k
@@ -711,7 +712,8 @@ void newton_schulz(const at::Tensor& g, at::Tensor out, int64_t steps,
 
 // Each matrix of a list in place.  They are of one type and device and fill
 // up to the same multiples of 128 rows and columns (of 128 columns and rows
-// the other way round).
+// the other way round).  Unless `exact`, all or none have the rows that make
+// the first steps' operands one part: no result depends on its company.
 void newton_schulz_list(std::vector<at::Tensor> mats, int64_t steps,
                         double a, double b, double c, double eps,
                         bool exact) {
@@ -743,6 +745,9 @@ void newton_schulz_list(std::vector<at::Tensor> mats, int64_t steps,
       TORCH_CHECK(i == 0 || (up(s, 128) == up(small, 128) &&
                              up(l, 128) == up(large, 128)),
                   "newton_schulz: matrices of different padded sizes");
+      TORCH_CHECK(exact || i == 0 || (s >= kFewRows) == (least >= kFewRows),
+                  "newton_schulz: matrices of ", kFewRows, " rows and of "
+                  "fewer in one list");
       small = std::max(small, s);
       large = std::max(large, l);
       least = std::min(least, s);

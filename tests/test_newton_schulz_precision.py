@@ -173,3 +173,26 @@ def test_muon_bf16_masters_of_any_size(m, n, kind):
     if m >= 256:
         tol = tol + 2 * _off(_steps(g, _one_in_two_steps), want)
     assert bool((_off(got[None], want) <= tol).all())
+
+
+@GPU
+def test_precision_is_of_the_matrix_not_of_its_company():
+    """Matrices of 129 to 256 rows go through the products in one list, but
+    only those of 256 have steps in 11 bits."""
+    small = _matrices(1, 200, 300, 'rows', 'cuda', seed=2)[0]
+    large = _matrices(1, 256, 300, 'rows', 'cuda', seed=3)[0]
+    alone = [_step_of(torch.bfloat16, [t])[0] for t in (small, large)]
+    for order in (1, -1):
+        both = _step_of(torch.bfloat16, [small, large][::order])[::order]
+        for p, q in zip(alone, both):
+            assert torch.equal(p, q)
+
+
+@GPU
+def test_a_list_of_two_precisions_is_refused():
+    f = ops.ext().newton_schulz_list
+    mats = [torch.ones(200, 300, device='cuda'),
+            torch.ones(256, 300, device='cuda')]
+    with pytest.raises(RuntimeError, match='256'):
+        f(mats, 5, A, B, C, 1e-7, False)
+    f(mats, 5, A, B, C, 1e-7, True)
