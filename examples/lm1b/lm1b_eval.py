@@ -26,7 +26,7 @@ import torch
 
 import data_utils
 from parallax_amd.models.lm1b import LM1BModel
-from parallax_amd.ops import linear_cross_entropy
+from parallax_amd.ops.linear_ce import check_labels, linear_cross_entropy
 
 
 @torch.no_grad()
@@ -49,6 +49,7 @@ def evaluate_perplexity(model, dataset, batch_size=16, num_steps=20,
         if emb.dtype != body:
             emb = emb.to(body)
         hs, state = model.lstm(emb, state)
+        check_labels(y, w_full.shape[0])
         nll = linear_cross_entropy(hs.float(), w_full, b_full, y,
                                    reduction='sum')
         tot_nll += float(nll)

@@ -16,7 +16,8 @@ import torch
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)),
                                 '..', '..'))
 
-from parallax_amd.ops import linear_cross_entropy  # noqa: E402
+from parallax_amd.ops.linear_ce import (check_labels,  # noqa: E402
+                                        linear_cross_entropy)
 
 
 def _decoder_nll(model, dec, thought, tgt):
@@ -27,8 +28,9 @@ def _decoder_nll(model, dec, thought, tgt):
     outs, _ = dec(torch.cat([emb, th], dim=-1))
     h = model.out_proj(outs)
     y = tgt[:, 1:]
-    return linear_cross_entropy(h, model.emb.full_weight(), None, y,
-                                reduction='sum'), y.numel()
+    w = model.emb.full_weight()
+    check_labels(y, w.shape[0])
+    return linear_cross_entropy(h, w, None, y, reduction='sum'), y.numel()
 
 
 @torch.no_grad()

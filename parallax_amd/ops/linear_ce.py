@@ -49,6 +49,17 @@ def _check(inputs, weight, bias, labels, label_smoothing, reduction):
                         % labels.dtype)
 
 
+def check_labels(labels, words, ignore_index=-100):
+    """Raises IndexError where a label is neither a word nor
+    ``ignore_index``.  The loss clamps such labels, since it does not wait
+    for the GPU; what reads its result on the host anyway, as a perplexity
+    does, asks here first."""
+    out = (labels != ignore_index) & ((labels < 0) | (labels >= words))
+    if bool(out.any()):
+        raise IndexError('label %d outside the vocabulary of %d words'
+                         % (int(labels[out][0]), words))
+
+
 def _plain(x, weight, bias, labels, ignore_index, smoothing, reduction):
     live = labels != ignore_index
     # a product with what ignored rows hold would carry it into the gradients
