@@ -60,13 +60,18 @@ def check_labels(labels, words, ignore_index=-100):
                          % (int(labels[out][0]), words))
 
 
+def _wide(t):
+    """In 32 bits, or 64 where it has them (on the host alone)."""
+    return t.to(torch.promote_types(t.dtype, torch.float32))
+
+
 def _plain(x, weight, bias, labels, ignore_index, smoothing, reduction):
     live = labels != ignore_index
     # a product with what ignored rows hold would carry it into the gradients
-    x = torch.where(live[:, None], x.float(), 0.0)
-    logits = x @ weight.float().t()
+    x = torch.where(live[:, None], _wide(x), 0.0)
+    logits = x @ _wide(weight).t()
     if bias is not None:
-        logits = logits + bias.float()
+        logits = logits + bias.to(logits.dtype)
     # labels outside the vocabulary go to its nearest end, as on the GPU
     y = torch.where(live, labels.clamp(0, weight.shape[0] - 1), 0)
     lse = torch.logsumexp(logits, 1)
@@ -89,7 +94,8 @@ def linear_cross_entropy(inputs, weight, bias, labels, reduction='mean',
     Rows whose label is ``ignore_index`` have no loss and no gradient, and
     their inputs are not read; other labels are clamped to the vocabulary.
     'mean' is over the rows that count (NaN where none does).  The loss is
-    fp32: a scalar, or the shape of ``labels`` for 'none'.  ``weight`` is
+    fp32 (fp64 of fp64 inputs, which the host takes and the GPU refuses): a
+    scalar, or the shape of ``labels`` for 'none'.  ``weight`` is
     cast to the type of ``inputs`` where the two differ; under autocast
     both are cast to its type, as a product's operands are.
     """
@@ -101,11 +107,11 @@ def linear_cross_entropy(inputs, weight, bias, labels, reduction='mean',
     if weight.dtype != x.dtype:
         weight = weight.to(x.dtype)
     if x.shape[0] == 0:  # no rows: what a sum over nothing is
-        z = x.float().sum() + weight[:0].float().sum()
+        z = _wide(x).sum() + _wide(weight[:0]).sum()
         if bias is not None:
-            z = z + bias[:0].float().sum()
+            z = z + bias[:0].to(z.dtype).sum()
         if reduction == 'none':
-            return (x.float().sum(-1) + z).reshape(labels.shape)
+            return (_wide(x).sum(-1) + z).reshape(labels.shape)
         return z / 0 if reduction == 'mean' else z
     if _ops.use_native(x):
         losses = _ops.ext().linear_ce(x, weight, bias, y.contiguous(),

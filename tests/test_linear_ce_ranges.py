@@ -165,3 +165,24 @@ def test_what_ignored_rows_hold_is_not_read(dev, reduction, ignore):
     for p, q in zip(*outs):
         assert torch.isfinite(p).all() and torch.equal(p, q)
     assert not outs[1][1][::3].any() and outs[1][1][1::3].any()
+
+
+def test_fp64_on_the_host():
+    """64 bits stay 64 bits, so torch's own check against differences
+    holds; the GPU refuses them."""
+    x, w, b, y = _spread('cpu', n=6, v=20, d=5, seed=5)
+    y[2] = -100
+    x, w, b = (t.double().requires_grad_() for t in (x, w, b / 10))
+    for reduction in ('mean', 'none'):
+        def f(x, w, b):
+            return ops.linear_cross_entropy(x, w, b, y, reduction=reduction,
+                                            label_smoothing=0.2)
+
+        assert f(x, w, b).dtype == torch.float64
+        assert torch.autograd.gradcheck(f, (x, w, b))
+        assert ops.linear_cross_entropy(
+            x[:0], w, b, y[:0], reduction=reduction).dtype == torch.float64
+    z = x @ w.t() + b
+    want = torch.nn.functional.cross_entropy(z, y)
+    got = ops.linear_cross_entropy(x, w, b, y)
+    assert abs(float(got - want)) < 1e-13
