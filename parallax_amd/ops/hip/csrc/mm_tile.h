@@ -211,8 +211,11 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// What a wave has read from LDS has arrived before it lets others write
+// there: the compiler puts no such wait before a barrier, and whether the
+// products that need the values stand before it is up to its scheduling.
 __device__ __forceinline__ void barrier() {
-  asm volatile("" ::: "memory");
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
