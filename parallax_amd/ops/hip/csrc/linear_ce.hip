@@ -572,8 +572,14 @@ __global__ __launch_bounds__(256) void lce_join_kernel(Join p) {
       if (live && p.bias.p) a += load_as(p.bias.p, y * p.bias.rs, p.bias.type);
       const float l = m * kLn2 + logf(s);
       p.lse[r] = l;
-      float out = l - (1.f - p.eps) * a;
-      if (p.eps != 0.f) out -= p.eps * (t * kLn2 / (float)p.V);
+      // lse and the label's logit are sums in different orders: where they
+      // are equal, the difference may round to less than nothing (NaN stays)
+      float out = l - a;
+      if (out < 0.f) out = 0.f;
+      if (p.eps != 0.f) {
+        const float rest = l - t * kLn2 / (float)p.V;
+        out = (1.f - p.eps) * out + p.eps * (rest < 0.f ? 0.f : rest);
+      }
       p.loss[r] = live ? out : 0.f;
     }
   }

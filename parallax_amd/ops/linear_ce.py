@@ -75,9 +75,9 @@ def _plain(x, weight, bias, labels, ignore_index, smoothing, reduction):
     # labels outside the vocabulary go to its nearest end, as on the GPU
     y = torch.where(live, labels.clamp(0, weight.shape[0] - 1), 0)
     lse = torch.logsumexp(logits, 1)
-    losses = lse - (1 - smoothing) * logits.gather(1, y[:, None])[:, 0]
+    losses = lse - logits.gather(1, y[:, None])[:, 0]
     if smoothing:
-        losses = losses - smoothing * logits.mean(1)
+        losses = (1 - smoothing) * losses + smoothing * (lse - logits.mean(1))
     losses = torch.where(live, losses, torch.zeros_like(losses))
     if reduction == 'none':
         return losses
@@ -95,7 +95,8 @@ def linear_cross_entropy(inputs, weight, bias, labels, reduction='mean',
     their inputs are not read; other labels are clamped to the vocabulary.
     'mean' is over the rows that count (NaN where none does).  The loss is
     fp32 (fp64 of fp64 inputs, which the host takes and the GPU refuses): a
-    scalar, or the shape of ``labels`` for 'none'.  ``weight`` is
+    scalar, or the shape of ``labels`` for 'none'; none is negative.
+    ``weight`` is
     cast to the type of ``inputs`` where the two differ; under autocast
     both are cast to its type, as a product's operands are.
     """

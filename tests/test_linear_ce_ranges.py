@@ -186,3 +186,29 @@ def test_fp64_on_the_host():
     want = torch.nn.functional.cross_entropy(z, y)
     got = ops.linear_cross_entropy(x, w, b, y)
     assert abs(float(got - want)) < 1e-13
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('eps', [0.0, 1e-9])
+def test_no_loss_is_negative(dev, dtype, eps):
+    """Labels of a probability that rounds to 1: lse and the label's logit
+    are sums in different orders, each off by its rounding."""
+    g = torch.Generator().manual_seed(6)
+    w = torch.randn(200, 96, generator=g)
+    y = torch.randint(0, 200, (300,), generator=g)
+    x = w[y] * 20 + torch.randn(300, 96, generator=g)
+    x, w, y = x.to(dtype).to(dev), w.to(dtype).to(dev), y.to(dev)
+    each = ops.linear_cross_entropy(x, w, None, y, reduction='none',
+                                    label_smoothing=eps)
+    z = x.double() @ w.double().t()
+    want = (1 - eps) * (torch.logsumexp(z, 1)
+                        - z.gather(1, y[:, None])[:, 0]) \
+        + eps * (torch.logsumexp(z, 1) - z.mean(1))
+    tol = 2 * (96 + 32) * E * (x.double().abs() @ w.double().abs().t()) \
+        .amax(1) + 8 * E * z.abs().amax(1)
+    assert float(z.amax(1).min()) > 500
+    assert bool((each >= 0).all()), float(each.min())
+    assert bool(((each.double() - want).abs() <= tol).all())
+    assert bool(torch.isnan(ops.linear_cross_entropy(
+        x * float('nan'), w, None, y, reduction='none')).all())
