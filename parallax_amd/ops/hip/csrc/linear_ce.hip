@@ -11,8 +11,8 @@
 // (max, sum, total) per row; a second kernel joins them and takes the
 // label's logit as a dot product of its own.  Backward goes over pieces of
 // the vocabulary: the logits of a piece are computed again, become G in 16
-// bits (bounded by a fixed budget, so it stays in the last-level cache),
-// and two products read G: dw of the piece, finished, and dx, which adds up
+// bits (of a fixed budget up to 360,000 rows, 90,000 in fp32, so it stays in the
+// last-level cache), and two products read G: dw of the piece, finished, and dx, which adds up
 // in fp32 over the pieces.  All of it is bound by the matrix units: 2,560
 // rows of 512, 793,470 words, bf16, forward and backward 8.9 ms for 8.3
 // TFLOP (the logits counted twice), 0.94 PF; a large library product reaches
@@ -53,9 +53,11 @@ using namespace mm;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// G of one piece of the vocabulary takes at most this much
+// G of one piece of the vocabulary takes at most this much, or what 256 words
+// take where that is more: 512 B a row, 2 KB in fp32 (its two forms), so 2 GB
+// for the most rows there can be
 constexpr long kPieceBytes = 176L << 20;
-// and so do the split parts of an fp32 table's piece
+// and the split parts of an fp32 table's piece at most this, or 256 words'
 constexpr long kSplitBytes = 128L << 20;
 
 __host__ __device__ inline long up(long x, long m) {
@@ -965,6 +967,8 @@ using Mid = Tile<128, 128, 64, 64, 64, 2>;
 using MidParts = Tile<128, 128, 32, 64, 64, 2>;
 template <int PARTS>
 using MidOf = std::conditional_t<PARTS == 2, MidParts, Mid>;
+template <int PARTS>
+using BigOf = std::conditional_t<PARTS == 2, MidParts, Big>;
 // few rows, or rows that leave much of a larger tile empty: wide in the words
 using Flat = Tile<64, 256, 64, 32, 64, 2>;
 using FlatT = Tile<256, 64, 64, 32, 64, 2>;
@@ -1236,7 +1240,12 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x,
     using C = decltype(tile);
     const int nmt = (int)((p.n + C::BM - 1) / C::BM);
     const long piece_tiles = (std::min(piece, p.v) + C::BN - 1) / C::BN;
-    // a workgroup takes several tiles of words as long as ~2000 are left
+    // A workgroup takes several tiles of words, so that its sums are joined
+    // once, as long as ~2,000 workgroups are left, which are several turns
+    // of all CUs.  2,560 rows x 793,470 words of 512 in bf16: one tile 2,213
+    // us, four 1,933, eight 1,914, sixteen 1,996; 320 rows in fp32, where
+    // pieces are short: one 1,591, two 1,700, eight 2,086; 512 x 32,000
+    // (500 tiles) in bf16 one 33, four 47.
     int tpb = (int)std::min<long>(8, piece_tiles * nmt / 2048);
     if (tpb < 1) tpb = 1;
     const long span = (long)C::BN * tpb;
@@ -1370,7 +1379,11 @@ std::vector<at::Tensor> linear_ce_bwd(
   piece = std::max(256L, std::min(piece, ((1L << 30) - 1) / w_ld / 256 * 256));
   TORCH_CHECK(piece % 256 == 0, "linear_ce_bwd: pieces of whole tiles");
   const int ldg = (int)p.np * p.parts;
-  // dx: few tiles and a long k, so k is cut until the chip is full
+  // dx: few tiles and a long k, so k is cut until two workgroups a CU have
+  // work: 2,560 rows x 100,000 words of 512 in bf16, dx alone: 128 in all
+  // 1,610 us, 256 1,005, 512 915, 1,024 988.  At least 512 words each (256
+  // and 1,024 are alike).  128 x 128 tiles: 2,560 rows 874 us and 1,306 with
+  // 64 x 64, 129 rows 114 and 119.
   const int dx_tile = p.n > 128 && p.dp >= 128 ? 128 : 64;
   const long dx_tiles = ((p.n + dx_tile - 1) / dx_tile) *
                         ((p.dp + dx_tile - 1) / dx_tile);
@@ -1495,7 +1508,9 @@ std::vector<at::Tensor> linear_ce_bwd(
                 kx.row.g, sc, xinv, want_dx ? Gx : nullptr, tinv);
             HIP_CHECK_KERNEL();
           };
-          if (p.np > 4096) {
+          // dw alone, D = 64: 512 rows x 50,000 words 167 us with a wave a
+          // word and 181 with a workgroup, 2,048 x 20,000 239 and 226
+          if (p.np >= 1024) {
             launch(lce_split_kernel<true>, words);
           } else {
             launch(lce_split_kernel<false>, words / 4);
@@ -1519,9 +1534,18 @@ std::vector<at::Tensor> linear_ce_bwd(
                 p.type, (int)vp, (int)p.d, mt, nt);
             HIP_CHECK_KERNEL();
           };
+          // 256 x 256 tiles where they fill three quarters of the CUs and
+          // the sum over the rows is long: with dw alone 2,048 rows of 512
+          // against 8,192 words (64 tiles) 111 us and 88 with 128 x 128,
+          // 24,576 (192) 198 and 197, 32,768 (256) 238 and 250; 256 rows,
+          // 100,000 words 144 and 135.  Two parts leave the LDS less time:
+          // 2,048 rows 1,068 and 856 us, never less.  64 x 64 for few:
+          // 1,024 rows of 256 in fp32 against 6,400 words (25) 95 us and
+          // 102 with 128 x 128, 16,384 (64) 178 and 169.
           const long cover = ((vp + 255) / 256) * ((p.dp + 255) / 256);
-          if (cover >= 192 && p.dp % 256 == 0) {
-            run(Big{});
+          if (PARTS == 1 && p.n >= 1024 && cover >= 192 &&
+              p.dp % 256 == 0) {
+            run(BigOf<PARTS>{});
           } else if (cover >= 48 && p.dp >= 128) {
             run(MidOf<PARTS>{});
           } else {
