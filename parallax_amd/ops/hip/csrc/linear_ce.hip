@@ -11,13 +11,15 @@
 // (max, sum, total) per row; a second kernel joins them and takes the
 // label's logit as a dot product of its own.  Backward goes over pieces of
 // the vocabulary: the logits of a piece are computed again, become G in 16
-// bits (of a fixed budget up to 360,000 rows, 90,000 in fp32, so it stays in the
-// last-level cache), and two products read G: dw of the piece, finished, and dx, which adds up
-// in fp32 over the pieces.  All of it is bound by the matrix units: 2,560
-// rows of 512, 793,470 words, bf16, forward and backward 8.9 ms for 8.3
-// TFLOP (the logits counted twice), 0.94 PF; a large library product reaches
-// 1.41.  Row sums, maxima, lse and all sums over k are fp32.  No atomics:
-// every result is independent of the order of blocks.
+// bits (of a fixed budget up to 360,000 rows, 90,000 in fp32, so it stays in
+// the last-level cache), and two products read G: dw of the piece, finished,
+// and dx, which adds up in fp32 over the pieces.  The time is that of the
+// products, which keep the matrix units busy for 33 to 58% of it (the LDS for
+// 23 to 32%; the rest is waits for the stages' loads, exponentials and
+// stores): 2,560 rows of 512, 793,470 words, bf16, forward and backward 8.9
+// ms for 8.3 TFLOP (the logits counted twice), 0.94 PF; a large library
+// product reaches 1.41.  Row sums, maxima, lse and all sums over k are fp32.
+// No atomics: every result is independent of the order of blocks.
 //
 // Types.  bf16 and fp16 inputs are multiplied as they are; G is rounded to
 // the same type once, relative to the largest |g|, and the results are
@@ -209,8 +211,8 @@ __device__ __forceinline__ void load8(const Pack& p, const char* src, long c,
 }
 
 // A wave takes one row, or several of fewer than 512 values, eight values a
-// lane at a time.  Bound by memory: 61,000 fp32 rows of 512 into pairs 57 us,
-// 4.4 TB/s read and written.
+// lane at a time.  Bound by memory: 793,470 fp32 rows of 512 into pairs 0.83
+// ms, 3.9 TB/s read and written.
 template <int PARTS>
 __global__ __launch_bounds__(256) void lce_pack_kernel(Pack p) {
   __shared__ float scratch[PX_BLOCK / WAVE];
@@ -349,10 +351,10 @@ struct Logits {
 };
 
 // max, sum of exp and (SMOOTH) total of each row, in powers of 2, over `tpb`
-// tiles of words.  2,560 x 793,470 x 512 bf16: 2.17 ms, 0.96 PF; what the
+// tiles of words.  2,560 x 793,470 x 512 bf16: 2.16 ms, 0.96 PF; what the
 // product alone does not reach is the exponentials, a quarter of the rate of
 // other instructions, under which only the other workgroup's products run.
-// fp32, 320 rows: 76 us for 61,000 words, 0.79 PF of 16-bit products.
+// fp32, 320 rows: 0.95 ms, 0.82 PF of 16-bit products.
 template <class C, int XL, int PARTS, bool BF, bool SMOOTH>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_fwd_kernel(
     Logits p, float* __restrict__ part, int vb0, int nblocks, int nmt,
@@ -632,7 +634,7 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(
 // words are the tile's m: a lane holds four neighbouring rows of one word,
 // sums over the rows stay in it, and dw reads G k-contiguous.
 // DB: sums of each tile of rows into dbp[row tile][..], or as they are into
-// db where there is one.  2,560 x 32,768 x 512 bf16: 126 us, 0.68 PF: beside
+// db where there is one.  2,560 x 32,768 x 512 bf16: 124 us, 0.69 PF: beside
 // the exponentials 168 MB of G go out, 34 us by themselves.
 template <class C, int XL, int PARTS, bool BF, bool DB>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
@@ -749,7 +751,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
 // The rows of x have scales of their own, 1 / xinv, which dw sums over: they
 // are undone here.  A wave (WIDE: a workgroup) takes a word; in its place, a
 // wave has read what it writes over, 1 KiB, before.  cols: of the np, those
-// that G has been made for.
+// that G has been made for.  Bound by memory: 20,000 words x 1,024 rows 40
+// us, 6.2 TB/s of the 82 MB in and 164 MB out, part of them in cache.
 template <bool WIDE>
 __global__ __launch_bounds__(256) void lce_split_kernel(
     float* __restrict__ G, int np, int cols, int words,
@@ -823,7 +826,7 @@ __global__ __launch_bounds__(256) void lce_db_kernel(
 }
 
 // dw[v, :] = 1/S sum_n G[n, v] x[n, :]  (x k-strided).  32,768 x 512 over
-// 2,560 rows bf16: 85 us, 1.01 PF.  tinv: what is left to undo of a word's
+// 2,560 rows bf16: 82 us, 1.05 PF.  tinv: what is left to undo of a word's
 // scale (PARTS = 2).
 template <class C, int PARTS, bool BF>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
@@ -874,7 +877,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
 }
 
 // part[slice][n, :] (+)= sum over a slice of the piece's words G[n, v] w[v, :]
-// (both k-strided).  2,560 x 512 over 32,768 words bf16: 94 us, 0.91 PF; on
+// (both k-strided).  2,560 x 512 over 32,768 words bf16: 92 us, 0.94 PF; on
 // 256 x 256 tiles the partial sums cost more than the product gains.
 template <class C, int PARTS, bool BF>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dx_kernel(

@@ -102,7 +102,7 @@ __device__ __forceinline__ f4 load_four(const void* p, long i, int type) {
 }
 
 // Sums of squares in 64 bits (an fp32 square of 1e-20 or 1e20 is lost), one
-// partial per block.  Bound by memory: 25 MB 8.5 us, 3.0 TB/s.
+// partial per block.  Bound by memory: 25 MB 8.7 us, 2.9 TB/s.
 __global__ __launch_bounds__(256) void ns_norm_kernel(
     Batch batch, int type, double* __restrict__ part) {
   __shared__ double red[4];
@@ -272,7 +272,7 @@ __device__ __forceinline__ void put_tile(char* lds, const Matrix& out, int m0,
 // Where there are few tiles, k is cut (CUT = 1): each workgroup leaves its
 // sums in `part`, and a second kernel (CUT = 2) adds them up in order and
 // goes on.  (Left to the last workgroup of a tile, the fences that takes
-// cost more than the launch: 146 us for 12 x 512 x 2048, 42 this way, 0.58
+// cost more than the launch: 146 us for 12 x 512 x 2048, 42 this way, 0.57
 // PF of the 16-bit products on and above the diagonal.)
 template <class C, int PARTS, bool SECOND, int CUT>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void ns_sym_kernel(
 
 // X' = a X + B X (two parts: B holds the a); the last one goes to the result.
 // The sums start from a X, so that it is read while the first stages are on
-// their way.  1024 x 8192 in two parts: 58 us, 0.89 PF of 16-bit products,
+// their way.  1024 x 8192 in two parts: 59 us, 0.88 PF of 16-bit products,
 // of which the product alone takes 44; all its 512 workgroups run at once,
 // so none covers the other's 32 MB of X' on the way out.
 template <class C, int PARTS>
