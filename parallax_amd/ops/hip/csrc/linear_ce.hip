@@ -11,9 +11,9 @@
 // (max, sum, total) per row; a second kernel joins them and takes the
 // label's logit as a dot product of its own.  Backward goes over pieces of
 // the vocabulary: the logits of a piece are computed again, become G in 16
-// bits (of a fixed budget up to 360,000 rows, 90,000 in fp32, so it stays in
-// the last-level cache), and two products read G: dw of the piece, finished,
-// and dx, which adds up in fp32 over the pieces.  The time is that of the
+// bits (of a fixed budget up to 360,000 rows, 180,000 in fp32; in 16 bits it
+// stays in the last-level cache), and two products read G: dw of the piece,
+// finished, and dx, which adds up in fp32 over the pieces.  The time is that of the
 // products, which keep the matrix units busy for 33 to 58% of it (the LDS for
 // 23 to 32%; the rest is waits for the stages' loads, exponentials and
 // stores): 2,560 rows of 512, 793,470 words, bf16, forward and backward 8.9
@@ -28,9 +28,10 @@
 // scaling by a power of two, and so is G: three products in the place of one.
 // Two parts hold 22 bits of values down to 2^-17 of the largest that shares
 // their scale, and 2^-39 of that of smaller ones, so scales have to follow
-// the values: x has one a row, and G is made in fp32 and split twice, for dw
-// with one a word (the words of a large vocabulary differ by 1e12 and more in
-// probability, and each has a gradient of its own) and for dx with one a row.
+// the values: x has one a row, and G goes out twice, for dw with one for each
+// word and tile of rows (the words of a large vocabulary differ by 1e12 and
+// more in probability, and each has a gradient of its own), for dx with one
+// for each row.
 // w has one a row in the forward and a single one in the backward: dx is
 // exact to 2^-38 of the row's |g| max |w| where its values are below that.
 //
@@ -55,9 +56,9 @@ using namespace mm;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// G of one piece of the vocabulary takes at most this much, or what 256 words
-// take where that is more: 512 B a row, 2 KB in fp32 (its two forms), so 2 GB
-// for the most rows there can be
+// G of one piece of the vocabulary takes at most this much (fp32: each of its
+// two forms), or what 256 words take where that is more: 512 B a row, 1 KB
+// each in fp32, so 2 GB in all for the most rows there can be
 constexpr long kPieceBytes = 176L << 20;
 // and the split parts of an fp32 table's piece at most this, or 256 words'
 constexpr long kSplitBytes = 128L << 20;
@@ -629,18 +630,22 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(
 
 // --- backward ---------------------------------------------------------------
 
-// G of one piece, transposed: [words][ldg], zeros outside the matrix, in the
-// inputs' 16 bits or (PARTS = 2) in fp32 for lce_split_kernel.  The
+// G of one piece, transposed: [words][ldg], zeros outside the matrix.  The
 // words are the tile's m: a lane holds four neighbouring rows of one word,
-// sums over the rows stay in it, and dw reads G k-contiguous.
+// sums over the rows stay in it, and dw reads G k-contiguous.  PARTS = 2: in
+// pairs of parts, twice.  For dx (Gx) scaled by a power of two for each row;
+// for dw (G) by one for each word and tile of rows, whose reciprocal goes to
+// tinv[tile][words], and with the scales undone that the rows of x have
+// (20,000 words x 999 rows of 256 63 us, 44 with one form under one scale).
 // DB: sums of each tile of rows into dbp[row tile][..], or as they are into
 // db where there is one.  2,560 x 32,768 x 512 bf16: 124 us, 0.69 PF: beside
 // the exponentials 168 MB of G go out, 34 us by themselves.
 template <class C, int XL, int PARTS, bool BF, bool DB>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
     Logits p, Rows rows, const float* __restrict__ sc, long V, long v0,
-    float eps, void* __restrict__ G, int ldg, float* __restrict__ dbp,
-    long db_ld, void* __restrict__ db, int db_type, int nvt, int nrt) {
+    float eps, ushort* __restrict__ G, ushort* __restrict__ Gx, int ldg,
+    float* __restrict__ tinv, long t_ld, float* __restrict__ dbp, long db_ld,
+    void* __restrict__ db, int db_type, int nvt, int nrt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int bid = die_contiguous(blockIdx.x, nvt * nrt);
   const int rt = bid % nrt, vt = bid / nrt;
@@ -702,11 +707,58 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
       for (int j = 0; j < C::FN; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
     }
   if constexpr (PARTS == 2) {
-    store_floats<C>(smem, static_cast<float*>(G) + (long)m0 * ldg + n0, ldg,
-                    [&](int i, int j) { return acc[i][j]; });
+    const long at = (long)m0 * ldg + n0 * 2;
+    auto four = [&](const float* v, int j) {  // of this lane's rows
+      return *reinterpret_cast<const f4*>(v + n0 + wn + j * 16 +
+                                          (lane >> 4) * 4);
+    };
+    if (Gx) {
+      store_pairs<C>(smem, Gx + at, ldg, [&](int i, int j) {
+        f4 g = S * four(rows.g, j);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) g[r] = scale_to_half(fabsf(g[r]));
+        return acc[i][j] * g;
+      });
+      __syncthreads();
+    }
+    if (tinv) {
+      float* red = reinterpret_cast<float*>(smem);  // [waves_n][BM]
+      float ts[C::FM] = {};
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) {
+        const f4 x = four(p.xinv, j);
+#pragma unroll
+        for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            ts[i] = fmaxf(ts[i], fabsf(acc[i][j][r] * x[r]));
+      }
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) {
+        ts[i] = fmaxf(ts[i], __shfl_xor(ts[i], 16, 64));
+        ts[i] = fmaxf(ts[i], __shfl_xor(ts[i], 32, 64));
+        if (lane < 16)
+          red[(wave % C::WAVES_N) * C::BM + wm + i * 16 + lane] = ts[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) {
+        const int m = wm + i * 16 + (lane & 15);
+#pragma unroll
+        for (int w = 0; w < C::WAVES_N; ++w)
+          ts[i] = fmaxf(ts[i], red[w * C::BM + m]);
+        ts[i] = scale_to_half(ts[i]);
+        if (lane < 16 && wave % C::WAVES_N == 0)
+          tinv[rt * t_ld + m0 + m] = 1.f / ts[i];
+      }
+      __syncthreads();
+      store_pairs<C>(smem, G + at, ldg, [&](int i, int j) {
+        return acc[i][j] * four(p.xinv, j) * ts[i];
+      });
+    }
   } else {
-    store_tile<C>(smem, static_cast<ushort*>(G) + (long)m0 * ldg + n0, ldg,
-                  C::BM, C::BN, [&](int i, int j) {
+    store_tile<C>(smem, G + (long)m0 * ldg + n0, ldg, C::BM, C::BN,
+                  [&](int i, int j) {
       const f4 v = acc[i][j];
       if (BF)
         return make_ushort4(bf16_bits(v[0]), bf16_bits(v[1]),
@@ -746,73 +798,6 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_grad_kernel(
   }
 }
 
-// fp32 G in pairs of parts: for dx (Gx) scaled by a power of two for each row,
-// for dw in its place by one for each word, whose reciprocal goes to tinv.
-// The rows of x have scales of their own, 1 / xinv, which dw sums over: they
-// are undone here.  A wave (WIDE: a workgroup) takes a word; in its place, a
-// wave has read what it writes over, 1 KiB, before.  cols: of the np, those
-// that G has been made for.  Bound by memory: 20,000 words x 1,024 rows 40
-// us, 6.2 TB/s of the 82 MB in and 164 MB out, part of them in cache.
-template <bool WIDE>
-__global__ __launch_bounds__(256) void lce_split_kernel(
-    float* __restrict__ G, int np, int cols, int words,
-    const float* __restrict__ g,
-    const float* __restrict__ sc, const float* __restrict__ xinv,
-    ushort* __restrict__ Gx, float* __restrict__ tinv) {
-  __shared__ float scratch[PX_BLOCK / WAVE];
-  constexpr int STEP = WIDE ? 1024 : 256;
-  const int v = WIDE ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int first = (WIDE ? threadIdx.x : threadIdx.x & 63) * 4;
-  if (v >= words) return;  // WIDE: never
-  float* row = G + (long)v * np;
-  float scale = 1.f;
-  if (tinv) {
-    float top = 0.f;
-#pragma unroll 4
-    for (int n = first; n < cols; n += STEP) {
-      const f4 a = *reinterpret_cast<const f4*>(row + n);
-      const f4 b = *reinterpret_cast<const f4*>(xinv + n);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(a[r] * b[r]));
-    }
-    if (WIDE) {
-      top = block_reduce_max(top, scratch);
-    } else {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1)
-        top = fmaxf(top, __shfl_xor(top, o, 64));
-    }
-    scale = scale_to_half(top);
-    if (first == 0) tinv[v] = 1.f / scale;
-  }
-  const float S = sc[0];
-#pragma unroll 2
-  for (int n = first; n < cols; n += STEP) {
-    const f4 a = *reinterpret_cast<const f4*>(row + n);
-    const long at = (long)v * np * 2 + (n >> 5) * 64 + (n & 31);
-    ushort h[4], l[4];
-    if (Gx) {
-      const f4 gn = *reinterpret_cast<const f4*>(g + n);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        split(a[r] * scale_to_half(fabsf(S * gn[r])), h[r], l[r]);
-      *reinterpret_cast<ushort4*>(Gx + at) =
-          make_ushort4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<ushort4*>(Gx + at + 32) =
-          make_ushort4(l[0], l[1], l[2], l[3]);
-    }
-    if (tinv) {
-      const f4 b = *reinterpret_cast<const f4*>(xinv + n);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) split(a[r] * b[r] * scale, h[r], l[r]);
-      ushort* to = reinterpret_cast<ushort*>(G) + at;
-      *reinterpret_cast<ushort4*>(to) = make_ushort4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<ushort4*>(to + 32) =
-          make_ushort4(l[0], l[1], l[2], l[3]);
-    }
-  }
-}
-
 // db from the sums of the tiles of rows, in their order (10 of 793,470 words:
 // 13 us, 2.4 TB/s).
 __global__ __launch_bounds__(256) void lce_db_kernel(
@@ -825,23 +810,58 @@ __global__ __launch_bounds__(256) void lce_db_kernel(
   store_as(db, v, type, s);
 }
 
+// Calls f behind every N stages of a product.
+template <int N, class F>
+struct TakeEvery {
+  static constexpr int EVERY = N;
+  F& f;
+  __device__ __forceinline__ void operator()() const { f(); }
+};
+
 // dw[v, :] = 1/S sum_n G[n, v] x[n, :]  (x k-strided).  32,768 x 512 over
-// 2,560 rows bf16: 82 us, 1.05 PF.  tinv: what is left to undo of a word's
-// scale (PARTS = 2).
-template <class C, int PARTS, bool BF>
+// 2,560 rows bf16: 82 us, 1.05 PF.  PARTS = 2: the sums over each ROWS rows
+// are scaled back by tinv[tile][words] and added up in fp32.
+template <class C, int PARTS, bool BF, int ROWS>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
     Operand G, Operand x, int kn, const float* __restrict__ sc,
-    const float* __restrict__ tinv, void* __restrict__ dw, int type, int vp,
-    int d, int nmt, int nnt) {
+    const float* __restrict__ tinv, long t_ld, void* __restrict__ dw,
+    int type, int vp, int d, int nmt, int nnt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int bid = die_contiguous(blockIdx.x, nmt * nnt);
   const int m0 = bid / nnt * C::BM, n0 = bid % nnt * C::BN;
-  f4 acc[C::FM][C::FN] = {};
-  product<C, KROWS, KCOLS, PARTS, BF>(smem, G, m0, x, n0, 0, kn, acc);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int wm = (wave / C::WAVES_N) * C::WM;
   const int wn = (wave % C::WAVES_N) * C::WN;
+  f4 acc[C::FM][C::FN] = {};
+  if constexpr (PARTS == 2) {
+    f4 part[C::FM][C::FN] = {};
+    float t[C::FM];  // of the tile of rows at hand: asked for one ahead
+    const float* next = tinv + m0 + wm + (lane & 15);
+    auto load = [&] {
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) t[i] = next[i * 16];
+      next += t_ld;
+    };
+    static_assert(ROWS % 32 == 0 && C::BK == 64, "stages of 32 rows");
+    int left = (kn + ROWS - 1) / ROWS;
+    load();
+    auto take = [&] {
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j) {
+          acc[i][j] += part[i][j] * t[i];
+          part[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+      if (--left > 0) load();
+    };
+    product<C, KROWS, KCOLS, PARTS, BF>(
+        smem, G, m0, x, n0, 0, kn, part,
+        TakeEvery<ROWS / 32, decltype(take)>{take});
+  } else {
+    product<C, KROWS, KCOLS, PARTS, BF>(smem, G, m0, x, n0, 0, kn, acc);
+  }
   const float back = sc[1];
   if (type != 2 && (d & 7) == 0) {
     store_tile<C>(smem, static_cast<ushort*>(dw) + (long)m0 * d + n0, d,
@@ -859,12 +879,11 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void lce_dw_kernel(
   for (int i = 0; i < C::FM; ++i) {
     const int v = m0 + wm + i * 16 + (lane & 15);
     if (v >= vp) continue;
-    const float word = PARTS == 2 ? tinv[v] : 1.f;
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) {
       const int c = n0 + wn + j * 16 + (lane >> 4) * 4;
       const long at = (long)v * d + c;
-      const f4 val = acc[i][j] * word * back;
+      const f4 val = acc[i][j] * back;
       if (type == 2 && c + 4 <= d && (d & 3) == 0) {
         *reinterpret_cast<f4*>(static_cast<float*>(dw) + at) = val;
       } else {
@@ -1371,8 +1390,7 @@ std::vector<at::Tensor> linear_ce_bwd(
   // words for which the tiles of dw fill the chip's 256 CUs once; a piece is
   // whole tiles of 256, as G and the words laid out are written by such
   const long wave_of_words = 256 * 256 / ((p.dp + 255) / 256) / 256 * 256;
-  // fp32: G of dw and that of dx
-  long piece = kPieceBytes / (p.np * (two ? 8 : 2));
+  long piece = kPieceBytes / (p.np * 2 * p.parts);
   piece = piece >= wave_of_words ? piece / wave_of_words * wave_of_words
                                  : piece / 256 * 256;
   piece = std::max(256L, std::min(piece, up(p.v, 256)));
@@ -1415,7 +1433,7 @@ std::vector<at::Tensor> linear_ce_bwd(
     const auto o_winv = mem.take<float>(two ? piece : 0);
     const auto o_G = mem.take<ushort>(piece * ldg);
     const auto o_Gx = mem.take<ushort>(two && want_dx ? piece * ldg : 0);
-    const auto o_tinv = mem.take<float>(two ? piece : 0);
+    const auto o_tinv = mem.take<float>(two && want_dw ? nrt * piece : 0);
     const auto o_part =
         mem.take<float>(want_dx ? slices * p.n * p.dp : 0);
     const auto o_dbp = mem.take<float>(want_db && nrt > 1 ? nrt * db_ld : 0);
@@ -1484,9 +1502,9 @@ std::vector<at::Tensor> linear_ce_bwd(
             constexpr int lds = R::template lds<PARTS>();
             allow_lds(kernel, lds);
             kernel<<<nvt * nrt, R::THREADS, lds, stream>>>(
-                q, kx.row, sc, p.v, v0, eps, G, ldg / PARTS, dbp, db_ld,
-                db_at,
-                want_db ? type_code(db) : 0, nvt, nrt);
+                q, kx.row, sc, p.v, v0, eps, G,
+                two && want_dx ? Gx : nullptr, ldg, tinv, piece, dbp, db_ld,
+                db_at, want_db ? type_code(db) : 0, nvt, nrt);
             HIP_CHECK_KERNEL();
           };
           if (want_db) {
@@ -1502,78 +1520,63 @@ std::vector<at::Tensor> linear_ce_bwd(
                 db_late ? db.data_ptr() : db_at, type_code(db));
             HIP_CHECK_KERNEL();
           }
-        }
-        if (two && (want_dx || want_dw)) {
-          const int words = (int)up(vp, 64);  // as many as are read
-          auto launch = [&](auto kernel, int blocks) {
-            kernel<<<blocks, 256, 0, stream>>>(
-                reinterpret_cast<float*>(G), (int)p.np, nrt * R::BN, words,
-                kx.row.g, sc, xinv, want_dx ? Gx : nullptr, tinv);
-            HIP_CHECK_KERNEL();
-          };
-          // dw alone, D = 64: 512 rows x 50,000 words 167 us with a wave a
-          // word and 181 with a workgroup, 2,048 x 20,000 239 and 226
-          if (p.np >= 1024) {
-            launch(lce_split_kernel<true>, words);
-          } else {
-            launch(lce_split_kernel<false>, words / 4);
+          // as rows of words for dw, as columns of rows for dx
+          const Operand g = operand(G, up(vp, 64), ldg, p.np);
+          const Operand gx = operand(Gx, up(vp, 64), ldg, p.np);
+          if (want_dw) {
+            auto run = [&](auto tile) {
+              using C = decltype(tile);
+              const int mt = (int)((vp + C::BM - 1) / C::BM);
+              const int nt = (int)((p.d + C::BN - 1) / C::BN);
+              auto kernel = lce_dw_kernel<C, PARTS, BF,
+                                          PARTS == 2 ? R::BN : 0>;
+              constexpr int lds = C::template lds<1>();
+              allow_lds(kernel, lds);
+              kernel<<<mt * nt, C::THREADS, lds, stream>>>(
+                  g, xr, (int)up(p.n, 64), sc, tinv, piece,
+                  static_cast<char*>(dw.data_ptr()) +
+                      v0 * p.d * dw.element_size(),
+                  p.type, (int)vp, (int)p.d, mt, nt);
+              HIP_CHECK_KERNEL();
+            };
+            // 256 x 256 tiles where they fill three quarters of the CUs and
+            // the sum over the rows is long: with dw alone 2,048 rows of 512
+            // against 8,192 words (64 tiles) 111 us and 88 with 128 x 128,
+            // 24,576 (192) 198 and 197, 32,768 (256) 238 and 250; 256 rows,
+            // 100,000 words 144 and 135.  Two parts leave the LDS less time:
+            // 2,048 rows 1,068 and 856 us, never less.  64 x 64 for few:
+            // 1,024 rows of 256 in fp32 against 6,400 words (25) 95 us and
+            // 102 with 128 x 128, 16,384 (64) 178 and 169.
+            const long cover = ((vp + 255) / 256) * ((p.dp + 255) / 256);
+            if (PARTS == 1 && p.n >= 1024 && cover >= 192 &&
+                p.dp % 256 == 0) {
+              run(BigOf<PARTS>{});
+            } else if (cover >= 48 && p.dp >= 128) {
+              run(MidOf<PARTS>{});
+            } else {
+              run(Small{});
+            }
           }
-        }
-        // as rows of words for dw, as columns of rows for dx
-        const Operand g = operand(G, up(vp, 64), ldg, p.np);
-        const Operand gx = operand(Gx, up(vp, 64), ldg, p.np);
-        if (want_dw) {
-          auto run = [&](auto tile) {
-            using C = decltype(tile);
-            const int mt = (int)((vp + C::BM - 1) / C::BM);
-            const int nt = (int)((p.d + C::BN - 1) / C::BN);
-            auto kernel = lce_dw_kernel<C, PARTS, BF>;
-            constexpr int lds = C::template lds<1>();
-            allow_lds(kernel, lds);
-            kernel<<<mt * nt, C::THREADS, lds, stream>>>(
-                g, xr, (int)up(p.n, 64), sc, tinv,
-                static_cast<char*>(dw.data_ptr()) +
-                    v0 * p.d * dw.element_size(),
-                p.type, (int)vp, (int)p.d, mt, nt);
-            HIP_CHECK_KERNEL();
-          };
-          // 256 x 256 tiles where they fill three quarters of the CUs and
-          // the sum over the rows is long: with dw alone 2,048 rows of 512
-          // against 8,192 words (64 tiles) 111 us and 88 with 128 x 128,
-          // 24,576 (192) 198 and 197, 32,768 (256) 238 and 250; 256 rows,
-          // 100,000 words 144 and 135.  Two parts leave the LDS less time:
-          // 2,048 rows 1,068 and 856 us, never less.  64 x 64 for few:
-          // 1,024 rows of 256 in fp32 against 6,400 words (25) 95 us and
-          // 102 with 128 x 128, 16,384 (64) 178 and 169.
-          const long cover = ((vp + 255) / 256) * ((p.dp + 255) / 256);
-          if (PARTS == 1 && p.n >= 1024 && cover >= 192 &&
-              p.dp % 256 == 0) {
-            run(BigOf<PARTS>{});
-          } else if (cover >= 48 && p.dp >= 128) {
-            run(MidOf<PARTS>{});
-          } else {
-            run(Small{});
-          }
-        }
-        if (want_dx) {
-          auto run = [&](auto tile) {
-            using C = decltype(tile);
-            const int mt = (int)((p.n + C::BM - 1) / C::BM);
-            const int nt = (int)((p.dp + C::BN - 1) / C::BN);
-            const int kv = (int)up(vp, 64);
-            const int kslice = (int)up((kv + slices - 1) / slices, 64);
-            auto kernel = lce_dx_kernel<C, PARTS, BF>;
-            constexpr int lds = C::template lds<1>();
-            allow_lds(kernel, lds);
-            kernel<<<mt * nt * slices, C::THREADS, lds, stream>>>(
-                gx, q.w, kv, kslice, mem.at<float>(o_part), (int)p.n,
-                (int)p.dp, v0 == 0, mt, nt, slices);
-            HIP_CHECK_KERNEL();
-          };
-          if (dx_tile == 128) {
-            run(MidOf<PARTS>{});
-          } else {
-            run(Small{});
+          if (want_dx) {
+            auto run = [&](auto tile) {
+              using C = decltype(tile);
+              const int mt = (int)((p.n + C::BM - 1) / C::BM);
+              const int nt = (int)((p.dp + C::BN - 1) / C::BN);
+              const int kv = (int)up(vp, 64);
+              const int kslice = (int)up((kv + slices - 1) / slices, 64);
+              auto kernel = lce_dx_kernel<C, PARTS, BF>;
+              constexpr int lds = C::template lds<1>();
+              allow_lds(kernel, lds);
+              kernel<<<mt * nt * slices, C::THREADS, lds, stream>>>(
+                  gx, q.w, kv, kslice, mem.at<float>(o_part), (int)p.n,
+                  (int)p.dp, v0 == 0, mt, nt, slices);
+              HIP_CHECK_KERNEL();
+            };
+            if (dx_tile == 128) {
+              run(MidOf<PARTS>{});
+            } else {
+              run(Small{});
+            }
           }
         }
       });

@@ -220,13 +220,21 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Takes the sums over the whole of k as they are.
+struct Whole {
+  static constexpr int EVERY = 0;
+};
+
 // acc[i][j] of wave (wm, wn): element (m, n) with
 //   m = m0 + wm + i*16 + (lane & 15), n = n0 + wn + j*16 + (lane>>4)*4 + r.
-// k runs over [k0, k1), both multiples of BK, of BK / 2 in pairs.
-template <class C, int AL, int BL, int PARTS, bool BF>
+// k runs over [k0, k1), both multiples of BK, of BK / 2 in pairs.  `take`
+// with EVERY > 0 is given the sums so far behind every so many stages and
+// the last one, and leaves acc as they shall go on.
+template <class C, int AL, int BL, int PARTS, bool BF, class F = Whole>
 __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
                                         const Operand& b, int n0, int k0,
-                                        int k1, f4 (&acc)[C::FM][C::FN]) {
+                                        int k1, f4 (&acc)[C::FM][C::FN],
+                                        F take = F()) {
   constexpr int BK = C::BK, ST = C::ST, T = C::THREADS;
   constexpr int STEP = BK / PARTS;
   Stager<C::BM, AL, BK, T, PARTS> sa;
@@ -326,8 +334,22 @@ __device__ __forceinline__ void product(char* lds, const Operand& a, int m0,
         multiply(fa, fb, acc);
       }
     }
+    if constexpr (F::EVERY > 0) {
+      if (t % F::EVERY == F::EVERY - 1 || t + 1 == total) {
+        if constexpr (APART) {
+#pragma unroll
+          for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < C::FN; ++j) {
+              acc[i][j] += low[i][j];
+              low[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+        take();
+      }
+    }
   }
-  if constexpr (APART) {
+  if constexpr (APART && F::EVERY == 0) {
 #pragma unroll
     for (int i = 0; i < C::FM; ++i)
 #pragma unroll
@@ -420,37 +442,6 @@ __device__ __forceinline__ void store_pairs(char* lds, ushort* out, long ld,
       const int r = c / PER_ROW, q = (c % PER_ROW) * 8;
       *reinterpret_cast<s8*>(out + (go * HALF + r) * ld + q) =
           *reinterpret_cast<const s8*>(lds + r * C::PAIR_ROW + q * 2);
-    }
-  }
-}
-
-// The same for values in fp32.
-template <class C, typename F>
-__device__ __forceinline__ void store_floats(char* lds, float* out, long ld,
-                                             F value) {
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  const int wm = (wave / C::WAVES_N) * C::WM;
-  const int wn = (wave % C::WAVES_N) * C::WN;
-  constexpr int HALF = C::BM / C::PAIR_GOES, PER_ROW = C::BN / 4;
-#pragma unroll
-  for (int go = 0; go < C::PAIR_GOES; ++go) {
-    if (go) __syncthreads();
-    if (wm / HALF == go) {
-#pragma unroll
-      for (int i = 0; i < C::FM; ++i)
-#pragma unroll
-        for (int j = 0; j < C::FN; ++j)
-          *reinterpret_cast<f4*>(
-              lds + (wm % HALF + i * 16 + (lane & 15)) * C::PAIR_ROW +
-              (wn + j * 16 + (lane >> 4) * 4) * 4) = value(i, j);
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int c = threadIdx.x; c < HALF * PER_ROW; c += C::THREADS) {
-      const int r = c / PER_ROW, q = (c % PER_ROW) * 4;
-      *reinterpret_cast<f4*>(out + (go * HALF + r) * ld + q) =
-          *reinterpret_cast<const f4*>(lds + r * C::PAIR_ROW + q * 4);
     }
   }
 }
