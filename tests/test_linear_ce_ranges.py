@@ -212,3 +212,15 @@ def test_no_loss_is_negative(dev, dtype, eps):
     assert bool(((each.double() - want).abs() <= tol).all())
     assert bool(torch.isnan(ops.linear_cross_entropy(
         x * float('nan'), w, None, y, reduction='none')).all())
+
+
+@GPU
+@pytest.mark.parametrize('n', [40, 130, 256, 300, 1000])
+@pytest.mark.parametrize('v,d', [(13001, 200), (700, 600)])
+def test_fp32_every_tile_of_both_gradients(n, v, d):
+    """Tiles of 64 and 128 rows behind one another, whose scales differ, in
+    the large and the small tile of dw."""
+    x, w, b, y = _spread('cuda', n=n, v=v, d=d, seed=n)
+    up = 10.0 ** torch.linspace(3, -12, n, device='cuda')
+    x *= 10.0 ** torch.linspace(-3, 0, n, device='cuda')[:, None]
+    _gradients_inside(x, w, b, y, up)
