@@ -24,16 +24,18 @@
 // Types.  bf16 and fp16 inputs are multiplied as they are; G is rounded to
 // the same type once, relative to the largest |g|, and the results are
 // scaled back (at most 2^-8 or 2^-11 of each value, as the final rounding of
-// the gradients is).  fp32 inputs are split into two fp16 parts after a
-// scaling by a power of two, and so is G: three products in the place of one.
-// Two parts hold 22 bits of values down to 2^-17 of the largest that shares
-// their scale, and 2^-39 of that of smaller ones, so scales have to follow
-// the values: x has one a row, and G goes out twice, for dw with one for each
-// word and tile of rows (the words of a large vocabulary differ by 1e12 and
-// more in probability, and each has a gradient of its own), for dx with one
-// for each row.
-// w has one a row in the forward and a single one in the backward: dx is
-// exact to 2^-38 of the row's |g| max |w| where its values are below that.
+// the gradients is; fp16 G below 2^-27 of the largest |g| is off by up to
+// 2^-38 of that).
+//
+// fp32 inputs are split into two fp16 parts after a scaling by a power of two,
+// and so is G: three products in the place of one.  Two parts hold 22 bits of
+// values down to 2^-17 of the largest that shares their scale, and 2^-39 of
+// that of smaller ones, so scales have to follow the values: x has one a row,
+// and G goes out twice, for dw with one for each word and tile of rows (the
+// words of a large vocabulary differ by 1e12 and more in probability, and
+// each has a gradient of its own), for dx with one for each row.  w has one a
+// row in the forward and a single one in the backward: dx is off by up to
+// 2^-38 of the row's |g| max |w| where its own terms are smaller.
 //
 // Rows whose label is ignored are read as zeros, so what lies in them (a
 // padded batch's garbage, NaN) reaches no gradient.
