@@ -224,3 +224,18 @@ def test_fp32_every_tile_of_both_gradients(n, v, d):
     up = 10.0 ** torch.linspace(3, -12, n, device='cuda')
     x *= 10.0 ** torch.linspace(-3, 0, n, device='cuda')[:, None]
     _gradients_inside(x, w, b, y, up)
+
+
+@GPU
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_the_most_rows(dtype):
+    """2^20 rows: a piece is 256 words, of which G takes up to 1 GB twice.
+    (dw is a sum of 2^20 terms, whose order the bound allows for.)"""
+    n, v, d = 1 << 20, 300, 16
+    g = torch.Generator(device='cuda').manual_seed(7)
+    x = torch.randn(n, d, generator=g, device='cuda').to(dtype)
+    w = torch.randn(v, d, generator=g, device='cuda').to(dtype)
+    b = torch.randn(v, generator=g, device='cuda').to(dtype)
+    y = torch.randint(0, v, (n,), generator=g, device='cuda')
+    up = torch.rand(n, generator=g, device='cuda') * 2.0 ** -20
+    _gradients_inside(x, w, b, y, up)
